@@ -1,0 +1,267 @@
+// Shared parts of the encoder attention kernels (encoder_attn_*_kernels.hip): arguments, operand fragments, tile staging,
+// key validity, relative positions.
+//
+// One family of kernels serves both operators.  With M maps per head (M = 1: softmax attention with a relative position
+// bias, M = 2: two-map "differential" attention), head h of sample b computes
+//     x_m[i][j] = scale q_m[i] . k_m[j] + T[bucket(pos(j) - pos(i))][h M + m],   P_m = softmax_j(x_m),
+//     o[i] = sum_j P_1[i][j] v[j]                     (M = 1, values D wide)
+//     o[i] = sum_j (P_1 - lam_h P_2)[i][j] v[j]       (M = 2, values 2 D wide)
+// and its gradients.  Exponentials are base 2 throughout (scale and bias are multiplied by log2 e in 32 bits, after the
+// matrix product, so no operand is rounded a second time).
+//
+// Matrix operands.  bf16 rows use v_mfma_f32_16x16x32_bf16 as they are; fp32 rows use v_mfma_f32_16x16x4_f32, true fp32
+// products: three bf16 passes over (hi, lo) splits carry 16 bits per operand, 30 times the rounding of an fp32 product.
+// A fragment covers kDims values of the contraction: lane (l15 = lane & 15, q4 = lane >> 4) holds, for row / column l15,
+//   bf16: values 8 q4 .. 8 q4 + 7 of 32;   fp32: values 4 q4 .. 4 q4 + 3 of 16 (four 4-deep instructions, one value each);
+// an accumulator gives the lane C[4 q4 + j][l15], j = 0..3.  With the owned rows (queries in the forward and the dQ pass,
+// keys in the dK / dV pass) as COLUMNS of every product, softmax sums stay inside a lane plus one exchange over q4, and
+// an accumulator (two of them for bf16) is the B fragment of the product that follows, without any exchange: the
+// contraction order it implies is 4 q4 + e (+ 16 for the second half), which tr_frag reads from LDS.
+#pragma once
+#include "common.hpp"
+
+namespace atrihip {
+
+struct EncAttnArgs {
+  const void* q;       // [B, Lq, H M, D] by strides
+  const void* k;       // [B, Lk, KV M, D]
+  const void* v;       // [B, Lk, KV, DV]
+  const void* dout;    // [B, Lq, H, DV]
+  void* out;           // [B, Lq, H, DV]
+  void* dq;
+  void* dk;
+  void* dv;
+  const float* table;  // [buckets, H M]; nullptr: no position bias
+  const int* lut;      // [2 R + 1] bucket of every clamped position difference
+  const float* lam;    // [H] (M = 2)
+  const unsigned long long* words;  // [B, ceil(Lk / 64)] validity bit of every key; nullptr: all keys
+  const int* qoff;     // [B] position of the first query, nullptr: q0 for all samples
+  float* stat;         // [M, B H Lq, 2] row maximum (log2 domain; +inf: no key) and 1 / sum (0: no key); nullptr: not wanted
+  float* o32;          // [M] x [B, Lq, H, DV] per-map outputs in 32 bits by strides (backward: their product with dO is delta)
+  float* delta;        // [M, B H Lq]
+  float* part_o;       // [splits, M, B H Lq, DV] unnormalised partial outputs (splits > 1)
+  float* part_ml;      // [splits, M, B H Lq, 2] their maxima and sums
+  float* hist;         // [B H ceil(Lq / queries per workgroup), M, 2 R + 1] partial sums of dS by position difference; nullptr: not wanted
+  long long qs[3], ks[3], vs[3], os[3], gs[3], dqs[3], dks[3], dvs[3];  // element strides: sample, token, head
+  long long o32s[4];   // o32: sample, token, head, map
+  int B, Lq, Lk, H, KV, D, DV, M;
+  int R, W, q0;        // clamp of the position difference; board width (0: sequence); position of the first query
+  int bf16, splits, hist_rows;
+  float scale;
+};
+
+typedef __attribute__((ext_vector_type(4))) short short4v;
+
+constexpr float kLog2E = 1.4426950408889634f;
+constexpr int kTile = 64;  // keys (queries in the dK / dV pass) staged per step
+
+template <typename T>
+struct Ops;
+
+template <>
+struct Ops<unsigned short> {
+  using Frag = short8;
+  static constexpr int kDims = 32;   // contraction values per fragment
+  static constexpr int kVec = 8;     // elements per 16 bytes
+  static constexpr int kSub = 2;     // 16-row accumulators per B fragment
+  static constexpr int row_pitch(int d) { return d + 8; }   // 16-lane b128 row reads: all 64 banks once
+  static constexpr int tr_pitch(int d) { return d + 16; }   // transposing reads: eight 32-byte rows on distinct banks
+  static __device__ __forceinline__ Frag zero() { return Frag{}; }
+  static __device__ __forceinline__ Frag row_frag(const unsigned short* t, int pitch, int row, int c, int q4) {
+    return *reinterpret_cast<const short8*>(t + row * pitch + c * 32 + q4 * 8);
+  }
+  // A fragment of the transpose: column n 16 + l15 of rows 32 kb + 4 q4 + e and 32 kb + 16 + 4 q4 + e, e = 0..3.  A 16-lane
+  // group of the transposing read takes four rows of 16 values; the lane supplies the address of a quarter row.
+  static __device__ __forceinline__ Frag tr_frag(const unsigned short* t, int pitch, int kb, int n, int l15, int q4) {
+    typedef __attribute__((address_space(3))) short4v* lds4;
+    unsigned short* p = const_cast<unsigned short*>(t) + (kb * 32 + 4 * q4 + (l15 >> 2)) * pitch + n * 16 + (l15 & 3) * 4;
+    const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
+    const short4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 16 * pitch));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  static __device__ __forceinline__ Frag acc_frag(const float4v* s) {  // probabilities and score gradients: rounded to bf16 like the operand they meet
+    return pack_bf16x8(s[0][0], s[0][1], s[0][2], s[0][3], s[1][0], s[1][1], s[1][2], s[1][3]);
+  }
+  static __device__ __forceinline__ float4v mma(const Frag& a, const Frag& b, float4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  // s -= value(f): what the next of several fragments of the same values has to carry.
+  static __device__ __forceinline__ void take(float4v* s, const Frag& f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e >> 2][e & 3] -= bf16_to_float((unsigned short)f[e]);
+  }
+  static __device__ __forceinline__ float dot(const Frag& a, const float* o) {
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(bf16_to_float((unsigned short)a[e]), o[e], s);
+    return s;
+  }
+  static __device__ __forceinline__ void store4(unsigned short* p, float a, float b, float c, float d) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
+  }
+};
+
+template <>
+struct Ops<float> {
+  using Frag = float4v;
+  static constexpr int kDims = 16;
+  static constexpr int kVec = 4;
+  static constexpr int kSub = 1;
+  static constexpr int row_pitch(int d) { return d + 4; }
+  static constexpr int tr_pitch(int d) { return d + 4; }
+  static __device__ __forceinline__ Frag zero() { return Frag{}; }
+  static __device__ __forceinline__ Frag row_frag(const float* t, int pitch, int row, int c, int q4) {
+    return *reinterpret_cast<const float4v*>(t + row * pitch + c * 16 + q4 * 4);
+  }
+  static __device__ __forceinline__ Frag tr_frag(const float* t, int pitch, int kb, int n, int l15, int q4) {
+    const float* p = t + (kb * 16 + 4 * q4) * pitch + n * 16 + l15;
+    return Frag{p[0], p[pitch], p[2 * pitch], p[3 * pitch]};
+  }
+  static __device__ __forceinline__ Frag acc_frag(const float4v* s) { return s[0]; }
+  static __device__ __forceinline__ void take(float4v*, const Frag&) {}
+  static __device__ __forceinline__ float4v mma(const Frag& a, const Frag& b, float4v c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ float dot(const Frag& a, const float* o) {
+    return fmaf(a[0], o[0], fmaf(a[1], o[1], fmaf(a[2], o[2], a[3] * o[3])));
+  }
+  static __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
+    *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+  }
+};
+
+// Consecutive logical workgroups on the same XCD (the hardware deals blockIdx out round robin over eight), so that the query
+// tiles of one (sample, head), and the heads that share keys, meet in one L2.
+__device__ __forceinline__ int xcd_order(int id, int n) {
+  const int per = n >> 3, extra = n & 7, xcd = id & 7, slot = id >> 3;
+  return xcd * per + (xcd < extra ? xcd : extra) + slot;
+}
+
+// Position of token t: its index, or on a W-wide board r (2 W - 1) + c, whose differences name (dr, dc) uniquely.
+__device__ __forceinline__ int token_pos(int t, int W) { return W > 0 ? t + (t / W) * (W - 1) : t; }
+__device__ __forceinline__ int query_origin(const EncAttnArgs& a, int b) {
+  const int o = a.qoff ? a.qoff[b] : a.q0;
+  return o < -(1 << 29) ? -(1 << 29) : o > (1 << 29) ? (1 << 29) : o;  // differences stay within 32 bits
+}
+__device__ __forceinline__ int clamp_slot(int d, int R2) { return d < 0 ? 0 : d > R2 ? R2 : d; }
+
+// log2 e times the bias; a finite bias stays finite (a table may hold the type's lowest value as a mask).
+__device__ __forceinline__ float bias_log2(float t) {
+  const float x = t * kLog2E;
+  if (__builtin_isinf(x) && !__builtin_isinf(t)) return copysignf(3.4028234663852886e38f, t);
+  return x;
+}
+__device__ __forceinline__ void fill_bias(const EncAttnArgs& a, float* bias, int head, int M, int tid) {
+  const int n = 2 * a.R + 1, hm = a.H * M;
+  for (int i = tid; i < n; i += 256) {
+    const float* row = a.table + (size_t)a.lut[i] * hm + head * M;
+    for (int m = 0; m < M; ++m) bias[m * n + i] = bias_log2(row[m]);
+  }
+}
+
+// Rows [t0, t0 + 64) of a [tokens, D] matrix on their way from memory to LDS: 16 bytes per thread and step, zeros where the row's
+// bit in `word` is clear (whatever the masked row holds) and beyond the matrix's width.
+template <typename T, int D>
+struct Stage {
+  static constexpr int kVecsPerRow = D / Ops<T>::kVec;
+  static constexpr int kN = kTile * kVecsPerRow / 256;
+  uint4 r[kN];
+  __device__ __forceinline__ void load(const T* base, long long pitch, int t0, unsigned long long word, int width, int tid) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int vi = tid + i * 256, row = vi / kVecsPerRow, col = (vi % kVecsPerRow) * Ops<T>::kVec;
+      r[i] = make_uint4(0, 0, 0, 0);
+      if (((word >> row) & 1) && col < width) r[i] = *reinterpret_cast<const uint4*>(base + (long long)(t0 + row) * pitch + col);
+    }
+  }
+  __device__ __forceinline__ void store(T* lds, int pitch, int tid) const {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int vi = tid + i * 256, row = vi / kVecsPerRow, col = (vi % kVecsPerRow) * Ops<T>::kVec;
+      *reinterpret_cast<uint4*>(lds + row * pitch + col) = r[i];
+    }
+  }
+};
+
+// Row fragments of up to 16 owned tokens straight from memory (each value is read by one lane).
+template <typename T, int C>
+__device__ __forceinline__ void load_rows(typename Ops<T>::Frag (&f)[C], const T* row, bool valid, int width, int q4) {
+  using Frag = typename Ops<T>::Frag;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int col = c * Ops<T>::kDims + q4 * Ops<T>::kVec;
+    f[c] = Ops<T>::zero();
+    if (valid && col < width) f[c] = *reinterpret_cast<const Frag*>(row + col);
+  }
+}
+
+__device__ __forceinline__ unsigned long long range_word(int t0, int L) {  // bits of rows t0 .. t0 + 63 that are below L
+  const int n = L - t0;
+  return n >= 64 ? ~0ULL : n <= 0 ? 0ULL : ((1ULL << n) - 1);
+}
+
+// The key tiles of one sample that hold a valid key, in order.  64 words are held across the wave at a time; every wave of a
+// workgroup walks the same list.
+struct TileWalk {
+  const unsigned long long* words;
+  int Lk, end, base;
+  unsigned long long mine, live, word;
+  __device__ __forceinline__ void start(const unsigned long long* w, int lk, int first, int last) {
+    words = w; Lk = lk; end = last; base = first - 64; live = 0; word = 0; mine = 0;
+    if (!w) base = first - 1;
+  }
+  // Next tile with a valid key (its bits in `word`), or `end`.
+  __device__ __forceinline__ int next() {
+    if (!words) {
+      ++base;
+      word = base < end ? range_word(base * kTile, Lk) : 0;
+      return base;
+    }
+    while (!live) {
+      base += 64;
+      if (base >= end) return end;
+      const int lane = threadIdx.x & 63;
+      mine = base + lane < end ? words[base + lane] : 0;
+      live = __ballot(mine != 0);
+    }
+    const int i = __ffsll((unsigned long long)live) - 1;
+    live &= live - 1;
+    const unsigned lo = __builtin_amdgcn_readlane((unsigned)mine, i), hi = __builtin_amdgcn_readlane((unsigned)(mine >> 32), i);
+    word = ((unsigned long long)hi << 32) | lo;
+    return base + i;
+  }
+};
+
+// Bias of a 16-query column against a 64-key tile when every difference is clamped the same way (long sequences).
+// -1: all below, +1: all above, 0: mixed.
+__device__ __forceinline__ int clamped_side(const EncAttnArgs& a, int kmin, int kmax, int qmin, int qmax) {
+  if (a.W > 0) return 0;
+  return kmin - qmax >= a.R ? 1 : kmax - qmin <= -a.R ? -1 : 0;
+}
+
+inline int enc_check(const EncAttnArgs& a) {
+  if (a.B < 1 || a.Lq < 1 || a.Lk < 1 || a.H < 1 || a.KV < 1 || a.H % a.KV != 0) return -10;
+  if (a.M < 1 || a.M > 2 || a.D < 8 || a.D % 8 != 0 || a.D > (a.M == 1 ? 128 : 64) || a.DV != a.D * a.M) return -11;
+  if (a.table && (a.R < 0 || a.R > 2047 || a.lut == nullptr)) return -12;
+  if (a.M == 1 && !a.table) return -13;
+  if (a.M == 2 && !a.lam) return -14;
+  if ((long long)a.B * a.H * ((a.Lq + 63) / 64) * (a.splits < 1 ? 1 : a.splits) >= (1LL << 31)) return -15;
+  if ((long long)a.B * a.KV * ((a.Lk + 63) / 64) >= (1LL << 31)) return -15;
+  if (a.Lq > (1 << 29) || a.Lk > (1 << 29)) return -16;
+  return 0;
+}
+// The padded head width a kernel is built for.
+inline int enc_width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+
+constexpr size_t kMaxLds = 160 * 1024;
+
+// Raises a kernel's dynamic LDS limit (attribute of the function on the current device) and reports what does not fit.
+template <typename F>
+inline int enc_lds(F* fn, size_t bytes) {
+  if (bytes > kMaxLds) return -20;
+  return hip_err(hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+}
+
+}  // namespace atrihip

@@ -1,0 +1,371 @@
+// Forward pass of the encoder attention operators (see encoder_attn.hpp for the mathematics and the operand layout), the
+// join of key splits, and the key-validity words.
+#include "encoder_attn.hpp"
+
+using namespace atrihip;
+
+namespace {
+
+// One 4-wave workgroup per (sample, head, 64 QS queries[, key split]); a wave owns 16 QS queries and walks the key tiles with the
+// running maximum and sum of the softmax; per lane the sum is partial (its own keys) until the end.
+// PL bf16 fragments per probability: one for inference (rounded like the values it meets); three, all 24 bits, when a backward
+// pass follows, for delta = dO . o has to match dP = dO V^T to 32 bits: the gradients of the table and of lam are sums
+// of p (dP - delta) in which everything but the error of delta cancels (with one fragment they were 1e-3 off).
+template <typename T, int D, int M, int QS, bool BIAS, int PL>
+__global__ __launch_bounds__(256) void enc_attn_fwd_kernel(EncAttnArgs a) {
+  using O = Ops<T>;
+  using Frag = typename O::Frag;
+  constexpr int DV = D * M, DC = D / O::kDims, NV = DV / 16, NKB = 4 / O::kSub;
+  constexpr int PK = O::row_pitch(D), PV = O::tr_pitch(DV);
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  T* k_lds = reinterpret_cast<T*>(smem);
+  T* v_lds = k_lds + M * kTile * PK;
+  int* pos_lds = reinterpret_cast<int*>(v_lds + kTile * PV);
+  float* bias_lds = reinterpret_cast<float*>(pos_lds + kTile);
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, q4 = lane >> 4;
+  const int nqt = (a.Lq + 64 * QS - 1) / (64 * QS);
+  int id = xcd_order(blockIdx.x, gridDim.x);
+  const int qt = id % nqt;
+  id /= nqt;
+  const int split = id % a.splits, bh = id / a.splits;
+  const int b = bh / a.H, h = bh - b * a.H, kvh = h / (a.H / a.KV);
+  const int tiles = (a.Lk + kTile - 1) / kTile;
+  const int per = (tiles + a.splits - 1) / a.splits;
+  const int t_first = split * per, t_last = t_first + per < tiles ? t_first + per : tiles;
+
+  const T* kb_ = reinterpret_cast<const T*>(a.k) + b * a.ks[0] + (long long)kvh * M * a.ks[2];
+  const T* vb_ = reinterpret_cast<const T*>(a.v) + b * a.vs[0] + kvh * a.vs[2];
+  const int R2 = 2 * a.R;
+  if constexpr (BIAS) fill_bias(a, bias_lds, h, M, tid);
+
+  const int q_first = (qt * 4 + wave) * 16 * QS;
+  const bool busy = q_first < a.Lq;  // wave-uniform
+  const int origin = BIAS ? query_origin(a, b) : 0;
+  Frag qf[M][QS][DC];
+  int pos_q[QS];
+#pragma unroll
+  for (int s = 0; s < QS; ++s) {
+    const int query = q_first + s * 16 + l15;
+    pos_q[s] = BIAS ? token_pos(query, a.W) + origin : 0;
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+      load_rows<T, DC>(qf[m][s], reinterpret_cast<const T*>(a.q) + b * a.qs[0] + (long long)query * a.qs[1] + (long long)(h * M + m) * a.qs[2],
+                       query < a.Lq, a.D, q4);
+  }
+  float4v o[M][QS][NV];
+  float run_max[M][QS], run_sum[M][QS];
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int s = 0; s < QS; ++s) {
+      run_max[m][s] = -INFINITY;
+      run_sum[m][s] = 0.f;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) o[m][s][n] = float4v{0.f, 0.f, 0.f, 0.f};
+    }
+  const float sl2 = a.scale * kLog2E;
+
+  Stage<T, D> sk[M];
+  Stage<T, DV> sv;
+  TileWalk walk;
+  walk.start(a.words ? a.words + (size_t)b * tiles : nullptr, a.Lk, t_first, t_last);
+  int t = walk.next();
+  if (t < t_last) {
+#pragma unroll
+    for (int m = 0; m < M; ++m) sk[m].load(kb_ + m * a.ks[2], a.ks[1], t * kTile, walk.word, a.D, tid);
+    sv.load(vb_, a.vs[1], t * kTile, walk.word, a.DV, tid);
+  }
+  while (t < t_last) {
+    const unsigned long long word = walk.word;
+    const int t0 = t * kTile;
+    __syncthreads();  // every wave is past its reads of the previous tile
+#pragma unroll
+    for (int m = 0; m < M; ++m) sk[m].store(k_lds + m * kTile * PK, PK, tid);
+    sv.store(v_lds, PV, tid);
+    if (BIAS && tid < kTile) pos_lds[tid] = token_pos(t0 + tid, a.W);
+    __syncthreads();
+    t = walk.next();
+    if (t < t_last) {  // the next tile's loads run under this tile's products
+#pragma unroll
+      for (int m = 0; m < M; ++m) sk[m].load(kb_ + m * a.ks[2], a.ks[1], t * kTile, walk.word, a.D, tid);
+      sv.load(vb_, a.vs[1], t * kTile, walk.word, a.DV, tid);
+    }
+    if (!busy) continue;
+
+    float4v st[M][QS][4];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+        for (int s = 0; s < QS; ++s) st[m][s][kt] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+          const Frag kf = O::row_frag(k_lds + m * kTile * PK, PK, kt * 16 + l15, c, q4);
+#pragma unroll
+          for (int s = 0; s < QS; ++s) st[m][s][kt] = O::mma(kf, qf[m][s][c], st[m][s][kt]);
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < QS; ++s) {
+        float4v* x = st[m][s];
+        if constexpr (BIAS) {
+          const float* bias = bias_lds + m * (R2 + 1);
+          const int qa = q_first + s * 16 + origin;
+          const int side = clamped_side(a, t0, t0 + kTile - 1, qa, qa + 15);
+          if (side != 0) {
+            const float c = bias[side > 0 ? R2 : 0];
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) x[kt][j] = fmaf(x[kt][j], sl2, c);
+          } else {
+            const int off = a.R - pos_q[s];
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) {
+              const int4 p = *reinterpret_cast<const int4*>(pos_lds + kt * 16 + q4 * 4);
+              const int pj[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) x[kt][j] = fmaf(x[kt][j], sl2, bias[clamp_slot(pj[j] + off, R2)]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[kt][j] *= sl2;
+        }
+        if (word != ~0ULL) {
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt) {
+            const unsigned bits = (unsigned)(word >> (kt * 16 + q4 * 4));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[kt][j] = (bits >> j) & 1 ? x[kt][j] : -INFINITY;
+          }
+        }
+        float top = run_max[m][s];
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top = fmaxf(top, x[kt][j]);
+        top = quad_row_max(top);
+        const float base = top == -INFINITY ? 0.f : top;  // nothing seen yet: exp2(-inf - 0) = 0, never inf - inf
+        const float fade = __builtin_amdgcn_exp2f(run_max[m][s] - base);
+        run_max[m][s] = top;
+        float sum = 0.f;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[kt][j] = __builtin_amdgcn_exp2f(x[kt][j] - base);
+            sum += x[kt][j];
+          }
+        run_sum[m][s] = fmaf(run_sum[m][s], fade, sum);
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[m][s][n][j] *= fade;
+      }
+    }
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) {
+      Frag pf[M][QS][PL];
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int s = 0; s < QS; ++s)
+#pragma unroll
+          for (int p = 0; p < PL; ++p) {
+            pf[m][s][p] = O::acc_frag(&st[m][s][kb * O::kSub]);
+            if (p + 1 < PL) O::take(&st[m][s][kb * O::kSub], pf[m][s][p]);
+          }
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const Frag vf = O::tr_frag(v_lds, PV, kb, n, l15, q4);
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int s = 0; s < QS; ++s)
+#pragma unroll
+            for (int p = PL - 1; p >= 0; --p) o[m][s][n] = O::mma(vf, pf[m][s][p], o[m][s][n]);
+      }
+    }
+  }
+  if (!busy) return;
+
+  const long long rows = (long long)a.B * a.H * a.Lq;
+  const float lam = M == 2 ? a.lam[h] : 0.f;
+#pragma unroll
+  for (int s = 0; s < QS; ++s) {
+    const int query = q_first + s * 16 + l15;
+    float inv[M];
+    const long long row = (long long)bh * a.Lq + query;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const float sum = quad_row_sum(run_sum[m][s]);
+      inv[m] = sum == 0.f ? 0.f : 1.0f / sum;
+      if (query < a.Lq && q4 == 0) {
+        if (a.splits > 1) {
+          float* ml = a.part_ml + 2 * (((long long)split * M + m) * rows + row);
+          ml[0] = run_max[m][s];
+          ml[1] = sum;
+        } else if (a.stat) {
+          *reinterpret_cast<float2*>(a.stat + 2 * (m * rows + row)) = make_float2(sum == 0.f ? INFINITY : run_max[m][s], inv[m]);
+        }
+      }
+    }
+    if (query >= a.Lq) continue;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int dim = n * 16 + q4 * 4;
+      if (dim >= a.DV) continue;
+      float4v r[M];
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        r[m] = o[m][s][n];
+        if (a.splits > 1) {
+          Ops<float>::store4(a.part_o + (((long long)split * M + m) * rows + row) * a.DV + dim, r[m][0], r[m][1], r[m][2], r[m][3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) r[m][j] *= inv[m];
+          if (a.o32) Ops<float>::store4(a.o32 + b * a.o32s[0] + (long long)query * a.o32s[1] + h * a.o32s[2] + m * a.o32s[3] + dim, r[m][0], r[m][1], r[m][2], r[m][3]);
+        }
+      }
+      if (a.splits > 1) continue;
+      if constexpr (M == 2) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[0][j] = fmaf(-lam, r[1][j], r[0][j]);
+      }
+      O::store4(reinterpret_cast<T*>(a.out) + b * a.os[0] + (long long)query * a.os[1] + h * a.os[2] + dim, r[0][0], r[0][1], r[0][2], r[0][3]);
+    }
+  }
+}
+
+// Joins the partial softmaxes of `splits` key ranges: one thread per four output values of a row.
+template <typename T, int M>
+__global__ __launch_bounds__(256) void enc_attn_join_kernel(EncAttnArgs a) {
+  const long long rows = (long long)a.B * a.H * a.Lq;
+  const int quads = a.DV / 4;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * quads) return;
+  const long long row = i / quads;
+  const int dim = (int)(i - row * quads) * 4;
+  const int query = (int)(row % a.Lq);
+  const long long bh = row / a.Lq;
+  const int b = (int)(bh / a.H), h = (int)(bh - (long long)b * a.H);
+  float4v r[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    const float* ml = a.part_ml + 2 * (m * rows + row);
+    const float* po = a.part_o + (m * rows + row) * a.DV + dim;
+    const long long step = (long long)M * rows;
+    float top = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[2 * s * step]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    float4v acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; ++s) {
+      const float w = __builtin_amdgcn_exp2f(ml[2 * s * step] - base);
+      const float4v p = *reinterpret_cast<const float4v*>(po + s * step * a.DV);
+      sum = fmaf(ml[2 * s * step + 1], w, sum);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = fmaf(p[j], w, acc[j]);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[m][j] = acc[j] * inv;
+    if (a.stat && dim == 0) *reinterpret_cast<float2*>(a.stat + 2 * (m * rows + row)) = make_float2(sum == 0.f ? INFINITY : top, inv);
+    if (a.o32) Ops<float>::store4(a.o32 + b * a.o32s[0] + (long long)query * a.o32s[1] + h * a.o32s[2] + m * a.o32s[3] + dim, r[m][0], r[m][1], r[m][2], r[m][3]);
+  }
+  if constexpr (M == 2) {
+    const float lam = a.lam[h];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[0][j] = fmaf(-lam, r[1][j], r[0][j]);
+  }
+  Ops<T>::store4(reinterpret_cast<T*>(a.out) + b * a.os[0] + (long long)query * a.os[1] + h * a.os[2] + dim, r[0][0], r[0][1], r[0][2], r[0][3]);
+}
+
+// One 64-bit word per 64 keys of a byte mask [B, Lk] (strides in bytes); one wave per word.
+__global__ __launch_bounds__(256) void key_words_kernel(const unsigned char* mask, long long sb, long long sk, unsigned long long* words, int B, int Lk) {
+  const int tiles = (Lk + 63) / 64;
+  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (w >= (long long)B * tiles) return;
+  const int b = (int)(w / tiles), key = (int)(w - (long long)b * tiles) * 64 + (threadIdx.x & 63);
+  const bool on = key < Lk && mask[b * sb + key * sk] != 0;
+  const unsigned long long bits = __ballot(on);
+  if ((threadIdx.x & 63) == 0) words[w] = bits;
+}
+
+template <typename T, int D, int M, int QS, bool BIAS, int PL>
+int launch_fwd_planes(const EncAttnArgs& a, hipStream_t stream) {
+  using O = Ops<T>;
+  size_t lds = sizeof(T) * (size_t)kTile * (M * O::row_pitch(D) + O::tr_pitch(D * M)) + kTile * sizeof(int);
+  if (BIAS) lds += sizeof(float) * (size_t)M * (2 * a.R + 1);
+  const int rc = enc_lds(enc_attn_fwd_kernel<T, D, M, QS, BIAS, PL>, lds);
+  if (rc) return rc;
+  const int nqt = (a.Lq + 64 * QS - 1) / (64 * QS);
+  hipLaunchKernelGGL((enc_attn_fwd_kernel<T, D, M, QS, BIAS, PL>), dim3((unsigned)(a.B * a.H * nqt * a.splits)), dim3(256), lds, stream, a);
+  return hip_err(hipGetLastError());
+}
+
+template <typename T, int D, int M, int QS, bool BIAS>
+int launch_fwd(const EncAttnArgs& a, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    if (a.o32) return launch_fwd_planes<T, D, M, QS, BIAS, 3>(a, stream);
+  }
+  return launch_fwd_planes<T, D, M, QS, BIAS, 1>(a, stream);
+}
+
+template <typename T>
+int dispatch_fwd(const EncAttnArgs& a, hipStream_t stream) {
+  const int w = enc_width(a.D);
+  if (a.M == 1) {
+    const bool wide = a.Lq > 64;  // two query tiles per wave once they exist: every staged fragment feeds two products
+    if (w == 32) return wide ? launch_fwd<T, 32, 1, 2, true>(a, stream) : launch_fwd<T, 32, 1, 1, true>(a, stream);
+    if (w == 64) return wide ? launch_fwd<T, 64, 1, 2, true>(a, stream) : launch_fwd<T, 64, 1, 1, true>(a, stream);
+    return launch_fwd<T, 128, 1, 1, true>(a, stream);
+  }
+  if (w == 32) return a.table ? launch_fwd<T, 32, 2, 1, true>(a, stream) : launch_fwd<T, 32, 2, 1, false>(a, stream);
+  return a.table ? launch_fwd<T, 64, 2, 1, true>(a, stream) : launch_fwd<T, 64, 2, 1, false>(a, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int atri_sizeof_encattn() { return (int)sizeof(EncAttnArgs); }
+
+// Validity words [B, ceil(Lk / 64)] of a byte mask (nonzero: the key takes part), element strides sb / sk.
+int atri_enc_key_words(const void* mask, long long sb, long long sk, void* words, int B, int Lk, hipStream_t stream) {
+  if (B < 1 || Lk < 1 || !mask || !words) return -10;
+  const long long n = (long long)B * ((Lk + 63) / 64);
+  if ((n + 3) / 4 >= (1LL << 31)) return -15;
+  hipLaunchKernelGGL(key_words_kernel, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, stream, reinterpret_cast<const unsigned char*>(mask), sb, sk,
+                     reinterpret_cast<unsigned long long*>(words), B, Lk);
+  return hip_err(hipGetLastError());
+}
+
+// out (and, where the pointers are set, stat and o32) of one attention call.
+int atri_enc_attn_fwd(const EncAttnArgs* args, hipStream_t stream) {
+  if (!args) return -1;
+  const EncAttnArgs& a = *args;
+  const int rc = enc_check(a);
+  if (rc) return rc;
+  if (!a.q || !a.k || !a.v || !a.out || a.splits < 1 || (a.splits > 1 && (!a.part_o || !a.part_ml))) return -17;
+  const int rc2 = a.bf16 ? dispatch_fwd<unsigned short>(a, stream) : dispatch_fwd<float>(a, stream);
+  if (rc2 || a.splits == 1) return rc2;
+  const long long n = (long long)a.B * a.H * a.Lq * (a.DV / 4);
+  if ((n + 255) / 256 >= (1LL << 31)) return -15;
+  const dim3 grid((unsigned)((n + 255) / 256));
+  if (a.bf16) {
+    if (a.M == 1) hipLaunchKernelGGL((enc_attn_join_kernel<unsigned short, 1>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((enc_attn_join_kernel<unsigned short, 2>), grid, dim3(256), 0, stream, a);
+  } else {
+    if (a.M == 1) hipLaunchKernelGGL((enc_attn_join_kernel<float, 1>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((enc_attn_join_kernel<float, 2>), grid, dim3(256), 0, stream, a);
+  }
+  return hip_err(hipGetLastError());
+}
+
+}  // extern "C"

@@ -1,0 +1,328 @@
+"""Encoder attention operators (relative position bias, two maps) on the GPU against the same formulas in 64 bits."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U32, U16 = 2.0**-24, 2.0**-8  # half a step of fp32 / bf16, relative
+
+
+def _tol(dtype: torch.dtype, d: int, lq: int, lk: int) -> float:
+    """Relative 2-norm error allowed on an output or gradient.
+
+    fp32: rounding errors of a sum of n products grow like sqrt(n) u; a score (n = d) enters exponentially, the sums
+    over keys / queries follow, and a gradient passes through two such chains: u (8 sqrt(d) + 8 sqrt(max(lq, lk)) + 64).
+    bf16: one rounding of the probability (or score gradient) that meets the other operand, one of the result: 2 * 2^-8;
+    the 32-bit part above is far below."""
+    wide = U32 * (8 * math.sqrt(d) + 8 * math.sqrt(max(lq, lk)) + 64)
+    return wide if dtype == torch.float32 else 2 * U16 + wide
+
+
+def _rel(x: torch.Tensor, y: torch.Tensor) -> float:
+    y = y.double()
+    y = y.detach()
+    n = float(y.norm())
+    e = float((x.detach().double() - y).norm())
+    return e / n if n else e
+
+
+def _inputs(dtype, maps, b, lq, lk, h, kv, d, buckets, seed=0, std=1.0):  # noqa: ANN001
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def r(*s, dt=dtype, m=1.0):  # noqa: ANN002
+        return (torch.randn(*s, generator=g, device="cuda") * m).to(dt)
+
+    return {
+        "q": r(b, lq, h * maps, d, m=std), "k": r(b, lk, kv * maps, d, m=std), "v": r(b, lk, kv, d * maps),
+        "table": r(buckets.num_buckets, h * maps, dt=torch.float32, m=0.5) if buckets else None,
+        "lam": (torch.rand(h, generator=g, device="cuda") * 0.6 + 0.1) if maps == 2 else None,
+        "dout": r(b, lq, h, d * maps),
+    }
+
+
+def _call(t, buckets, mask, off):  # noqa: ANN001
+    from alphatriangle_amd.ops import attention as A
+
+    if t["lam"] is None:
+        return A.relative_attention(t["q"], t["k"], t["v"], t["table"], buckets, key_mask=mask, query_offset=off)
+    return A.differential_attention(t["q"], t["k"], t["v"], t["lam"], t["table"], buckets, key_mask=mask, query_offset=off)
+
+
+def _compare(inp, buckets, mask=None, off=0):  # noqa: ANN001
+    from alphatriangle_amd.ops.attention import attention_reference
+
+    names = [n for n in ("q", "k", "v", "table", "lam") if inp[n] is not None]
+    t = dict(inp)
+    for n in names:
+        t[n] = inp[n].detach().clone().requires_grad_(True)
+    out = _call(t, buckets, mask, off)
+    grads = torch.autograd.grad(out, [t[n] for n in names], inp["dout"])
+    with torch.no_grad():
+        plain = _call(inp, buckets, mask, off)
+    w = {n: (inp[n].double().requires_grad_(True) if n in names else None) for n in ("q", "k", "v", "table", "lam")}
+    ref = attention_reference(w["q"], w["k"], w["v"], w["lam"], w["table"], buckets, mask, inp["q"].shape[3] ** -0.5, off)
+    rg = torch.autograd.grad(ref, [w[n] for n in names], inp["dout"].double())
+    torch.cuda.synchronize()
+    one_bucket = buckets is not None and buckets.pairs(inp["q"].shape[1], inp["k"].shape[1], off).unique().numel() == 1
+    dt, d, lq, lk = inp["q"].dtype, inp["q"].shape[3], inp["q"].shape[1], inp["k"].shape[1]
+    if dt == torch.float32:
+        assert torch.equal(plain, out), "with and without a backward pass to come"
+    assert _rel(plain, ref) <= _tol(dt, d, lq, lk), ("out without gradients", _rel(plain, ref))
+    assert _rel(out, ref) <= _tol(dt, d, lq, lk), ("out", _rel(out, ref))
+    for n, g, e in zip(names, grads, rg):
+        assert g.dtype == t[n].dtype and g.shape == t[n].shape
+        # sums over every pair whose terms cancel (softmax gradients add up to zero in a row): 16 times the room
+        tol = 16 * _tol(torch.float32, d, lq, lk) if n in ("table", "lam") else _tol(dt, d, lq, lk)
+        if (lk == 1 and n in ("q", "k", "table")) or (n == "table" and one_bucket):
+            # zero by definition (a row's score gradients add up to delta - delta): what is left are roundings of the terms
+            # p (dP - delta), |dP| <= sum |dO| |v|, over the rows that meet in one value
+            rows = inp["dout"].shape[0] * lq
+            assert float((g.double() - e).abs().max()) <= 64 * U32 * d * float(inp["dout"].abs().max()) * rows
+        else:
+            assert _rel(g, e) <= tol, (n, _rel(g, e), tol)
+    return out, dict(zip(names, grads))
+
+
+def _plan(kind):  # noqa: ANN001
+    from alphatriangle_amd.ops.attention import RelativeBuckets
+
+    if kind is None:
+        return None
+    return RelativeBuckets.board(*kind, device="cuda") if isinstance(kind, tuple) else RelativeBuckets.log(32, kind, device="cuda")
+
+
+BOTH = [torch.float32, torch.bfloat16]
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("maps,d", [(1, 8), (1, 32), (1, 40), (1, 64), (1, 96), (1, 128), (2, 8), (2, 32), (2, 48), (2, 64)])
+def test_head_widths(dtype, maps, d):
+    b, l, h = 2, 97, 3
+    _compare(_inputs(dtype, maps, b, l, l, h, h, d, _plan(20)), _plan(20))
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("lq,lk", [(1, 1), (1, 2), (2, 1), (1, 64), (16, 17), (63, 65), (64, 64), (65, 63), (128, 129), (1, 700), (130, 700), (700, 5)])
+def test_lengths(dtype, maps, lq, lk):
+    p = _plan(128)
+    _compare(_inputs(dtype, maps, 2, lq, lk, 2, 2, 32, p), p)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 9), (9, 1), (3, 5), (8, 15), (12, 21), (20, 30)])
+def test_boards(dtype, maps, rows, cols):
+    p = _plan((rows, cols))
+    n = rows * cols
+    _compare(_inputs(dtype, maps, 2, n, n, 2, 2, 32, p), p)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_widest_board(dtype):
+    """1024 cells, 3969 relative positions, two 64-wide maps: the sums by position take one LDS row for all waves."""
+    p = _plan((32, 32))
+    _compare(_inputs(dtype, 2, 1, 1024, 1024, 1, 1, 64, p), p)
+    _compare(_inputs(dtype, 1, 1, 1024, 1024, 2, 1, 128, p), p)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("h,kv", [(4, 1), (6, 2), (3, 3)])
+def test_shared_heads(dtype, maps, h, kv):
+    p = _plan(16)
+    _compare(_inputs(dtype, maps, 2, 70, 150, h, kv, 32, p), p)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("maps", [1, 2])
+def test_no_bias_and_long_saturated(dtype, maps):
+    if maps == 2:
+        _compare(_inputs(dtype, 2, 1, 300, 513, 2, 1, 32, None), None)
+    p = _plan(9)  # nearly every pair clamped
+    _compare(_inputs(dtype, maps, 1, 600, 520, 2, 2, 32, p), p)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("maps", [1, 2])
+def test_masks(dtype, maps):
+    """Ragged, scattered, whole tiles out, a sample without any key; masked rows hold NaN and infinities."""
+    p = _plan(32)
+    b, lq, lk = 4, 75, 400
+    inp = _inputs(dtype, maps, b, lq, lk, 4, 2, 32, p)
+    mask = torch.zeros(b, lk, dtype=torch.bool, device="cuda")
+    mask[0, :333] = True
+    mask[1] = torch.rand(lk, generator=torch.Generator().manual_seed(1)).cuda() < 0.3
+    mask[2, 200] = True
+    clean_out, clean = _compare(inp, p, mask)
+    assert bool((clean_out[3] == 0).all()) and all(bool((clean[n][3] == 0).all()) for n in ("q", "k", "v"))
+    assert bool((clean["k"][~mask] == 0).all()) and bool((clean["v"][~mask] == 0).all())
+    bad = dict(inp)
+    for n, x in (("k", math.nan), ("v", math.inf)):
+        bad[n] = inp[n].clone()
+        bad[n][~mask] = x
+    bad["k"][3] = -math.inf
+    names = [n for n in ("q", "k", "v", "table", "lam") if inp[n] is not None]
+    t = {**bad, **{n: bad[n].detach().clone().requires_grad_(True) for n in names}}
+    out = _call(t, p, mask, 0)
+    grads = torch.autograd.grad(out, [t[n] for n in names], inp["dout"])
+    assert torch.equal(out, clean_out)
+    for n, g in zip(names, grads):
+        assert torch.equal(g, clean[n]), n
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("maps", [1, 2])
+def test_table_of_infinities_and_lowest_values(dtype, maps):
+    """Buckets of -inf take their pairs out (a row may lose all of them: zeros); buckets of the lowest finite value leave a row that
+    has nothing else uniform."""
+    p = _plan(16)
+    inp = _inputs(dtype, maps, 2, 90, 40, 2, 2, 32, p)
+    near = p.pairs(90, 40)
+    inp["table"][near[0, 0], :] = -math.inf
+    out, g = _compare(inp, p)
+    assert bool(torch.isfinite(out).all()) and all(bool(torch.isfinite(x).all()) for x in g.values())
+    inp["table"][:] = -math.inf
+    out = _call(inp, p, None, 0)
+    assert bool((out == 0).all())
+    inp["table"][:] = torch.finfo(torch.float32).min
+    t = {n: (x.clone().requires_grad_(True) if n != "dout" and x is not None else x) for n, x in inp.items()}
+    out = _call(t, p, None, 0)
+    mean = inp["v"].double().mean(1, keepdim=True).expand(-1, 90, -1, -1)
+    want = mean if maps == 1 else mean * (1 - inp["lam"].double().view(1, 1, -1, 1))
+    assert _rel(out, want) <= _tol(dtype, 32, 90, 40)
+    dv = torch.autograd.grad(out, t["v"], inp["dout"])[0]
+    each = inp["dout"].double().sum(1, keepdim=True).expand(-1, 40, -1, -1) / 40
+    assert _rel(dv, each if maps == 1 else each * (1 - inp["lam"].double().view(1, 1, -1, 1))) <= _tol(dtype, 32, 90, 40)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("maps", [1, 2])
+def test_one_token_against_a_cache(dtype, maps):
+    """Single queries behind caches of different lengths (split keys), with an int and a per-sample offset."""
+    p = _plan(128)
+    b, lk = 3, 5000
+    inp = _inputs(dtype, maps, b, 1, lk, 4, 2, 64, p)
+    lengths = torch.tensor([5000, 1, 2777], device="cuda")
+    mask = torch.arange(lk, device="cuda")[None] < lengths[:, None]
+    _compare(inp, p, mask, (lengths - 1).to(torch.int32))
+    _compare(inp, p, None, lk - 1)
+    _compare(inp, p, None, 1 << 29)  # everything clamped
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_strides_orders_and_alignment(dtype):
+    p = _plan(24)
+    b, l, h, d = 3, 77, 2, 32
+    packed = torch.randn(l, b, 3, h, d, device="cuda").to(dtype)  # token-major packed projections, read in place
+    q, k, v = (packed[:, :, i].transpose(0, 1) for i in range(3))
+    base = _inputs(dtype, 1, b, l, l, h, h, d, p)
+    inp = {**base, "q": q, "k": k, "v": v}
+    want, grads = _compare({**base, "q": q.contiguous(), "k": k.contiguous(), "v": v.contiguous()}, p)
+    t = {n: x.detach().requires_grad_(True) for n, x in inp.items() if n in ("q", "k", "v", "table")}
+    out = _call({**inp, **t}, p, None, 0)
+    assert torch.equal(out, want) and out.stride(1) > out.stride(0)
+    got = torch.autograd.grad(out, list(t.values()), base["dout"].transpose(0, 1).contiguous().transpose(0, 1))
+    for n, g in zip(t, got):
+        assert torch.equal(g, grads[n]), n
+    # rows that start off a 16-byte boundary, a last dimension that is not contiguous, an expanded batch
+    odd = torch.randn(b * l * h * d + 1, device="cuda").to(dtype)[1:].view(b, l, h, d)
+    wide = torch.randn(b, l, h, 2 * d, device="cuda").to(dtype)[..., ::2]
+    one = torch.randn(1, l, h, d, device="cuda").to(dtype).expand(b, -1, -1, -1)
+    x = _call({**inp, "q": odd, "k": wide, "v": one}, p, None, 0)
+    y = _call({**inp, "q": odd.clone(), "k": wide.clone(), "v": one.clone()}, p, None, 0)
+    assert torch.equal(x, y)
+    rows = torch.zeros(b, 2 * l, dtype=torch.bool, device="cuda")
+    rows[:, ::3] = True
+    m = rows[:, ::2]
+    assert torch.equal(_call(inp, p, m, 0), _call(inp, p, m.contiguous(), 0))
+
+
+def test_repeatable_and_on_another_stream():
+    p = _plan((8, 15))
+    inp = _inputs(torch.bfloat16, 2, 16, 120, 120, 2, 2, 32, p)
+    first = _compare(inp, p)
+    again = _compare(inp, p)
+    assert torch.equal(first[0], again[0]) and all(torch.equal(first[1][n], again[1][n]) for n in first[1])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = _compare(inp, p)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(first[0], other[0]) and all(torch.equal(first[1][n], other[1][n]) for n in first[1])
+
+
+def test_captured_forward_and_backward():
+    """One graph of a training call, replayed on new inputs with eager calls and synchronizations in between."""
+    p = _plan(64)
+    inp = _inputs(torch.float32, 1, 2, 200, 900, 4, 2, 32, p)
+    names = ("q", "k", "v", "table")
+    static = {n: (x.clone() if x is not None else None) for n, x in inp.items()}
+    mask = torch.ones(2, 900, dtype=torch.bool, device="cuda")
+
+    def step():  # noqa: ANN202
+        t = {**static, **{n: static[n].detach().requires_grad_(True) for n in names}}
+        out = _call(t, p, mask, 0)
+        return (out.detach(), *torch.autograd.grad(out, [t[n] for n in names], static["dout"]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in range(4):
+        new = _inputs(torch.float32, 1, 2, 200, 900, 4, 2, 32, p, seed=seed)
+        mask.fill_(True)
+        mask[1, 100 * seed :] = False
+        for n, x in new.items():
+            if x is not None:
+                static[n].copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in captured]
+        want = step()
+        torch.cuda.synchronize()
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+
+
+def test_gradients_by_differences():
+    """Central differences of a random functional of the output in every argument (fp32, step 2^-6)."""
+    p = _plan(12)
+    for maps in (1, 2):
+        inp = _inputs(torch.float32, maps, 1, 9, 14, 2, 1, 16, p, std=0.5)
+        names = [n for n in ("q", "k", "v", "table", "lam") if inp[n] is not None]
+        t = {**inp, **{n: inp[n].clone().requires_grad_(True) for n in names}}
+        grads = torch.autograd.grad(_call(t, p, None, 0), [t[n] for n in names], inp["dout"])
+        eps = 2.0**-6
+        for n, g in zip(names, grads):
+            direction = torch.randn_like(inp[n])
+            direction /= direction.norm()
+            vals = []
+            for s in (eps, -eps):
+                out = _call({**inp, n: inp[n] + s * direction}, p, None, 0)
+                vals.append(float((out.double() * inp["dout"].double()).sum()))
+            slope = (vals[0] - vals[1]) / (2 * eps)
+            want = float((g.double() * direction.double()).sum())
+            # truncation: third derivative times eps^2 / 6 (order of |dout| |v| = 1e2 at most); rounding: u |f| / eps
+            assert abs(slope - want) <= eps**2 / 6 * 100 + 64 * U32 / eps * float(inp["dout"].norm()), (maps, n, slope, want)
+
+
+@pytest.mark.parametrize("maps", [1, 2])
+def test_empty_calls(maps):
+    p = _plan(16)
+    for b, lq, lk in ((0, 4, 4), (2, 0, 4), (2, 4, 0)):
+        inp = _inputs(torch.float32, maps, b, lq, lk, 2, 2, 32, p)
+        t = {n: (x.clone().requires_grad_(True) if n != "dout" and x is not None else x) for n, x in inp.items()}
+        out = _call(t, p, None, 0)
+        assert out.shape == inp["dout"].shape and bool((out == 0).all())
+        out.sum().backward()
+        assert all(x.grad is None or bool((x.grad == 0).all()) for n, x in t.items() if n != "dout" and x is not None)
