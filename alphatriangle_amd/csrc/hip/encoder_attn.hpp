@@ -6,8 +6,8 @@
 //     x_m[i][j] = scale q_m[i] . k_m[j] + T[bucket(pos(j) - pos(i))][h M + m],   P_m = softmax_j(x_m),
 //     o[i] = sum_j P_1[i][j] v[j]                     (M = 1, values D wide)
 //     o[i] = sum_j (P_1 - lam_h P_2)[i][j] v[j]       (M = 2, values 2 D wide)
-// and its gradients.  Exponentials are base 2 throughout (scale and bias are multiplied by log2 e in 32 bits, after the
-// matrix product, so no operand is rounded a second time).
+// and its gradients.  The bias, divided by the scale, is where the matrix product's accumulator starts, so the scores cost
+// no vector instruction until the exponential, exp2(fma(x, scale log2 e, -base)): see Exponent.
 //
 // Matrix operands.  bf16 rows use v_mfma_f32_16x16x32_bf16 as they are; fp32 rows use v_mfma_f32_16x16x4_f32, true fp32
 // products: three bf16 passes over (hi, lo) splits carry 16 bits per operand, 30 times the rounding of an fp32 product.
@@ -22,6 +22,7 @@
 
 namespace atrihip {
 
+// Filled by ops/attention.py in this order (8-byte fields first, then 4-byte ones).
 struct EncAttnArgs {
   const void* q;       // [B, Lq, H M, D] by strides
   const void* k;       // [B, Lk, KV M, D]
@@ -33,20 +34,32 @@ struct EncAttnArgs {
   void* dv;
   const float* table;  // [buckets, H M]; nullptr: no position bias
   const int* lut;      // [2 R + 1] bucket of every clamped position difference
+  const int* order;    // [2 R + 1] differences by bucket: those of bucket b at start[b] .. start[b + 1] - 1
+  const int* start;
   const float* lam;    // [H] (M = 2)
-  const unsigned long long* words;  // [B, ceil(Lk / 64)] validity bit of every key; nullptr: all keys
+  const unsigned char* mask;  // [B, Lk] bytes by strides (nonzero: the key takes part); nullptr: all keys
+  unsigned long long* words;  // [B, ceil(Lk / 64)] validity bit of every key, made from mask by the forward pass; nullptr: all keys
   const int* qoff;     // [B] position of the first query, nullptr: q0 for all samples
-  float* stat;         // [M, B H Lq, 2] row maximum (log2 domain; +inf: no key) and 1 / sum (0: no key); nullptr: not wanted
+  float* stat;         // [M, B H Lq, 2] row maximum of x / scale (+inf: no key) and 1 / sum (0: no key); nullptr: not wanted
   float* o32;          // [M] x [B, Lq, H, DV] per-map outputs in 32 bits by strides (backward: their product with dO is delta)
   float* delta;        // [M, B H Lq]
   float* part_o;       // [splits, M, B H Lq, DV] unnormalised partial outputs (splits > 1)
   float* part_ml;      // [splits, M, B H Lq, 2] their maxima and sums
-  float* hist;         // [B H ceil(Lq / queries per workgroup), M, 2 R + 1] partial sums of dS by position difference; nullptr: not wanted
+  float* hist;         // [workgroups of the query-owned pass, M, 2 R + 1] sums of dS by position difference; nullptr: not wanted
+  float* mid;          // [shares, H M, 2 R + 1] the same, added up over shares of the samples and query tiles
+  float* dq_part;      // [q_splits, B, H, Lq, M D] partial dQ in 32 bits (q_splits > 1)
+  float* kv_part;      // [k_splits, B, KV, Lk, M D + DV] partial dK and dV (k_splits > 1)
+  float* dtable;       // [buckets, H M]
+  float* dlam;         // [H]; nullptr: not wanted
   long long qs[3], ks[3], vs[3], os[3], gs[3], dqs[3], dks[3], dvs[3];  // element strides: sample, token, head
   long long o32s[4];   // o32: sample, token, head, map
+  long long ms[2];     // mask: sample, key
   int B, Lq, Lk, H, KV, D, DV, M;
   int R, W, q0;        // clamp of the position difference; board width (0: sequence); position of the first query
-  int bf16, splits, hist_rows;
+  int buckets, bf16, shares, hist_rows;
+  int splits, chunk;      // forward: key ranges per query tile, samples a workgroup walks one after the other
+  int q_splits, q_chunk;  // query-owned pass: the same
+  int k_splits, k_chunk;  // key-owned pass: query ranges per key tile, samples
   float scale;
 };
 
@@ -147,9 +160,19 @@ __device__ __forceinline__ int query_origin(const EncAttnArgs& a, int b) {
 }
 __device__ __forceinline__ int clamp_slot(int d, int R2) { return d < 0 ? 0 : d > R2 ? R2 : d; }
 
-// log2 e times the bias; a finite bias stays finite (a table may hold the type's lowest value as a mask).
-__device__ __forceinline__ float bias_log2(float t) {
-  const float x = t * kLog2E;
+// exp2 of (x - top) sl2, x and top in units of 1 / scale, sl2 = scale log2 e.  One fused multiply-add: base = top sl2 is rounded
+// once, and every value of a row carries the same base, so its rounding cancels against the sum.  Far rows (|base| of a
+// million: a table used as a mask) take the difference first, which is exact where they are equal; +inf (a row
+// without keys, a query behind the last) gives zeros either way.
+struct Exponent {
+  static __device__ __forceinline__ bool far(float base) { return fabsf(base) >= 1e6f && base != INFINITY; }
+  static __device__ __forceinline__ float near_(float x, float base, float sl2) { return __builtin_amdgcn_exp2f(fmaf(x, sl2, -base)); }
+  static __device__ __forceinline__ float far_(float x, float top, float sl2) { return __builtin_amdgcn_exp2f((x - top) * sl2); }
+};
+
+// The bias in units of 1 / scale; a finite bias stays finite (a table may hold the type's lowest value as a mask).
+__device__ __forceinline__ float bias_units(float t, float scale) {
+  const float x = t / scale;
   if (__builtin_isinf(x) && !__builtin_isinf(t)) return copysignf(3.4028234663852886e38f, t);
   return x;
 }
@@ -157,7 +180,7 @@ __device__ __forceinline__ void fill_bias(const EncAttnArgs& a, float* bias, int
   const int n = 2 * a.R + 1, hm = a.H * M;
   for (int i = tid; i < n; i += 256) {
     const float* row = a.table + (size_t)a.lut[i] * hm + head * M;
-    for (int m = 0; m < M; ++m) bias[m * n + i] = bias_log2(row[m]);
+    for (int m = 0; m < M; ++m) bias[m * n + i] = bias_units(row[m], a.scale);
   }
 }
 
@@ -202,35 +225,61 @@ __device__ __forceinline__ unsigned long long range_word(int t0, int L) {  // bi
   return n >= 64 ? ~0ULL : n <= 0 ? 0ULL : ((1ULL << n) - 1);
 }
 
-// The key tiles of one sample that hold a valid key, in order.  64 words are held across the wave at a time; every wave of a
-// workgroup walks the same list.
+__device__ __forceinline__ unsigned long long board_word(const EncAttnArgs& a, int b, int tile) {
+  if (tile * kTile >= a.Lk) return 0;
+  return a.words ? a.words[(size_t)b * ((a.Lk + kTile - 1) / kTile) + tile] : range_word(tile * kTile, a.Lk);
+}
+
+// The key tiles [first, last) of samples [sample, samples) that hold a valid key, in order: (sample, tile, word) names the tile
+// whose loads are under way, sample == samples the end.  64 validity words are held across the wave at a time; every wave
+// of a workgroup walks the same list.
 struct TileWalk {
   const unsigned long long* words;
-  int Lk, end, base;
-  unsigned long long mine, live, word;
-  __device__ __forceinline__ void start(const unsigned long long* w, int lk, int first, int last) {
-    words = w; Lk = lk; end = last; base = first - 64; live = 0; word = 0; mine = 0;
-    if (!w) base = first - 1;
+  int Lk, tiles, first, last, samples, base;
+  unsigned long long mine, live;
+  int sample, tile;
+  unsigned long long word;
+  __device__ __forceinline__ void open() {
+    base = first - (words ? 64 : 1);
+    live = 0;
   }
-  // Next tile with a valid key (its bits in `word`), or `end`.
-  __device__ __forceinline__ int next() {
-    if (!words) {
-      ++base;
-      word = base < end ? range_word(base * kTile, Lk) : 0;
-      return base;
+  __device__ __forceinline__ void start(const EncAttnArgs& a, int b0, int b1, int t0, int t1) {
+    words = a.words;
+    Lk = a.Lk;
+    tiles = (a.Lk + kTile - 1) / kTile;
+    first = t0;
+    last = t1;
+    samples = b1;
+    sample = b0;
+    mine = 0;
+    open();
+    next();
+  }
+  __device__ __forceinline__ void next() {
+    for (; sample < samples; ++sample, open()) {
+      if (!words) {
+        if (++base < last) {
+          tile = base;
+          word = range_word(base * kTile, Lk);
+          return;
+        }
+        continue;
+      }
+      while (!live && base + 64 < last) {
+        base += 64;
+        const int lane = threadIdx.x & 63;
+        mine = base + lane < last ? words[(size_t)sample * tiles + base + lane] : 0;
+        live = __ballot(mine != 0);
+      }
+      if (live) {
+        const int i = __ffsll(live) - 1;
+        live &= live - 1;
+        const unsigned lo = __builtin_amdgcn_readlane((unsigned)mine, i), hi = __builtin_amdgcn_readlane((unsigned)(mine >> 32), i);
+        word = ((unsigned long long)hi << 32) | lo;
+        tile = base + i;
+        return;
+      }
     }
-    while (!live) {
-      base += 64;
-      if (base >= end) return end;
-      const int lane = threadIdx.x & 63;
-      mine = base + lane < end ? words[base + lane] : 0;
-      live = __ballot(mine != 0);
-    }
-    const int i = __ffsll((unsigned long long)live) - 1;
-    live &= live - 1;
-    const unsigned lo = __builtin_amdgcn_readlane((unsigned)mine, i), hi = __builtin_amdgcn_readlane((unsigned)(mine >> 32), i);
-    word = ((unsigned long long)hi << 32) | lo;
-    return base + i;
   }
 };
 
@@ -241,14 +290,33 @@ __device__ __forceinline__ int clamped_side(const EncAttnArgs& a, int kmin, int 
   return kmin - qmax >= a.R ? 1 : kmax - qmin <= -a.R ? -1 : 0;
 }
 
+// Boards of 2 to 4 key tiles keep their bias (and the sums of dS by pair) in registers over all samples a workgroup walks: every
+// sample has the same positions.  The tiles are then unrolled: NT of them, with as many 16-row columns per wave as
+// keep 64 registers for each.  0: the general form (sequences, smaller and larger boards).
+inline int enc_board_tiles(int W, int Lk, int D, int M) {
+  const int tiles = (Lk + kTile - 1) / kTile;
+  if (W <= 0 || D > 32 || tiles < 2) return 0;
+  return tiles == 2 ? 2 : tiles <= 4 && M == 1 ? 4 : 0;
+}
+// 16-row columns per wave: queries in the forward and the query-owned pass, keys in the key-owned one.
+inline int enc_columns(int W, int L, int Lk, int D, int M, bool forward) {
+  if (M == 2 || D > 64) return 1;
+  const int nt = enc_board_tiles(W, Lk, D, M);
+  if (nt) return nt == 2 ? 2 : 1;
+  return forward && L <= 64 ? 1 : 2;  // two, once they exist: every staged fragment then feeds two products
+}
+
 inline int enc_check(const EncAttnArgs& a) {
   if (a.B < 1 || a.Lq < 1 || a.Lk < 1 || a.H < 1 || a.KV < 1 || a.H % a.KV != 0) return -10;
   if (a.M < 1 || a.M > 2 || a.D < 8 || a.D % 8 != 0 || a.D > (a.M == 1 ? 128 : 64) || a.DV != a.D * a.M) return -11;
   if (a.table && (a.R < 0 || a.R > 2047 || a.lut == nullptr)) return -12;
+  if (!(a.scale > 0.f) || !(a.scale < 3e38f)) return -19;
   if (a.M == 1 && !a.table) return -13;
   if (a.M == 2 && !a.lam) return -14;
-  if ((long long)a.B * a.H * ((a.Lq + 63) / 64) * (a.splits < 1 ? 1 : a.splits) >= (1LL << 31)) return -15;
-  if ((long long)a.B * a.KV * ((a.Lk + 63) / 64) >= (1LL << 31)) return -15;
+  if (a.splits < 1 || a.q_splits < 1 || a.k_splits < 1 || a.chunk < 1 || a.q_chunk < 1 || a.k_chunk < 1) return -18;
+  const long long most = a.splits > a.q_splits ? a.splits : a.q_splits;
+  if ((long long)a.B * a.H * ((a.Lq + 63) / 64) * most >= (1LL << 31)) return -15;
+  if ((long long)a.B * a.KV * ((a.Lk + 63) / 64) * a.k_splits >= (1LL << 31)) return -15;
   if (a.Lq > (1 << 29) || a.Lk > (1 << 29)) return -16;
   return 0;
 }

@@ -6,12 +6,16 @@
 //                 difference (the bias table's gradient before it is folded into buckets)
 //   key-owned:    dV = (P_1 - lam P_2)^T dO;  dK_m = scale dS_m^T Q_m
 // With two maps dP_1 = dO V^T and dP_2 = -lam dP_1, so one product serves both; d lam = -sum delta_2.
+#include <type_traits>
+
 #include "encoder_attn.hpp"
 
 using namespace atrihip;
 
 namespace {
 
+// Waves per SIMD the register allocation leaves room for: two where 256 registers hold the kernel (32-wide heads), else one.
+constexpr int waves_of(int D) { return D <= 32 ? 2 : 1; }
 constexpr int kDsPitch = kTile + 4;  // row pitch of a wave's 16 x 64 tile of dS on its way to the diagonal sums
 
 __device__ __forceinline__ void wave_lds_fence() {  // orders a wave's own LDS writes before its other lanes' reads
@@ -20,51 +24,40 @@ __device__ __forceinline__ void wave_lds_fence() {  // orders a wave's own LDS w
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// Adds a wave's 16 x 64 tile of dS (LDS, row = query) to the sums by position difference.  Lane l reads the element of every
-// row on its wrapped diagonal: key (l - 15 + row) mod 64, conflict free and each element once.  Pairs on different
-// diagonals never have the same (unclamped) difference, on a board either, so every slot of `sums` has one writer per
-// step and the order of the additions is fixed.  Clamped differences go to the lane's own lo / hi.
-__device__ __forceinline__ void add_diagonals(const EncAttnArgs& a, float* sums, const float* ds, const int* pos_k, int k0, int q0, int origin,
-                                              int lane, float& lo, float& hi) {
+// Adds a wave's 16 x 64 tile of dS (LDS, row = query) to its sums by position difference, without atomics (LDS additions of
+// floats took 2.8 cycles a lane here) and in a fixed order.
+// Sequences: lane l adds up the wrapped diagonal key = (l - 15 + row) mod 64, each element of the tile once, in registers;
+// different diagonals have different (unclamped) differences, so every slot has one writer.  Clamped ones go to lo / hi.
+// Boards: row by row; a row's 64 keys lie at 64 different positions, so again no two lanes meet in a slot.
+__device__ __forceinline__ void add_tile(const EncAttnArgs& a, float* sums, const float* ds, int pos_k, int pos_q, int k0, int q0, int lane, float& lo,
+                                         float& hi) {
   const int R2 = 2 * a.R;
   if (a.W == 0) {
-    float low_part = 0.f, high_part = 0.f;  // rows below the wrap (diagonal lane - 15), rows above it (diagonal lane + 49)
+    float before = 0.f, after = 0.f;  // rows past the wrap (diagonal lane - 15), rows before it (diagonal lane + 49)
 #pragma unroll
     for (int row = 0; row < 16; ++row) {
       const float v = ds[row * kDsPitch + ((lane - 15 + row) & 63)];
-      if (row >= 15 - lane) low_part += v; else high_part += v;
+      if (row >= 15 - lane) before += v; else after += v;
     }
-    const int slot = k0 - q0 - origin + a.R + lane - 15;
-    if (slot <= 0) lo += low_part; else if (slot >= R2) hi += low_part; else sums[slot] += low_part;
+    const int slot = k0 - q0 + a.R + lane - 15, slot2 = slot + 64;
+    if (slot <= 0) lo += before; else if (slot >= R2) hi += before; else sums[slot] += before;
     if (lane < 15) {
-      const int s2 = slot + 64;
-      if (s2 <= 0) lo += high_part; else if (s2 >= R2) hi += high_part; else sums[s2] += high_part;
+      if (slot2 <= 0) lo += after; else if (slot2 >= R2) hi += after; else sums[slot2] += after;
     }
-    wave_lds_fence();
     return;
   }
-  float run = 0.f;
-  int slot = -1;
 #pragma unroll
   for (int row = 0; row < 16; ++row) {
-    const int key = (lane - 15 + row) & 63;
-    const float v = ds[row * kDsPitch + key];
-    const bool valid = k0 + key < a.Lk && q0 + row < a.Lq;
-    const int s = valid ? clamp_slot(pos_k[key] - token_pos(q0 + row, a.W) + a.R, R2) : slot;
-    if (s != slot && slot >= 0) {
-      sums[slot] += run;
-      run = 0.f;
-    }
-    slot = s;
-    run += valid ? v : 0.f;
+    const int slot = pos_k - __builtin_amdgcn_readlane(pos_q, row) + a.R;
+    const float v = ds[row * kDsPitch + lane];
+    if (v != 0.f && slot >= 0 && slot <= R2) sums[slot] += v;  // rows and keys beyond the board hold zeros
+    wave_lds_fence();
   }
-  if (slot >= 0) sums[slot] += run;
-  wave_lds_fence();
 }
 
-// One 4-wave workgroup per (sample, head, 64 QS queries).
-template <typename T, int D, int M, int QS, bool BIAS>
-__global__ __launch_bounds__(256) void enc_attn_bwd_q_kernel(EncAttnArgs a) {
+// One 4-wave workgroup per (head, 64 QS queries, key range) and q_chunk samples, one after the other.
+template <typename T, int D, int M, int QS, bool BIAS, int NT>
+__global__ __launch_bounds__(256, NT > 0 ? 1 : waves_of(D)) void enc_attn_bwd_q_kernel(EncAttnArgs a) {
   using O = Ops<T>;
   using Frag = typename O::Frag;
   constexpr int DV = D * M, DC = D / O::kDims, VC = DV / O::kDims, ND = D / 16, NKB = 4 / O::kSub;
@@ -80,219 +73,329 @@ __global__ __launch_bounds__(256) void enc_attn_bwd_q_kernel(EncAttnArgs a) {
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, q4 = lane >> 4;
   const int nqt = (a.Lq + 64 * QS - 1) / (64 * QS);
-  const int id = xcd_order(blockIdx.x, gridDim.x);
-  const int qt = id % nqt, bh = id / nqt;
-  const int b = bh / a.H, h = bh - b * a.H, kvh = h / (a.H / a.KV);
+  const int group_id = xcd_order(blockIdx.x, gridDim.x);
+  int id = group_id;
+  const int qt = id % nqt;
+  id /= nqt;
+  const int split = id % a.q_splits;
+  id /= a.q_splits;
+  const int h = id % a.H, kvh = h / (a.H / a.KV);
+  const int b_first = id / a.H * a.q_chunk, b_last = b_first + a.q_chunk < a.B ? b_first + a.q_chunk : a.B;
   const int tiles = (a.Lk + kTile - 1) / kTile;
-  const T* kb_ = reinterpret_cast<const T*>(a.k) + b * a.ks[0] + (long long)kvh * M * a.ks[2];
-  const T* vb_ = reinterpret_cast<const T*>(a.v) + b * a.vs[0] + kvh * a.vs[2];
+  const int per = (tiles + a.q_splits - 1) / a.q_splits;
+  const int t_first = split * per, t_last = t_first + per < tiles ? t_first + per : tiles;
   const bool want_sums = BIAS && a.hist != nullptr;
-  if constexpr (BIAS) fill_bias(a, bias_lds, h, M, tid);
-  if (want_sums)
-    for (int i = tid; i < a.hist_rows * M * slots; i += 256) sum_lds[i] = 0.f;
   float* my_sums = sum_lds + (a.hist_rows == 4 ? wave * M * slots : 0);
-
   const long long rows = (long long)a.B * a.H * a.Lq;
   const int q_first = (qt * 4 + wave) * 16 * QS;
   const bool busy = q_first < a.Lq;
-  const int origin = BIAS ? query_origin(a, b) : 0;
   const float lam = M == 2 ? a.lam[h] : 0.f;
-  Frag qf[M][QS][DC], dof[QS][VC];
-  float top[M][QS], inv[M][QS], delta[M][QS];
-  int pos_q[QS];
-#pragma unroll
-  for (int s = 0; s < QS; ++s) {
-    const int query = q_first + s * 16 + l15;
-    const bool valid = query < a.Lq;
-    pos_q[s] = BIAS ? token_pos(query, a.W) + origin : 0;
-    load_rows<T, VC>(dof[s], reinterpret_cast<const T*>(a.dout) + b * a.gs[0] + (long long)query * a.gs[1] + h * a.gs[2], valid, a.DV, q4);
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-      load_rows<T, DC>(qf[m][s], reinterpret_cast<const T*>(a.q) + b * a.qs[0] + (long long)query * a.qs[1] + (long long)(h * M + m) * a.qs[2], valid,
-                       a.D, q4);
-      float2 st = make_float2(INFINITY, 0.f);
-      if (valid) st = *reinterpret_cast<const float2*>(a.stat + 2 * (m * rows + (long long)bh * a.Lq + query));
-      top[m][s] = st.x;
-      inv[m][s] = st.y;
-      const float* o = a.o32 + b * a.o32s[0] + (long long)query * a.o32s[1] + h * a.o32s[2] + m * a.o32s[3];
-      float dot = 0.f;
-#pragma unroll
-      for (int c = 0; c < VC; ++c) {
-        const int col = c * O::kDims + q4 * O::kVec;
-        if (!valid || col >= a.DV) continue;
-        float v[O::kVec];
-#pragma unroll
-        for (int e = 0; e < O::kVec; e += 4) {
-          const float4 u = *reinterpret_cast<const float4*>(o + col + e);
-          v[e] = u.x; v[e + 1] = u.y; v[e + 2] = u.z; v[e + 3] = u.w;
-        }
-        dot += O::dot(dof[s][c], v);
-      }
-      delta[m][s] = quad_row_sum(dot);
-      if (valid && q4 == 0) a.delta[m * rows + (long long)bh * a.Lq + query] = delta[m][s];
-    }
-  }
-  float4v dq[M][QS][ND];
-  float lo[M], hi[M];
-#pragma unroll
-  for (int m = 0; m < M; ++m) {
-    lo[m] = hi[m] = 0.f;
-#pragma unroll
-    for (int s = 0; s < QS; ++s)
-#pragma unroll
-      for (int n = 0; n < ND; ++n) dq[m][s][n] = float4v{0.f, 0.f, 0.f, 0.f};
-  }
   const float sl2 = a.scale * kLog2E;
 
   Stage<T, D> sk[M];
   Stage<T, DV> sv;
+  auto fetch = [&](const TileWalk& w) {
+    const T* kb = reinterpret_cast<const T*>(a.k) + w.sample * a.ks[0] + (long long)kvh * M * a.ks[2];
+#pragma unroll
+    for (int m = 0; m < M; ++m) sk[m].load(kb + m * a.ks[2], a.ks[1], w.tile * kTile, w.word, a.D, tid);
+    sv.load(reinterpret_cast<const T*>(a.v) + w.sample * a.vs[0] + kvh * a.vs[2], a.vs[1], w.tile * kTile, w.word, a.DV, tid);
+  };
   TileWalk walk;
-  walk.start(a.words ? a.words + (size_t)b * tiles : nullptr, a.Lk, 0, tiles);
-  int t = walk.next();
-  if (t < tiles) {
-#pragma unroll
-    for (int m = 0; m < M; ++m) sk[m].load(kb_ + m * a.ks[2], a.ks[1], t * kTile, walk.word, a.D, tid);
-    sv.load(vb_, a.vs[1], t * kTile, walk.word, a.DV, tid);
+  if constexpr (NT == 0) {
+    walk.start(a, b_first, b_last, t_first, t_last);
+  } else {
+    walk.sample = b_first;
+    walk.tile = 0;
+    walk.word = board_word(a, b_first, 0);
   }
-  while (t < tiles) {
-    const unsigned long long word = walk.word;
-    const int t0 = t * kTile;
+  if (walk.sample < b_last) fetch(walk);
+  if constexpr (BIAS) fill_bias(a, bias_lds, h, M, tid);
+  if (want_sums)
+    for (int i = tid; i < a.hist_rows * M * slots; i += 256) sum_lds[i] = 0.f;
+  float lo[M], hi[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m) lo[m] = hi[m] = 0.f;
+  int token_q[QS];
+#pragma unroll
+  for (int s = 0; s < QS; ++s) token_q[s] = BIAS ? token_pos(q_first + s * 16 + l15, a.W) : 0;
+  // Boards: the bias of this wave's pairs, and the sums of their dS over the samples.
+  float4v bias_reg[M][QS][NT ? NT * 4 : 1], sum_reg[M][QS][NT ? NT * 4 : 1];
+  if constexpr (NT > 0) {
     __syncthreads();
 #pragma unroll
-    for (int m = 0; m < M; ++m) sk[m].store(k_lds + m * kTile * PK, PK, tid);
-    sv.store(v_lds, PV, tid);
-    if (BIAS && tid < kTile) pos_lds[tid] = token_pos(t0 + tid, a.W);
-    __syncthreads();
-    t = walk.next();
-    if (t < tiles) {
+    for (int kt = 0; kt < NT * 4; ++kt)
 #pragma unroll
-      for (int m = 0; m < M; ++m) sk[m].load(kb_ + m * a.ks[2], a.ks[1], t * kTile, walk.word, a.D, tid);
-      sv.load(vb_, a.vs[1], t * kTile, walk.word, a.DV, tid);
+      for (int j = 0; j < 4; ++j) {
+        const int key = kt * 16 + q4 * 4 + j, pos = token_pos(key, a.W);
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int s = 0; s < QS; ++s) {
+            bias_reg[m][s][kt][j] = key < a.Lk ? bias_lds[m * slots + clamp_slot(pos - token_q[s] + a.R, R2)] : -INFINITY;
+            sum_reg[m][s][kt][j] = 0.f;
+          }
+      }
+  }
+
+  for (int b = b_first; b < b_last; ++b) {
+    const int origin = BIAS ? query_origin(a, b) : 0;
+    const long long row0 = ((long long)b * a.H + h) * a.Lq;
+    Frag qf[M][QS][DC], dof[QS][VC];
+    float top[M][QS], inv[M][QS], delta[M][QS];
+#pragma unroll
+    for (int s = 0; s < QS; ++s) {
+      const int query = q_first + s * 16 + l15;
+      const bool valid = query < a.Lq;
+      load_rows<T, VC>(dof[s], reinterpret_cast<const T*>(a.dout) + b * a.gs[0] + (long long)query * a.gs[1] + h * a.gs[2], valid, a.DV, q4);
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        load_rows<T, DC>(qf[m][s], reinterpret_cast<const T*>(a.q) + b * a.qs[0] + (long long)query * a.qs[1] + (long long)(h * M + m) * a.qs[2], valid,
+                         a.D, q4);
+        float2 st = make_float2(INFINITY, 0.f);
+        if (valid) st = *reinterpret_cast<const float2*>(a.stat + 2 * (m * rows + row0 + query));
+        top[m][s] = st.x;
+        inv[m][s] = st.y;
+        const float* o = a.o32 + b * a.o32s[0] + (long long)query * a.o32s[1] + h * a.o32s[2] + m * a.o32s[3];
+        float dot = 0.f;
+#pragma unroll
+        for (int c = 0; c < VC; ++c) {
+          const int col = c * O::kDims + q4 * O::kVec;
+          if (!valid || col >= a.DV) continue;
+          float v[O::kVec];
+#pragma unroll
+          for (int e = 0; e < O::kVec; e += 4) {
+            const float4 u = *reinterpret_cast<const float4*>(o + col + e);
+            v[e] = u.x; v[e + 1] = u.y; v[e + 2] = u.z; v[e + 3] = u.w;
+          }
+          dot += O::dot(dof[s][c], v);
+        }
+        delta[m][s] = quad_row_sum(dot);
+        if (valid && q4 == 0 && split == 0) a.delta[m * rows + row0 + query] = delta[m][s];
+      }
     }
-    float4v ds[M][QS][4];
-    int side[QS];
-    if (busy) {
+    float4v dq[M][QS][ND];
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int s = 0; s < QS; ++s)
+#pragma unroll
+        for (int n = 0; n < ND; ++n) dq[m][s][n] = float4v{0.f, 0.f, 0.f, 0.f};
+
+    float base[M][QS];
+    bool far_any = false;
+#pragma unroll
+    for (int m = 0; m < M; ++m)
 #pragma unroll
       for (int s = 0; s < QS; ++s) {
-        const int qa = q_first + s * 16 + origin;
-        side[s] = BIAS ? clamped_side(a, t0, t0 + kTile - 1, qa, qa + 15) : 0;
+        base[m][s] = top[m][s] * sl2;
+        far_any |= Exponent::far(base[m][s]);
       }
+    const bool far = __any(far_any);
+    // One staged tile; kt0 is its first 16-key block where bias and sums are in registers.
+    auto tile = [&](auto kt0_) {
+      constexpr int kt0 = decltype(kt0_)::value;
+      const unsigned long long word = NT > 0 && !a.words ? ~0ULL : walk.word;
+      const int t0 = walk.tile * kTile;
+      __syncthreads();
 #pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) {
-        float4v dp[QS][O::kSub];
+      for (int m = 0; m < M; ++m) sk[m].store(k_lds + m * kTile * PK, PK, tid);
+      sv.store(v_lds, PV, tid);
+      if (BIAS && NT == 0 && tid < kTile) pos_lds[tid] = token_pos(t0 + tid, a.W);
+      __syncthreads();
+      if constexpr (NT == 0) {
+        walk.next();
+      } else {
+        constexpr bool last = kt0 / 4 + 1 == NT;
+        walk.tile = last ? 0 : kt0 / 4 + 1;
+        walk.sample = b + (last ? 1 : 0);
+        if (walk.sample < b_last) walk.word = board_word(a, walk.sample, walk.tile);
+      }
+      if (walk.sample < b_last) fetch(walk);
+      float4v ds[M][QS][4];  // without the row's 1 / sum, which joins at the end of the row
+      int side[QS];
+      if (busy) {
 #pragma unroll
-        for (int u = 0; u < O::kSub; ++u) {
-          const int kt = kb * O::kSub + u;
+        for (int s = 0; s < QS; ++s) {
+          const int qa = q_first + s * 16 + origin;
+          side[s] = BIAS && NT == 0 ? clamped_side(a, t0, t0 + kTile - 1, qa, qa + 15) : 0;
+        }
 #pragma unroll
-          for (int s = 0; s < QS; ++s) dp[s][u] = float4v{0.f, 0.f, 0.f, 0.f};
+        for (int kb = 0; kb < NKB; ++kb) {
 #pragma unroll
-          for (int c = 0; c < VC; ++c) {
-            const Frag vf = O::row_frag(v_lds, PV, kt * 16 + l15, c, q4);
+          for (int u = 0; u < O::kSub; ++u) {
+            const int kt = kb * O::kSub + u;
+            float4v dp[QS];
 #pragma unroll
-            for (int s = 0; s < QS; ++s) dp[s][u] = O::mma(vf, dof[s][c], dp[s][u]);
+            for (int s = 0; s < QS; ++s) dp[s] = float4v{-delta[0][s], -delta[0][s], -delta[0][s], -delta[0][s]};  // dP - delta of the first map
+#pragma unroll
+            for (int c = 0; c < VC; ++c) {
+              const Frag vf = O::row_frag(v_lds, PV, kt * 16 + l15, c, q4);
+#pragma unroll
+              for (int s = 0; s < QS; ++s) dp[s] = O::mma(vf, dof[s][c], dp[s]);
+            }
+            int4 p4 = make_int4(0, 0, 0, 0);
+            if constexpr (BIAS && NT == 0) p4 = *reinterpret_cast<const int4*>(pos_lds + kt * 16 + q4 * 4);
+            const int pj[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+              float4v x[QS];
+#pragma unroll
+              for (int s = 0; s < QS; ++s) {
+                if constexpr (NT > 0) {
+                  x[s] = bias_reg[m][s][kt0 + kt];
+                } else if constexpr (BIAS) {
+                  const float* bias = bias_lds + m * slots;
+                  if (side[s] != 0) {
+                    const float c = bias[side[s] > 0 ? R2 : 0];
+                    x[s] = float4v{c, c, c, c};
+                  } else {
+                    const int off = a.R - token_q[s] - origin;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[s][j] = bias[clamp_slot(pj[j] + off, R2)];
+                  }
+                } else {
+                  x[s] = float4v{0.f, 0.f, 0.f, 0.f};
+                }
+              }
+#pragma unroll
+              for (int c = 0; c < DC; ++c) {
+                const Frag kf = O::row_frag(k_lds + m * kTile * PK, PK, kt * 16 + l15, c, q4);
+#pragma unroll
+                for (int s = 0; s < QS; ++s) x[s] = O::mma(kf, qf[m][s][c], x[s]);
+              }
+#pragma unroll
+              for (int s = 0; s < QS; ++s) {
+                const float shift = m == 0 ? 0.f : delta[0][s] - delta[m][s];
+                if (far) {
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) x[s][j] = Exponent::far_(x[s][j], top[m][s], sl2);
+                } else {
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) x[s][j] = Exponent::near_(x[s][j], base[m][s], sl2);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) ds[m][s][kt][j] = x[s][j] * (m == 0 ? dp[s][j] : dp[s][j] + shift);
+                if (word != ~0ULL) {
+                  const unsigned bits = (unsigned)(word >> (kt * 16 + q4 * 4));
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) ds[m][s][kt][j] = (bits >> j) & 1 ? ds[m][s][kt][j] : 0.f;
+                }
+              }
+            }
           }
 #pragma unroll
           for (int m = 0; m < M; ++m) {
-            float4v x[QS];
+            Frag sf[QS];
 #pragma unroll
-            for (int s = 0; s < QS; ++s) x[s] = float4v{0.f, 0.f, 0.f, 0.f};
+            for (int s = 0; s < QS; ++s) sf[s] = O::acc_frag(&ds[m][s][kb * O::kSub]);
 #pragma unroll
-            for (int c = 0; c < DC; ++c) {
-              const Frag kf = O::row_frag(k_lds + m * kTile * PK, PK, kt * 16 + l15, c, q4);
+            for (int n = 0; n < ND; ++n) {
+              const Frag kf = O::tr_frag(k_lds + m * kTile * PK, PK, kb, n, l15, q4);
 #pragma unroll
-              for (int s = 0; s < QS; ++s) x[s] = O::mma(kf, qf[m][s][c], x[s]);
+              for (int s = 0; s < QS; ++s) dq[m][s][n] = O::mma(kf, sf[s], dq[m][s][n]);
             }
-            const unsigned bits = (unsigned)(word >> (kt * 16 + q4 * 4));
-            int4 p4 = make_int4(0, 0, 0, 0);
-            if constexpr (BIAS) p4 = *reinterpret_cast<const int4*>(pos_lds + kt * 16 + q4 * 4);
-            const int pj[4] = {p4.x, p4.y, p4.z, p4.w};
+          }
+        }
+        if constexpr (NT > 0) {
+#pragma unroll
+          for (int m = 0; m < M; ++m)
 #pragma unroll
             for (int s = 0; s < QS; ++s) {
-              float add[4] = {0.f, 0.f, 0.f, 0.f};
-              if constexpr (BIAS) {
-                const float* bias = bias_lds + m * slots;
-                if (side[s] != 0) {
-                  const float c = bias[side[s] > 0 ? R2 : 0];
+              const float c = m == 0 ? inv[m][s] : -lam * inv[m][s];
 #pragma unroll
-                  for (int j = 0; j < 4; ++j) add[j] = c;
-                } else {
-                  const int off = a.R - pos_q[s];
+              for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-                  for (int j = 0; j < 4; ++j) add[j] = bias[clamp_slot(pj[j] + off, R2)];
-                }
-              }
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                float p = __builtin_amdgcn_exp2f(fmaf(x[s][j], sl2, add[j]) - top[m][s]) * inv[m][s];
-                p = (bits >> j) & 1 ? p : 0.f;
-                const float g = p * (dp[s][u][j] - delta[m][s]);
-                ds[m][s][kt][j] = m == 0 ? g : -lam * g;
-              }
+                for (int j = 0; j < 4; ++j) sum_reg[m][s][kt0 + kt][j] = fmaf(ds[m][s][kt][j], c, sum_reg[m][s][kt0 + kt][j]);
             }
-          }
-        }
-#pragma unroll
-        for (int m = 0; m < M; ++m) {
-          Frag sf[QS];
-#pragma unroll
-          for (int s = 0; s < QS; ++s) sf[s] = O::acc_frag(&ds[m][s][kb * O::kSub]);
-#pragma unroll
-          for (int n = 0; n < ND; ++n) {
-            const Frag kf = O::tr_frag(k_lds + m * kTile * PK, PK, kb, n, l15, q4);
-#pragma unroll
-            for (int s = 0; s < QS; ++s) dq[m][s][n] = O::mma(kf, sf[s], dq[m][s][n]);
-          }
         }
       }
-    }
-    if constexpr (BIAS) {
-      if (want_sums) {
-        for (int turn = 0; turn < (a.hist_rows == 4 ? 1 : 4); ++turn) {  // one row of sums for all waves: they take turns
-          if (busy && (a.hist_rows == 4 || turn == wave)) {
-            float* tile = ds_lds + wave * 16 * kDsPitch;
+      if constexpr (BIAS && NT == 0) {
+        if (want_sums) {
+          const int pos_k = pos_lds[lane];
+          for (int turn = 0; turn < (a.hist_rows == 4 ? 1 : 4); ++turn) {  // one row of sums for all waves: they take turns
+            if (busy && (a.hist_rows == 4 || turn == wave)) {
+              float* buf = ds_lds + wave * 16 * kDsPitch;
 #pragma unroll
-            for (int m = 0; m < M; ++m)
+              for (int m = 0; m < M; ++m)
 #pragma unroll
-              for (int s = 0; s < QS; ++s) {
-                if (side[s] != 0) {
-                  float all = 0.f;
+                for (int s = 0; s < QS; ++s) {
+                  const float c = m == 0 ? inv[m][s] : -lam * inv[m][s];
+                  if (side[s] != 0) {
+                    float all = 0.f;
 #pragma unroll
-                  for (int kt = 0; kt < 4; ++kt)
+                    for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) all += ds[m][s][kt][j];
-                  if (side[s] > 0) hi[m] += all; else lo[m] += all;
-                } else {
+                      for (int j = 0; j < 4; ++j) all += ds[m][s][kt][j];
+                    if (side[s] > 0) hi[m] = fmaf(all, c, hi[m]); else lo[m] = fmaf(all, c, lo[m]);
+                  } else {
 #pragma unroll
-                  for (int kt = 0; kt < 4; ++kt)
-                    *reinterpret_cast<float4v*>(tile + l15 * kDsPitch + kt * 16 + q4 * 4) = ds[m][s][kt];
-                  wave_lds_fence();
-                  add_diagonals(a, my_sums + m * slots, tile, pos_lds, t0, q_first + s * 16, origin, lane, lo[m], hi[m]);
+                    for (int kt = 0; kt < 4; ++kt)
+                      *reinterpret_cast<float4v*>(buf + l15 * kDsPitch + kt * 16 + q4 * 4) = ds[m][s][kt] * c;
+                    wave_lds_fence();
+                    add_tile(a, my_sums + m * slots, buf, pos_k, token_q[s] + origin, t0, q_first + s * 16 + origin, lane, lo[m], hi[m]);
+                    wave_lds_fence();
+                  }
                 }
-              }
+            }
+            if (a.hist_rows != 4) __syncthreads();
           }
-          if (a.hist_rows != 4) __syncthreads();
         }
       }
+    };
+    if constexpr (NT == 0) {
+      while (walk.sample == b) tile(std::integral_constant<int, 0>{});
+    } else {
+      tile(std::integral_constant<int, 0>{});
+      tile(std::integral_constant<int, 4>{});
+      if constexpr (NT == 4) {
+        tile(std::integral_constant<int, 8>{});
+        tile(std::integral_constant<int, 12>{});
+      }
     }
-  }
 
-  if (busy) {
+    if (!busy) continue;
 #pragma unroll
     for (int s = 0; s < QS; ++s) {
       const int query = q_first + s * 16 + l15;
       if (query >= a.Lq) continue;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
+        const float c = a.scale * (m == 0 ? inv[m][s] : -lam * inv[m][s]);
         T* row = reinterpret_cast<T*>(a.dq) + b * a.dqs[0] + (long long)query * a.dqs[1] + (long long)(h * M + m) * a.dqs[2];
+        float* part = a.dq_part + ((split * rows + row0 + query) * M + m) * a.D;
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
           const int dim = n * 16 + q4 * 4;
-          if (dim < a.D) O::store4(row + dim, dq[m][s][n][0] * a.scale, dq[m][s][n][1] * a.scale, dq[m][s][n][2] * a.scale, dq[m][s][n][3] * a.scale);
+          const float4v g = dq[m][s][n] * c;
+          if (dim >= a.D) continue;
+          if (a.q_splits > 1) Ops<float>::store4(part + dim, g[0], g[1], g[2], g[3]);
+          else O::store4(row + dim, g[0], g[1], g[2], g[3]);
         }
       }
     }
   }
   if (!want_sums) return;
+  if constexpr (NT > 0) {  // the board's pairs, once for all samples
+    float* buf = ds_lds + wave * 16 * kDsPitch;
+    for (int turn = 0; turn < (a.hist_rows == 4 ? 1 : 4); ++turn) {
+      if (busy && (a.hist_rows == 4 || turn == wave)) {
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int s = 0; s < QS; ++s) {
+#pragma unroll
+              for (int kt = 0; kt < 4; ++kt)
+                *reinterpret_cast<float4v*>(buf + l15 * kDsPitch + kt * 16 + q4 * 4) = sum_reg[m][s][tt * 4 + kt];
+              wave_lds_fence();
+              add_tile(a, my_sums + m * slots, buf, token_pos(tt * kTile + lane, a.W), token_q[s], 0, 0, lane, lo[m], hi[m]);
+              wave_lds_fence();
+            }
+      }
+      if (a.hist_rows != 4) __syncthreads();
+    }
+  }
   // The clamped ends, wave by wave, then the four rows of sums in order.
 #pragma unroll
   for (int m = 0; m < M; ++m) {
@@ -306,7 +409,7 @@ __global__ __launch_bounds__(256) void enc_attn_bwd_q_kernel(EncAttnArgs a) {
     }
   }
   __syncthreads();
-  float* part = a.hist + (size_t)(bh * (long long)nqt + qt) * M * slots;
+  float* part = a.hist + (size_t)group_id * M * slots;
   for (int i = tid; i < M * slots; i += 256) {
     float s = sum_lds[i];
     if (a.hist_rows == 4) s = (s + sum_lds[M * slots + i]) + (sum_lds[2 * M * slots + i] + sum_lds[3 * M * slots + i]);
@@ -314,10 +417,10 @@ __global__ __launch_bounds__(256) void enc_attn_bwd_q_kernel(EncAttnArgs a) {
   }
 }
 
-// One 4-wave workgroup per (sample, key / value head, 64 KS keys); a wave owns 16 KS keys and walks the query tiles of every
-// query head that shares them.
-template <typename T, int D, int M, int KS, bool BIAS>
-__global__ __launch_bounds__(256) void enc_attn_bwd_k_kernel(EncAttnArgs a) {
+// One 4-wave workgroup per (key / value head, 64 KS keys, query range) and k_chunk samples; a wave owns 16 KS keys and walks the
+// query tiles of every query head that shares them.
+template <typename T, int D, int M, int KS, bool BIAS, int NT>
+__global__ __launch_bounds__(256, waves_of(D)) void enc_attn_bwd_k_kernel(EncAttnArgs a) {
   using O = Ops<T>;
   using Frag = typename O::Frag;
   constexpr int DV = D * M, DC = D / O::kDims, VC = DV / O::kDims, ND = D / 16, NV = DV / 16, NKB = 4 / O::kSub;
@@ -329,53 +432,33 @@ __global__ __launch_bounds__(256) void enc_attn_bwd_k_kernel(EncAttnArgs a) {
   float* top_lds = reinterpret_cast<float*>(pos_lds + kTile);
   float* inv_lds = top_lds + M * kTile;
   float* delta_lds = inv_lds + M * kTile;
-  float* bias_lds = delta_lds + M * kTile;
+  int* far_lds = reinterpret_cast<int*>(delta_lds + M * kTile);  // one flag per map (and padding)
+  float* bias_lds = reinterpret_cast<float*>(far_lds + 4);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, q4 = lane >> 4;
   const int nkt = (a.Lk + 64 * KS - 1) / (64 * KS);
-  const int id = xcd_order(blockIdx.x, gridDim.x);
-  const int kt_ = id % nkt, bkv = id / nkt;
-  const int b = bkv / a.KV, kvh = bkv - b * a.KV, group = a.H / a.KV;
+  int id = xcd_order(blockIdx.x, gridDim.x);
+  const int kt_ = id % nkt;
+  id /= nkt;
+  const int split = id % a.k_splits;
+  id /= a.k_splits;
+  const int kvh = id % a.KV, group = a.H / a.KV;
+  const int b_first = id / a.KV * a.k_chunk, b_last = b_first + a.k_chunk < a.B ? b_first + a.k_chunk : a.B;
   const int tiles = (a.Lk + kTile - 1) / kTile, qtiles = (a.Lq + kTile - 1) / kTile;
+  const int all = group * qtiles, per = (all + a.k_splits - 1) / a.k_splits;
+  const int s_first = split * per, s_last = s_first + per < all ? s_first + per : all;
   const int k_first = (kt_ * 4 + wave) * 16 * KS;
   const int R2 = 2 * a.R, slots = BIAS ? R2 + 1 : 0;
-
-  Frag kf[M][KS][DC], vf[KS][VC];
-  bool live[KS];
-  int pos_k[KS];
-  bool any = false;
-#pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    const int key = k_first + s * 16 + l15;
-    live[s] = key < a.Lk && (!a.words || ((a.words[(size_t)b * tiles + (key >> 6)] >> (key & 63)) & 1));
-    any |= live[s];
-    pos_k[s] = BIAS ? token_pos(key, a.W) : 0;
-#pragma unroll
-    for (int m = 0; m < M; ++m)
-      load_rows<T, DC>(kf[m][s], reinterpret_cast<const T*>(a.k) + b * a.ks[0] + (long long)key * a.ks[1] + (long long)(kvh * M + m) * a.ks[2], live[s],
-                       a.D, q4);
-    load_rows<T, VC>(vf[s], reinterpret_cast<const T*>(a.v) + b * a.vs[0] + (long long)key * a.vs[1] + kvh * a.vs[2], live[s], a.DV, q4);
-  }
-  float4v dk[M][KS][ND], dv[KS][NV];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) {
-#pragma unroll
-    for (int n = 0; n < NV; ++n) dv[s][n] = float4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int m = 0; m < M; ++m)
-#pragma unroll
-      for (int n = 0; n < ND; ++n) dk[m][s][n] = float4v{0.f, 0.f, 0.f, 0.f};
-  }
   const float sl2 = a.scale * kLog2E;
   const long long rows = (long long)a.B * a.H * a.Lq;
-  const bool busy = __ballot(any) != 0;                 // this wave has a key that takes part
-  const int steps = __syncthreads_or(any) ? group * qtiles : 0;  // the workgroup has one
-  const int origin = BIAS ? query_origin(a, b) : 0;
+  int pos_k[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) pos_k[s] = BIAS ? token_pos(k_first + s * 16 + l15, a.W) : 0;
 
   Stage<T, D> sq[M];
   Stage<T, DV> sg;
   float2 stat = make_float2(0.f, 0.f);  // waves 0 .. M - 1: maximum and 1 / sum of a query, waves M .. 2 M - 1: its delta
-  auto fetch = [&](int step) {
+  auto fetch = [&](int b, int step) {
     const int h = kvh * group + step / qtiles, t0 = (step % qtiles) * kTile;
     const unsigned long long word = range_word(t0, a.Lq);
 #pragma unroll
@@ -391,149 +474,267 @@ __global__ __launch_bounds__(256) void enc_attn_bwd_k_kernel(EncAttnArgs a) {
       stat.x = i < a.Lq ? a.delta[(which - M) * rows + row] : 0.f;
     }
   };
-  if (steps) fetch(0);
-  for (int step = 0; step < steps; ++step) {
-    const int h = kvh * group + step / qtiles, t0 = (step % qtiles) * kTile;
-    const float lam = M == 2 ? a.lam[h] : 0.f;
+  if (s_first < s_last) fetch(b_first, s_first);
+  int bias_head = -1;
+  float4v bias_reg[M][KS][NT ? NT * 4 : 1];  // boards (no key range, no shared heads): the bias of this wave's pairs
+  if constexpr (NT > 0) {
+    fill_bias(a, bias_lds, kvh, M, tid);
+    bias_head = kvh;
     __syncthreads();
 #pragma unroll
-    for (int m = 0; m < M; ++m) sq[m].store(q_lds + m * kTile * PQ, PQ, tid);
-    sg.store(g_lds, PG, tid);
-    if (tid < M * kTile) {
-      top_lds[tid] = stat.x;
-      inv_lds[tid] = stat.y;
-    } else if (tid < 2 * M * kTile) {
-      delta_lds[tid - M * kTile] = stat.x;
+    for (int qt = 0; qt < NT * 4; ++qt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int pos = token_pos(qt * 16 + q4 * 4 + j, a.W);
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int s = 0; s < KS; ++s) bias_reg[m][s][qt][j] = bias_lds[m * slots + clamp_slot(pos_k[s] - pos + a.R, R2)];
+      }
+  }
+
+  for (int b = b_first; b < b_last; ++b) {
+    const int origin = BIAS ? query_origin(a, b) : 0;
+    Frag kf[M][KS][DC], vf[KS][VC];
+    bool live[KS];
+    bool any = false;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int key = k_first + s * 16 + l15;
+      live[s] = key < a.Lk && (!a.words || ((a.words[(size_t)b * tiles + (key >> 6)] >> (key & 63)) & 1));
+      any |= live[s];
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+        load_rows<T, DC>(kf[m][s], reinterpret_cast<const T*>(a.k) + b * a.ks[0] + (long long)key * a.ks[1] + (long long)(kvh * M + m) * a.ks[2],
+                         live[s], a.D, q4);
+      load_rows<T, VC>(vf[s], reinterpret_cast<const T*>(a.v) + b * a.vs[0] + (long long)key * a.vs[1] + kvh * a.vs[2], live[s], a.DV, q4);
     }
-    if (BIAS && tid < kTile) pos_lds[tid] = token_pos(t0 + tid, a.W) + origin;
-    if (BIAS && step % qtiles == 0) fill_bias(a, bias_lds, h, M, tid);
-    __syncthreads();
-    if (step + 1 < steps) fetch(step + 1);
-    if (!busy) continue;
-    int side[KS];
+    float4v dk[M][KS][ND], dv[KS][NV];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) side[s] = BIAS ? clamped_side(a, k_first + s * 16, k_first + s * 16 + 15, t0 + origin, t0 + kTile - 1 + origin) : 0;
+    for (int s = 0; s < KS; ++s) {
 #pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) {
-      float4v pmix[KS][O::kSub], ds[M][KS][O::kSub];
+      for (int n = 0; n < NV; ++n) dv[s][n] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int u = 0; u < O::kSub; ++u) {
-        const int qt = kb * O::kSub + u;
-        float4v dp[KS];
+      for (int m = 0; m < M; ++m)
 #pragma unroll
-        for (int s = 0; s < KS; ++s) dp[s] = float4v{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < ND; ++n) dk[m][s][n] = float4v{0.f, 0.f, 0.f, 0.f};
+    }
+    const bool busy = __ballot(any) != 0;                         // this wave has a key that takes part
+    const int last = __syncthreads_or(any) ? s_last : s_first;    // the workgroup has one
+    // One staged query tile; qt0 is its first 16-query block where the bias is in registers.
+    auto tile = [&](int step, auto qt0_) {
+      constexpr int qt0 = decltype(qt0_)::value;
+      const int h = kvh * group + step / qtiles, t0 = (step % qtiles) * kTile;
+      const float lam = M == 2 ? a.lam[h] : 0.f;
+      __syncthreads();
 #pragma unroll
-        for (int c = 0; c < VC; ++c) {
-          const Frag gf = O::row_frag(g_lds, PG, qt * 16 + l15, c, q4);
+      for (int m = 0; m < M; ++m) sq[m].store(q_lds + m * kTile * PQ, PQ, tid);
+      sg.store(g_lds, PG, tid);
+      if (tid < M * kTile) {
+        top_lds[tid] = stat.x;
+        inv_lds[tid] = stat.y;
+        const bool far = __any(Exponent::far(stat.x * sl2));
+        if (lane == 0) far_lds[wave] = far;
+      } else if (tid < 2 * M * kTile) {
+        delta_lds[tid - M * kTile] = stat.x;
+      }
+      if (BIAS && NT == 0 && tid < kTile) pos_lds[tid] = token_pos(t0 + tid, a.W) + origin;
+      if (BIAS && h != bias_head) {
+        fill_bias(a, bias_lds, h, M, tid);
+        bias_head = h;
+      }
+      __syncthreads();
+      if (step + 1 < last) fetch(b, step + 1);
+      else if (b + 1 < b_last) fetch(b + 1, s_first);
+      if (!busy) return;
+      const bool far = far_lds[0] | (M == 2 ? far_lds[1] : 0);
+      int side[KS];
 #pragma unroll
-          for (int s = 0; s < KS; ++s) dp[s] = O::mma(gf, vf[s][c], dp[s]);
+      for (int s = 0; s < KS; ++s)
+        side[s] = BIAS && NT == 0 ? clamped_side(a, k_first + s * 16, k_first + s * 16 + 15, t0 + origin, t0 + kTile - 1 + origin) : 0;
+      auto block = [&](auto kb_, int kb) {
+        constexpr int kbc = decltype(kb_)::value;  // the block where it has to be a constant (registers), 0 otherwise
+        float4v pmix[KS][O::kSub], ds[M][KS][O::kSub];
+#pragma unroll
+        for (int u = 0; u < O::kSub; ++u) {
+          const int qt = kb * O::kSub + u;
+          const float4v del4 = *reinterpret_cast<const float4v*>(delta_lds + qt * 16 + q4 * 4);
+          float4v dp[KS];
+#pragma unroll
+          for (int s = 0; s < KS; ++s) dp[s] = -del4;  // dP - delta of the first map
+#pragma unroll
+          for (int c = 0; c < VC; ++c) {
+            const Frag gf = O::row_frag(g_lds, PG, qt * 16 + l15, c, q4);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) dp[s] = O::mma(gf, vf[s][c], dp[s]);
+          }
+          int4 p4 = make_int4(0, 0, 0, 0);
+          if constexpr (BIAS && NT == 0) p4 = *reinterpret_cast<const int4*>(pos_lds + qt * 16 + q4 * 4);
+          const int pj[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+          for (int m = 0; m < M; ++m) {
+            float4v x[KS];
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+              if constexpr (NT > 0) {
+                x[s] = bias_reg[m][s][qt0 + kbc * O::kSub + u];
+              } else if constexpr (BIAS) {
+                const float* bias = bias_lds + m * slots;
+                if (side[s] != 0) {
+                  const float c = bias[side[s] > 0 ? R2 : 0];
+                  x[s] = float4v{c, c, c, c};
+                } else {
+                  const int off = a.R + pos_k[s];
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) x[s][j] = bias[clamp_slot(off - pj[j], R2)];
+                }
+              } else {
+                x[s] = float4v{0.f, 0.f, 0.f, 0.f};
+              }
+            }
+#pragma unroll
+            for (int c = 0; c < DC; ++c) {
+              const Frag qf = O::row_frag(q_lds + m * kTile * PQ, PQ, qt * 16 + l15, c, q4);
+#pragma unroll
+              for (int s = 0; s < KS; ++s) x[s] = O::mma(qf, kf[m][s][c], x[s]);
+            }
+            const float4v top4 = *reinterpret_cast<const float4v*>(top_lds + m * kTile + qt * 16 + q4 * 4);
+            const float4v inv4 = *reinterpret_cast<const float4v*>(inv_lds + m * kTile + qt * 16 + q4 * 4);
+            float4v shift = {0.f, 0.f, 0.f, 0.f};
+            if (m > 0) shift = del4 - *reinterpret_cast<const float4v*>(delta_lds + m * kTile + qt * 16 + q4 * 4);
+            const float4v base4 = top4 * sl2;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+              // a masked key's column is garbage of its own (its rows were read as zeros) and is zeroed when written
+              if (far) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[s][j] = Exponent::far_(x[s][j], top4[j], sl2);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[s][j] = Exponent::near_(x[s][j], base4[j], sl2);
+              }
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float p = x[s][j] * inv4[j];
+                if (m == 0) {
+                  pmix[s][u][j] = p;
+                  ds[m][s][u][j] = p * dp[s][j];
+                } else {
+                  const float w = -lam * p;
+                  pmix[s][u][j] += w;
+                  ds[m][s][u][j] = w * (dp[s][j] + shift[j]);
+                }
+              }
+            }
+          }
         }
-        int4 p4 = make_int4(0, 0, 0, 0);
-        if constexpr (BIAS) p4 = *reinterpret_cast<const int4*>(pos_lds + qt * 16 + q4 * 4);
-        const int pj[4] = {p4.x, p4.y, p4.z, p4.w};
+        Frag pf[KS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) pf[s] = O::acc_frag(pmix[s]);
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          const Frag gf = O::tr_frag(g_lds, PG, kb, n, l15, q4);
+#pragma unroll
+          for (int s = 0; s < KS; ++s) dv[s][n] = O::mma(gf, pf[s], dv[s][n]);
+        }
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-          float4v x[KS];
+          Frag sf[KS];
 #pragma unroll
-          for (int s = 0; s < KS; ++s) x[s] = float4v{0.f, 0.f, 0.f, 0.f};
+          for (int s = 0; s < KS; ++s) sf[s] = O::acc_frag(ds[m][s]);
 #pragma unroll
-          for (int c = 0; c < DC; ++c) {
-            const Frag qf = O::row_frag(q_lds + m * kTile * PQ, PQ, qt * 16 + l15, c, q4);
+          for (int n = 0; n < ND; ++n) {
+            const Frag qf = O::tr_frag(q_lds + m * kTile * PQ, PQ, kb, n, l15, q4);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) x[s] = O::mma(qf, kf[m][s][c], x[s]);
-          }
-          const float4v top4 = *reinterpret_cast<const float4v*>(top_lds + m * kTile + qt * 16 + q4 * 4);
-          const float4v inv4 = *reinterpret_cast<const float4v*>(inv_lds + m * kTile + qt * 16 + q4 * 4);
-          const float4v del4 = *reinterpret_cast<const float4v*>(delta_lds + m * kTile + qt * 16 + q4 * 4);
-#pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            float add[4] = {0.f, 0.f, 0.f, 0.f};
-            if constexpr (BIAS) {
-              const float* bias = bias_lds + m * slots;
-              if (side[s] != 0) {
-                const float c = bias[side[s] > 0 ? R2 : 0];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) add[j] = c;
-              } else {
-                const int off = a.R + pos_k[s];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) add[j] = bias[clamp_slot(off - pj[j], R2)];
-              }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float p = __builtin_amdgcn_exp2f(fmaf(x[s][j], sl2, add[j]) - top4[j]) * inv4[j];
-              p = live[s] ? p : 0.f;
-              const float g = p * (dp[s][j] - del4[j]);
-              if (m == 0) {
-                pmix[s][u][j] = p;
-                ds[m][s][u][j] = g;
-              } else {
-                pmix[s][u][j] = fmaf(-lam, p, pmix[s][u][j]);
-                ds[m][s][u][j] = -lam * g;
-              }
-            }
+            for (int s = 0; s < KS; ++s) dk[m][s][n] = O::mma(qf, sf[s], dk[m][s][n]);
           }
         }
+      };
+      if constexpr (NT > 0) {
+        block(std::integral_constant<int, 0>{}, 0);
+        block(std::integral_constant<int, 1>{}, 1);
+        if constexpr (NKB == 4) {
+          block(std::integral_constant<int, 2>{}, 2);
+          block(std::integral_constant<int, 3>{}, 3);
+        }
+      } else {
+#pragma unroll 1
+        for (int kb = 0; kb < NKB; ++kb) block(std::integral_constant<int, 0>{}, kb);
       }
-      Frag pf[KS];
+    };
+    if constexpr (NT == 0) {
+      for (int step = s_first; step < last; ++step) tile(step, std::integral_constant<int, 0>{});
+    } else if (last > s_first) {
+      tile(0, std::integral_constant<int, 0>{});
+      tile(1, std::integral_constant<int, 4>{});
+      if constexpr (NT == 4) {
+        tile(2, std::integral_constant<int, 8>{});
+        if (last > 3) tile(3, std::integral_constant<int, 12>{});
+      }
+    }
+    if (last == s_first && b + 1 < b_last && s_first < s_last) fetch(b + 1, s_first);  // nothing took part: the tile under way was this sample's
 #pragma unroll
-      for (int s = 0; s < KS; ++s) pf[s] = O::acc_frag(pmix[s]);
+    for (int s = 0; s < KS; ++s) {
+      const int key = k_first + s * 16 + l15;
+      if (key >= a.Lk) continue;
+      const long long krow = ((long long)b * a.KV + kvh) * a.Lk + key;
+      float* part = a.kv_part + (split * ((long long)a.B * a.KV * a.Lk) + krow) * (M * a.D + a.DV);
+      T* dv_row = reinterpret_cast<T*>(a.dv) + b * a.dvs[0] + (long long)key * a.dvs[1] + kvh * a.dvs[2];
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
-        const Frag gf = O::tr_frag(g_lds, PG, kb, n, l15, q4);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) dv[s][n] = O::mma(gf, pf[s], dv[s][n]);
+        const int dim = n * 16 + q4 * 4;
+        if (dim >= a.DV) continue;
+        const float4v g = live[s] ? dv[s][n] : float4v{0.f, 0.f, 0.f, 0.f};
+        if (a.k_splits > 1) Ops<float>::store4(part + M * a.D + dim, g[0], g[1], g[2], g[3]);
+        else O::store4(dv_row + dim, g[0], g[1], g[2], g[3]);
       }
 #pragma unroll
       for (int m = 0; m < M; ++m) {
-        Frag sf[KS];
-#pragma unroll
-        for (int s = 0; s < KS; ++s) sf[s] = O::acc_frag(ds[m][s]);
+        T* dk_row = reinterpret_cast<T*>(a.dk) + b * a.dks[0] + (long long)key * a.dks[1] + (long long)(kvh * M + m) * a.dks[2];
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
-          const Frag qf = O::tr_frag(q_lds + m * kTile * PQ, PQ, kb, n, l15, q4);
-#pragma unroll
-          for (int s = 0; s < KS; ++s) dk[m][s][n] = O::mma(qf, sf[s], dk[m][s][n]);
+          const int dim = n * 16 + q4 * 4;
+          if (dim >= a.D) continue;
+          const float4v g = live[s] ? dk[m][s][n] * a.scale : float4v{0.f, 0.f, 0.f, 0.f};
+          if (a.k_splits > 1) Ops<float>::store4(part + m * a.D + dim, g[0], g[1], g[2], g[3]);
+          else O::store4(dk_row + dim, g[0], g[1], g[2], g[3]);
         }
-      }
-    }
-  }
-#pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    const int key = k_first + s * 16 + l15;
-    if (key >= a.Lk) continue;
-    T* dv_row = reinterpret_cast<T*>(a.dv) + b * a.dvs[0] + (long long)key * a.dvs[1] + kvh * a.dvs[2];
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int dim = n * 16 + q4 * 4;
-      if (dim < a.DV) O::store4(dv_row + dim, dv[s][n][0], dv[s][n][1], dv[s][n][2], dv[s][n][3]);
-    }
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-      T* dk_row = reinterpret_cast<T*>(a.dk) + b * a.dks[0] + (long long)key * a.dks[1] + (long long)(kvh * M + m) * a.dks[2];
-#pragma unroll
-      for (int n = 0; n < ND; ++n) {
-        const int dim = n * 16 + q4 * 4;
-        if (dim < a.D) O::store4(dk_row + dim, dk[m][s][n][0] * a.scale, dk[m][s][n][1] * a.scale, dk[m][s][n][2] * a.scale, dk[m][s][n][3] * a.scale);
       }
     }
   }
 }
 
-// mid[z][h M + m][slot] = sum of hist over a share of the (sample, query tile) workgroups of head h: one wave per share row, in order.
-__global__ __launch_bounds__(256) void enc_hist_sum_kernel(const float* hist, float* mid, int B, int H, int nqt, int M, int slots, int shares) {
+// dest (heads of `width` values) = sum over the splits of rows [S][B, G, L][pitch] from column `from`, in order: four values per thread.
+template <typename T>
+__global__ __launch_bounds__(256) void enc_grad_join_kernel(const float* part, int splits, int B, int G, int L, int pitch, int from, int maps, int width,
+                                                            T* dest, long long sb, long long st, long long sh) {
+  const int quads = maps * width / 4;
+  const long long rows = (long long)B * G * L, i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * quads) return;
+  const long long row = i / quads;
+  const int col = (int)(i - row * quads) * 4, m = col / width;
+  float4v s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int p = 0; p < splits; ++p) s += *reinterpret_cast<const float4v*>(part + (p * rows + row) * pitch + from + col);
+  const int token = (int)(row % L);
+  const long long bg = row / L;
+  const int b = (int)(bg / G), g = (int)(bg - (long long)b * G);
+  Ops<T>::store4(dest + b * sb + token * st + ((long long)g * maps + m) * sh + (col - m * width), s[0], s[1], s[2], s[3]);
+}
+
+// mid[z][h M + m][slot] = sum of hist over a share of head h's workgroups, `per_head` for each of `outer` sample chunks, in order.
+__global__ __launch_bounds__(256) void enc_hist_sum_kernel(const float* hist, float* mid, int outer, int H, int per_head, int M, int slots, int shares) {
   __shared__ float part[4][64];
   const int slot = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
   const int hm = blockIdx.y, h = hm / M, m = hm - h * M, z = blockIdx.z;
-  const int total = B * nqt, per = (total + shares - 1) / shares;
+  const int total = outer * per_head, per = (total + shares - 1) / shares;
   const int first = z * per, last = first + per < total ? first + per : total;
   float s = 0.f;
   if (slot < slots) {
 #pragma unroll 4
     for (int r = first + wave; r < last; r += 4) {
-      const int b = r / nqt, qt = r - b * nqt;
-      s += hist[(((size_t)b * H + h) * nqt + qt) * M * slots + (size_t)m * slots + slot];
+      const int o = r / per_head, i = r - o * per_head;
+      s += hist[(((size_t)o * H + h) * per_head + i) * M * slots + (size_t)m * slots + slot];
     }
   }
   part[wave][threadIdx.x & 63] = s;
@@ -584,9 +785,10 @@ __global__ __launch_bounds__(1024) void enc_dlam_kernel(const float* delta2, flo
   }
 }
 
-template <typename T, int D, int M, int S, bool BIAS>
+template <typename T, int D, int M, int S, bool BIAS, int NT = 0>
 int launch_bwd(EncAttnArgs a, hipStream_t stream) {
   using O = Ops<T>;
+  constexpr int NK = NT;  // the key-owned pass unrolls the same way where heads are not shared
   const size_t slots = BIAS ? 2 * a.R + 1 : 0;
   const size_t tiles = sizeof(T) * (size_t)kTile * (M * O::row_pitch(D) + O::row_pitch(D * M)) + kTile * sizeof(int);
   size_t lds_q = tiles;
@@ -597,28 +799,64 @@ int launch_bwd(EncAttnArgs a, hipStream_t stream) {
     if (lds_q + sizeof(float) * 4 * M * slots > kMaxLds / 2) a.hist_rows = 1;
     lds_q += sizeof(float) * a.hist_rows * M * slots;
   }
-  int rc = enc_lds(enc_attn_bwd_q_kernel<T, D, M, S, BIAS>, lds_q);
-  if (rc) return rc;
-  const size_t lds_k = tiles + sizeof(float) * (3 * M * kTile + M * slots);
-  rc = enc_lds(enc_attn_bwd_k_kernel<T, D, M, S, BIAS>, lds_k);
+  int rc = enc_lds(enc_attn_bwd_q_kernel<T, D, M, S, BIAS, NT>, lds_q);
   if (rc) return rc;
   const int nqt = (a.Lq + 64 * S - 1) / (64 * S), nkt = (a.Lk + 64 * S - 1) / (64 * S);
-  hipLaunchKernelGGL((enc_attn_bwd_q_kernel<T, D, M, S, BIAS>), dim3((unsigned)(a.B * a.H * nqt)), dim3(256), lds_q, stream, a);
+  hipLaunchKernelGGL((enc_attn_bwd_q_kernel<T, D, M, S, BIAS, NT>), dim3((unsigned)((a.B + a.q_chunk - 1) / a.q_chunk * a.H * nqt * a.q_splits)), dim3(256),
+                     lds_q, stream, a);
   rc = hip_err(hipGetLastError());
   if (rc) return rc;
-  if (!a.dk) return 0;
-  hipLaunchKernelGGL((enc_attn_bwd_k_kernel<T, D, M, S, BIAS>), dim3((unsigned)(a.B * a.KV * nkt)), dim3(256), lds_k, stream, a);
+  const size_t lds_k = tiles + sizeof(float) * (3 * M * kTile + 4 + M * slots);
+  const dim3 grid((unsigned)((a.B + a.k_chunk - 1) / a.k_chunk * a.KV * nkt * a.k_splits));
+  if (NK > 0 && (a.KV != a.H || a.k_splits > 1)) {
+    rc = enc_lds(enc_attn_bwd_k_kernel<T, D, M, S, BIAS, 0>, lds_k);
+    if (rc) return rc;
+    hipLaunchKernelGGL((enc_attn_bwd_k_kernel<T, D, M, S, BIAS, 0>), grid, dim3(256), lds_k, stream, a);
+  } else {
+    rc = enc_lds(enc_attn_bwd_k_kernel<T, D, M, S, BIAS, NK>, lds_k);
+    if (rc) return rc;
+    hipLaunchKernelGGL((enc_attn_bwd_k_kernel<T, D, M, S, BIAS, NK>), grid, dim3(256), lds_k, stream, a);
+  }
   return hip_err(hipGetLastError());
 }
 
 template <typename T>
+int join_grad(const EncAttnArgs& a, const float* part, int splits, int G, int L, int pitch, int from, int maps, int width, void* dest, const long long* st,
+              hipStream_t stream) {
+  const long long n = (long long)a.B * G * L * (maps * width / 4);
+  if ((n + 255) / 256 >= (1LL << 31)) return -15;
+  hipLaunchKernelGGL((enc_grad_join_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, part, splits, a.B, G, L, pitch, from, maps, width,
+                     reinterpret_cast<T*>(dest), st[0], st[1], st[2]);
+  return hip_err(hipGetLastError());
+}
+
+template <typename T>
+int join_grads(const EncAttnArgs& a, hipStream_t stream) {
+  if (a.q_splits > 1) {
+    const int rc = join_grad<T>(a, a.dq_part, a.q_splits, a.H, a.Lq, a.M * a.D, 0, a.M, a.D, a.dq, a.dqs, stream);
+    if (rc) return rc;
+  }
+  if (a.k_splits > 1) {
+    const int pitch = a.M * a.D + a.DV;
+    const int rc = join_grad<T>(a, a.kv_part, a.k_splits, a.KV, a.Lk, pitch, 0, a.M, a.D, a.dk, a.dks, stream);
+    if (rc) return rc;
+    return join_grad<T>(a, a.kv_part, a.k_splits, a.KV, a.Lk, pitch, a.M * a.D, 1, a.DV, a.dv, a.dvs, stream);
+  }
+  return 0;
+}
+
+template <typename T>
 int dispatch_bwd(const EncAttnArgs& a, hipStream_t stream) {
-  const int w = enc_width(a.D);
+  const int w = enc_width(a.D), nt = a.q_splits == 1 ? enc_board_tiles(a.table ? a.W : 0, a.Lk, a.D, a.M) : 0;
   if (a.M == 1) {
+    if (nt == 2) return launch_bwd<T, 32, 1, 2, true, 2>(a, stream);
+    if (nt == 4) return launch_bwd<T, 32, 1, 1, true, 4>(a, stream);
+    if (w == 32 && enc_columns(a.W, a.Lq, a.Lk, a.D, a.M, false) == 1) return launch_bwd<T, 32, 1, 1, true>(a, stream);
     if (w == 32) return launch_bwd<T, 32, 1, 2, true>(a, stream);
     if (w == 64) return launch_bwd<T, 64, 1, 2, true>(a, stream);
     return launch_bwd<T, 128, 1, 1, true>(a, stream);
   }
+  if (nt == 2) return launch_bwd<T, 32, 2, 1, true, 2>(a, stream);
   if (w == 32) return a.table ? launch_bwd<T, 32, 2, 1, true>(a, stream) : launch_bwd<T, 32, 2, 1, false>(a, stream);
   return a.table ? launch_bwd<T, 64, 2, 1, true>(a, stream) : launch_bwd<T, 64, 2, 1, false>(a, stream);
 }
@@ -627,37 +865,42 @@ int dispatch_bwd(const EncAttnArgs& a, hipStream_t stream) {
 
 extern "C" {
 
-// Queries per workgroup of the query-owned pass (rows of EncAttnArgs::hist per (sample, head): ceil(Lq / this)).
-int atri_enc_attn_bwd_queries(int D, int M) { return M == 1 && D <= 64 ? 128 : 64; }
-
-// dq, dk, dv (every element written), delta and, where hist is set, the sums of dS by position difference.
+// dq, dk, dv (every element written), delta and, where hist / dlam are set, the gradients of the table and of lam.
 int atri_enc_attn_bwd(const EncAttnArgs* args, hipStream_t stream) {
   if (!args) return -1;
   const EncAttnArgs& a = *args;
-  const int rc = enc_check(a);
+  int rc = enc_check(a);
   if (rc) return rc;
   if (!a.q || !a.k || !a.v || !a.dout || !a.dq || !a.dk || !a.dv || !a.stat || !a.o32 || !a.delta) return -17;
-  return a.bf16 ? dispatch_bwd<unsigned short>(a, stream) : dispatch_bwd<float>(a, stream);
-}
-
-// dtable [buckets, H M] from hist [B H nqt, M, slots]; mid is [shares, H M, slots] scratch; order / start list the slots of every bucket.
-int atri_enc_table_grad(const float* hist, float* mid, const int* order, const int* start, float* dtable, int B, int H, int M, int nqt, int slots,
-                        int buckets, int shares, hipStream_t stream) {
-  if (!hist || !mid || !order || !start || !dtable) return -17;
-  if (B < 1 || H < 1 || M < 1 || nqt < 1 || slots < 1 || buckets < 1 || shares < 1 || shares > 65535 || (long long)H * M > 65535) return -10;
-  if ((long long)B * nqt >= (1LL << 31) || (long long)buckets * H * M >= (1LL << 31) || (long long)slots * shares >= (1LL << 31)) return -15;
-  hipLaunchKernelGGL(enc_hist_sum_kernel, dim3((slots + 63) / 64, H * M, shares), dim3(256), 0, stream, hist, mid, B, H, nqt, M, slots, shares);
-  const int rc = hip_err(hipGetLastError());
+  const int slots = 2 * a.R + 1, hm = a.H * a.M;
+  if (a.hist) {
+    if (!a.table || !a.mid || !a.order || !a.start || !a.dtable) return -17;
+    if (a.buckets < 1 || a.shares < 1 || a.shares > 65535 || hm > 65535 || (long long)a.buckets * hm >= (1LL << 31) ||
+        (long long)slots * a.shares >= (1LL << 31))
+      return -15;
+  }
+  if (a.dlam && a.M != 2) return -14;
+  if ((a.q_splits > 1 && !a.dq_part) || (a.k_splits > 1 && !a.kv_part)) return -17;
+  rc = a.bf16 ? dispatch_bwd<unsigned short>(a, stream) : dispatch_bwd<float>(a, stream);
   if (rc) return rc;
-  hipLaunchKernelGGL(enc_bucket_sum_kernel, dim3((unsigned)((buckets * H * M + 3) / 4)), dim3(256), 0, stream, mid, order, start, dtable, buckets, H * M,
-                     slots, shares);
-  return hip_err(hipGetLastError());
-}
-
-int atri_enc_dlam(const float* delta2, float* dlam, int B, int H, int Lq, hipStream_t stream) {
-  if (!delta2 || !dlam || B < 1 || H < 1 || Lq < 1) return -10;
-  hipLaunchKernelGGL(enc_dlam_kernel, dim3(H), dim3(1024), 0, stream, delta2, dlam, B, H, Lq);
-  return hip_err(hipGetLastError());
+  rc = a.bf16 ? join_grads<unsigned short>(a, stream) : join_grads<float>(a, stream);
+  if (rc) return rc;
+  if (a.hist) {
+    const int per = 64 * enc_columns(a.table ? a.W : 0, a.Lq, a.Lk, a.D, a.M, false), nqt = (a.Lq + per - 1) / per;
+    hipLaunchKernelGGL(enc_hist_sum_kernel, dim3((slots + 63) / 64, hm, a.shares), dim3(256), 0, stream, a.hist, a.mid,
+                       (a.B + a.q_chunk - 1) / a.q_chunk, a.H, nqt * a.q_splits, a.M, slots, a.shares);
+    rc = hip_err(hipGetLastError());
+    if (rc) return rc;
+    hipLaunchKernelGGL(enc_bucket_sum_kernel, dim3((unsigned)((a.buckets * hm + 3) / 4)), dim3(256), 0, stream, a.mid, a.order, a.start, a.dtable, a.buckets, hm,
+                       slots, a.shares);
+    rc = hip_err(hipGetLastError());
+    if (rc) return rc;
+  }
+  if (a.dlam) {
+    hipLaunchKernelGGL(enc_dlam_kernel, dim3(a.H), dim3(1024), 0, stream, a.delta + (long long)a.B * a.H * a.Lq, a.dlam, a.B, a.H, a.Lq);
+    rc = hip_err(hipGetLastError());
+  }
+  return rc;
 }
 
 }  // extern "C"

@@ -1,18 +1,21 @@
 // Forward pass of the encoder attention operators (see encoder_attn.hpp for the mathematics and the operand layout), the
 // join of key splits, and the key-validity words.
+#include <type_traits>
+
 #include "encoder_attn.hpp"
 
 using namespace atrihip;
 
 namespace {
 
-// One 4-wave workgroup per (sample, head, 64 QS queries[, key split]); a wave owns 16 QS queries and walks the key tiles with the
+// One 4-wave workgroup per (head, 64 QS queries, key split) and `chunk` samples, one after the other: the bias is laid out once
+// and the next sample's first tile loads while this one's last is multiplied.  A wave owns 16 QS queries and walks the key tiles with the
 // running maximum and sum of the softmax; per lane the sum is partial (its own keys) until the end.
 // PL bf16 fragments per probability: one for inference (rounded like the values it meets); three, all 24 bits, when a backward
 // pass follows, for delta = dO . o has to match dP = dO V^T to 32 bits: the gradients of the table and of lam are sums
 // of p (dP - delta) in which everything but the error of delta cancels (with one fragment they were 1e-3 off).
-template <typename T, int D, int M, int QS, bool BIAS, int PL>
-__global__ __launch_bounds__(256) void enc_attn_fwd_kernel(EncAttnArgs a) {
+template <typename T, int D, int M, int QS, bool BIAS, int PL, int NT>
+__global__ __launch_bounds__(256, NT > 0 ? 2 : 1) void enc_attn_fwd_kernel(EncAttnArgs a) {
   using O = Ops<T>;
   using Frag = typename O::Frag;
   constexpr int DV = D * M, DC = D / O::kDims, NV = DV / 16, NKB = 4 / O::kSub;
@@ -28,216 +31,266 @@ __global__ __launch_bounds__(256) void enc_attn_fwd_kernel(EncAttnArgs a) {
   int id = xcd_order(blockIdx.x, gridDim.x);
   const int qt = id % nqt;
   id /= nqt;
-  const int split = id % a.splits, bh = id / a.splits;
-  const int b = bh / a.H, h = bh - b * a.H, kvh = h / (a.H / a.KV);
+  const int split = id % a.splits;
+  id /= a.splits;
+  const int h = id % a.H, kvh = h / (a.H / a.KV);
+  const int b_first = id / a.H * a.chunk, b_last = b_first + a.chunk < a.B ? b_first + a.chunk : a.B;
   const int tiles = (a.Lk + kTile - 1) / kTile;
   const int per = (tiles + a.splits - 1) / a.splits;
   const int t_first = split * per, t_last = t_first + per < tiles ? t_first + per : tiles;
-
-  const T* kb_ = reinterpret_cast<const T*>(a.k) + b * a.ks[0] + (long long)kvh * M * a.ks[2];
-  const T* vb_ = reinterpret_cast<const T*>(a.v) + b * a.vs[0] + kvh * a.vs[2];
   const int R2 = 2 * a.R;
-  if constexpr (BIAS) fill_bias(a, bias_lds, h, M, tid);
-
   const int q_first = (qt * 4 + wave) * 16 * QS;
   const bool busy = q_first < a.Lq;  // wave-uniform
-  const int origin = BIAS ? query_origin(a, b) : 0;
-  Frag qf[M][QS][DC];
-  int pos_q[QS];
-#pragma unroll
-  for (int s = 0; s < QS; ++s) {
-    const int query = q_first + s * 16 + l15;
-    pos_q[s] = BIAS ? token_pos(query, a.W) + origin : 0;
-#pragma unroll
-    for (int m = 0; m < M; ++m)
-      load_rows<T, DC>(qf[m][s], reinterpret_cast<const T*>(a.q) + b * a.qs[0] + (long long)query * a.qs[1] + (long long)(h * M + m) * a.qs[2],
-                       query < a.Lq, a.D, q4);
-  }
-  float4v o[M][QS][NV];
-  float run_max[M][QS], run_sum[M][QS];
-#pragma unroll
-  for (int m = 0; m < M; ++m)
-#pragma unroll
-    for (int s = 0; s < QS; ++s) {
-      run_max[m][s] = -INFINITY;
-      run_sum[m][s] = 0.f;
-#pragma unroll
-      for (int n = 0; n < NV; ++n) o[m][s][n] = float4v{0.f, 0.f, 0.f, 0.f};
-    }
   const float sl2 = a.scale * kLog2E;
+  const float lam = M == 2 ? a.lam[h] : 0.f;
 
   Stage<T, D> sk[M];
   Stage<T, DV> sv;
-  TileWalk walk;
-  walk.start(a.words ? a.words + (size_t)b * tiles : nullptr, a.Lk, t_first, t_last);
-  int t = walk.next();
-  if (t < t_last) {
+  auto fetch = [&](const TileWalk& w) {
+    const T* kb = reinterpret_cast<const T*>(a.k) + w.sample * a.ks[0] + (long long)kvh * M * a.ks[2];
 #pragma unroll
-    for (int m = 0; m < M; ++m) sk[m].load(kb_ + m * a.ks[2], a.ks[1], t * kTile, walk.word, a.D, tid);
-    sv.load(vb_, a.vs[1], t * kTile, walk.word, a.DV, tid);
-  }
-  while (t < t_last) {
-    const unsigned long long word = walk.word;
-    const int t0 = t * kTile;
-    __syncthreads();  // every wave is past its reads of the previous tile
+    for (int m = 0; m < M; ++m) sk[m].load(kb + m * a.ks[2], a.ks[1], w.tile * kTile, w.word, a.D, tid);
+    sv.load(reinterpret_cast<const T*>(a.v) + w.sample * a.vs[0] + kvh * a.vs[2], a.vs[1], w.tile * kTile, w.word, a.DV, tid);
+  };
+  Frag qf[M][QS][DC];
+  auto fetch_queries = [&](int b) {
 #pragma unroll
-    for (int m = 0; m < M; ++m) sk[m].store(k_lds + m * kTile * PK, PK, tid);
-    sv.store(v_lds, PV, tid);
-    if (BIAS && tid < kTile) pos_lds[tid] = token_pos(t0 + tid, a.W);
-    __syncthreads();
-    t = walk.next();
-    if (t < t_last) {  // the next tile's loads run under this tile's products
+    for (int s = 0; s < QS; ++s) {
+      const int query = q_first + s * 16 + l15;
 #pragma unroll
-      for (int m = 0; m < M; ++m) sk[m].load(kb_ + m * a.ks[2], a.ks[1], t * kTile, walk.word, a.D, tid);
-      sv.load(vb_, a.vs[1], t * kTile, walk.word, a.DV, tid);
+      for (int m = 0; m < M; ++m)
+        load_rows<T, DC>(qf[m][s], reinterpret_cast<const T*>(a.q) + b * a.qs[0] + (long long)query * a.qs[1] + (long long)(h * M + m) * a.qs[2],
+                         query < a.Lq, a.D, q4);
     }
-    if (!busy) continue;
-
-    float4v st[M][QS][4];
+  };
+  TileWalk walk;
+  if constexpr (NT == 0) {
+    walk.start(a, b_first, b_last, t_first, t_last);
+  } else {
+    walk.sample = b_first;
+    walk.tile = 0;
+    walk.word = board_word(a, b_first, 0);
+  }
+  if (walk.sample < b_last) fetch(walk);
+  fetch_queries(b_first);
+  if constexpr (BIAS) fill_bias(a, bias_lds, h, M, tid);
+  int token_q[QS];
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
+  for (int s = 0; s < QS; ++s) token_q[s] = BIAS ? token_pos(q_first + s * 16 + l15, a.W) : 0;
+  float4v bias_reg[M][QS][NT ? NT * 4 : 1];
+  if constexpr (NT > 0) {
+    __syncthreads();
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
+    for (int kt = 0; kt < NT * 4; ++kt)
 #pragma unroll
-        for (int s = 0; s < QS; ++s) st[m][s][kt] = float4v{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < 4; ++j) {
+        const int key = kt * 16 + q4 * 4 + j, pos = token_pos(key, a.W);
 #pragma unroll
-        for (int c = 0; c < DC; ++c) {
-          const Frag kf = O::row_frag(k_lds + m * kTile * PK, PK, kt * 16 + l15, c, q4);
+        for (int m = 0; m < M; ++m)
 #pragma unroll
-          for (int s = 0; s < QS; ++s) st[m][s][kt] = O::mma(kf, qf[m][s][c], st[m][s][kt]);
-        }
+          for (int s = 0; s < QS; ++s) bias_reg[m][s][kt][j] = key < a.Lk ? bias_lds[m * (R2 + 1) + clamp_slot(pos - token_q[s] + a.R, R2)] : -INFINITY;
       }
+  }
+
+  for (int b = b_first; b < b_last; ++b) {
+    const int origin = BIAS ? query_origin(a, b) : 0;
+    float4v o[M][QS][NV];
+    float run_max[M][QS], run_sum[M][QS];
+#pragma unroll
+    for (int m = 0; m < M; ++m)
 #pragma unroll
       for (int s = 0; s < QS; ++s) {
-        float4v* x = st[m][s];
-        if constexpr (BIAS) {
-          const float* bias = bias_lds + m * (R2 + 1);
-          const int qa = q_first + s * 16 + origin;
-          const int side = clamped_side(a, t0, t0 + kTile - 1, qa, qa + 15);
-          if (side != 0) {
-            const float c = bias[side > 0 ? R2 : 0];
+        run_max[m][s] = -INFINITY;
+        run_sum[m][s] = 0.f;
 #pragma unroll
-            for (int kt = 0; kt < 4; ++kt)
+        for (int n = 0; n < NV; ++n) o[m][s][n] = float4v{0.f, 0.f, 0.f, 0.f};
+      }
+    // One staged tile; kt0 is its first 16-key block where the bias is in registers.
+    auto tile = [&](auto kt0_) {
+      constexpr int kt0 = decltype(kt0_)::value;
+      // tail keys of a board are -inf in its bias already
+      const unsigned long long word = NT > 0 && !a.words ? ~0ULL : walk.word;
+      const int t0 = walk.tile * kTile;
+      __syncthreads();  // every wave is past its reads of the previous tile
 #pragma unroll
-              for (int j = 0; j < 4; ++j) x[kt][j] = fmaf(x[kt][j], sl2, c);
+      for (int m = 0; m < M; ++m) sk[m].store(k_lds + m * kTile * PK, PK, tid);
+      sv.store(v_lds, PV, tid);
+      if (BIAS && NT == 0 && tid < kTile) pos_lds[tid] = token_pos(t0 + tid, a.W);
+      __syncthreads();
+      if constexpr (NT == 0) {
+        walk.next();
+      } else {
+        constexpr bool last = kt0 / 4 + 1 == NT;
+        walk.tile = last ? 0 : kt0 / 4 + 1;
+        walk.sample = b + (last ? 1 : 0);
+        if (walk.sample < b_last) walk.word = board_word(a, walk.sample, walk.tile);
+      }
+      if (walk.sample < b_last) fetch(walk);  // the next tile's loads (this sample's or the next one's) run under this tile's products
+      if (!busy) return;
+
+      float4v st[M][QS][4];
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+          if constexpr (NT > 0) {
+#pragma unroll
+            for (int s = 0; s < QS; ++s) st[m][s][kt] = bias_reg[m][s][kt0 + kt];
+          } else if constexpr (BIAS) {
+            const float* bias = bias_lds + m * (R2 + 1);
+            const int4 p = *reinterpret_cast<const int4*>(pos_lds + kt * 16 + q4 * 4);
+            const int pj[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+            for (int s = 0; s < QS; ++s) {
+              const int qa = q_first + s * 16 + origin;
+              const int side = clamped_side(a, t0, t0 + kTile - 1, qa, qa + 15);
+              if (side != 0) {
+                const float c = bias[side > 0 ? R2 : 0];
+                st[m][s][kt] = float4v{c, c, c, c};
+              } else {
+                const int off = a.R - token_q[s] - origin;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) st[m][s][kt][j] = bias[clamp_slot(pj[j] + off, R2)];
+              }
+            }
           } else {
-            const int off = a.R - pos_q[s];
+#pragma unroll
+            for (int s = 0; s < QS; ++s) st[m][s][kt] = float4v{0.f, 0.f, 0.f, 0.f};
+          }
+#pragma unroll
+          for (int c = 0; c < DC; ++c) {
+            const Frag kf = O::row_frag(k_lds + m * kTile * PK, PK, kt * 16 + l15, c, q4);
+#pragma unroll
+            for (int s = 0; s < QS; ++s) st[m][s][kt] = O::mma(kf, qf[m][s][c], st[m][s][kt]);
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < QS; ++s) {
+          float4v* x = st[m][s];
+          if (word != ~0ULL) {
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) {
-              const int4 p = *reinterpret_cast<const int4*>(pos_lds + kt * 16 + q4 * 4);
-              const int pj[4] = {p.x, p.y, p.z, p.w};
+              const unsigned bits = (unsigned)(word >> (kt * 16 + q4 * 4));
 #pragma unroll
-              for (int j = 0; j < 4; ++j) x[kt][j] = fmaf(x[kt][j], sl2, bias[clamp_slot(pj[j] + off, R2)]);
+              for (int j = 0; j < 4; ++j) x[kt][j] = (bits >> j) & 1 ? x[kt][j] : -INFINITY;
             }
           }
-        } else {
+          float top = run_max[m][s];
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[kt][j] *= sl2;
-        }
-        if (word != ~0ULL) {
+            for (int j = 0; j < 4; ++j) top = fmaxf(top, x[kt][j]);
+          top = quad_row_max(top);
+          const float from = top == -INFINITY ? 0.f : top;  // nothing seen yet: exp2(-inf - 0) = 0, never inf - inf
+          const float base = from * sl2;
+          float fade, sum = 0.f;
+          if (__any(Exponent::far(base))) {
+            fade = Exponent::far_(run_max[m][s], from, sl2);
 #pragma unroll
-          for (int kt = 0; kt < 4; ++kt) {
-            const unsigned bits = (unsigned)(word >> (kt * 16 + q4 * 4));
+            for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[kt][j] = (bits >> j) & 1 ? x[kt][j] : -INFINITY;
+              for (int j = 0; j < 4; ++j) x[kt][j] = Exponent::far_(x[kt][j], from, sl2);
+          } else {
+            fade = __builtin_amdgcn_exp2f(run_max[m][s] * sl2 - base);
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) x[kt][j] = Exponent::near_(x[kt][j], base, sl2);
+          }
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum += x[kt][j];
+          run_max[m][s] = top;
+          run_sum[m][s] = fmaf(run_sum[m][s], fade, sum);
+          if (__any(fade != 1.0f)) {
+#pragma unroll
+            for (int n = 0; n < NV; ++n)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) o[m][s][n][j] *= fade;
           }
         }
-        float top = run_max[m][s];
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) top = fmaxf(top, x[kt][j]);
-        top = quad_row_max(top);
-        const float base = top == -INFINITY ? 0.f : top;  // nothing seen yet: exp2(-inf - 0) = 0, never inf - inf
-        const float fade = __builtin_amdgcn_exp2f(run_max[m][s] - base);
-        run_max[m][s] = top;
-        float sum = 0.f;
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[kt][j] = __builtin_amdgcn_exp2f(x[kt][j] - base);
-            sum += x[kt][j];
-          }
-        run_sum[m][s] = fmaf(run_sum[m][s], fade, sum);
-#pragma unroll
-        for (int n = 0; n < NV; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[m][s][n][j] *= fade;
       }
-    }
 #pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) {
-      Frag pf[M][QS][PL];
-#pragma unroll
-      for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int s = 0; s < QS; ++s)
-#pragma unroll
-          for (int p = 0; p < PL; ++p) {
-            pf[m][s][p] = O::acc_frag(&st[m][s][kb * O::kSub]);
-            if (p + 1 < PL) O::take(&st[m][s][kb * O::kSub], pf[m][s][p]);
-          }
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        const Frag vf = O::tr_frag(v_lds, PV, kb, n, l15, q4);
+      for (int kb = 0; kb < NKB; ++kb) {
+        Frag pf[M][QS][PL];
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
           for (int s = 0; s < QS; ++s)
 #pragma unroll
-            for (int p = PL - 1; p >= 0; --p) o[m][s][n] = O::mma(vf, pf[m][s][p], o[m][s][n]);
-      }
-    }
-  }
-  if (!busy) return;
-
-  const long long rows = (long long)a.B * a.H * a.Lq;
-  const float lam = M == 2 ? a.lam[h] : 0.f;
+            for (int p = 0; p < PL; ++p) {
+              pf[m][s][p] = O::acc_frag(&st[m][s][kb * O::kSub]);
+              if (p + 1 < PL) O::take(&st[m][s][kb * O::kSub], pf[m][s][p]);
+            }
 #pragma unroll
-  for (int s = 0; s < QS; ++s) {
-    const int query = q_first + s * 16 + l15;
-    float inv[M];
-    const long long row = (long long)bh * a.Lq + query;
+        for (int n = 0; n < NV; ++n) {
+          const Frag vf = O::tr_frag(v_lds, PV, kb, n, l15, q4);
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      const float sum = quad_row_sum(run_sum[m][s]);
-      inv[m] = sum == 0.f ? 0.f : 1.0f / sum;
-      if (query < a.Lq && q4 == 0) {
-        if (a.splits > 1) {
-          float* ml = a.part_ml + 2 * (((long long)split * M + m) * rows + row);
-          ml[0] = run_max[m][s];
-          ml[1] = sum;
-        } else if (a.stat) {
-          *reinterpret_cast<float2*>(a.stat + 2 * (m * rows + row)) = make_float2(sum == 0.f ? INFINITY : run_max[m][s], inv[m]);
+          for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int s = 0; s < QS; ++s)
+#pragma unroll
+              for (int p = PL - 1; p >= 0; --p) o[m][s][n] = O::mma(vf, pf[m][s][p], o[m][s][n]);
         }
       }
+    };
+    if constexpr (NT == 0) {
+      while (walk.sample == b) tile(std::integral_constant<int, 0>{});
+    } else {
+      tile(std::integral_constant<int, 0>{});
+      tile(std::integral_constant<int, 4>{});
+      if constexpr (NT == 4) {
+        tile(std::integral_constant<int, 8>{});
+        tile(std::integral_constant<int, 12>{});
+      }
     }
-    if (query >= a.Lq) continue;
+    if (b + 1 < b_last) fetch_queries(b + 1);
+    if (!busy) continue;
+    const long long rows = (long long)a.B * a.H * a.Lq;
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int dim = n * 16 + q4 * 4;
-      if (dim >= a.DV) continue;
-      float4v r[M];
+    for (int s = 0; s < QS; ++s) {
+      const int query = q_first + s * 16 + l15;
+      float inv[M];
+      const long long row = ((long long)b * a.H + h) * a.Lq + query;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
-        r[m] = o[m][s][n];
-        if (a.splits > 1) {
-          Ops<float>::store4(a.part_o + (((long long)split * M + m) * rows + row) * a.DV + dim, r[m][0], r[m][1], r[m][2], r[m][3]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) r[m][j] *= inv[m];
-          if (a.o32) Ops<float>::store4(a.o32 + b * a.o32s[0] + (long long)query * a.o32s[1] + h * a.o32s[2] + m * a.o32s[3] + dim, r[m][0], r[m][1], r[m][2], r[m][3]);
+        const float sum = quad_row_sum(run_sum[m][s]);
+        inv[m] = sum == 0.f ? 0.f : 1.0f / sum;
+        if (query < a.Lq && q4 == 0) {
+          if (a.splits > 1) {
+            float* ml = a.part_ml + 2 * (((long long)split * M + m) * rows + row);
+            ml[0] = run_max[m][s];
+            ml[1] = sum;
+          } else if (a.stat) {
+            *reinterpret_cast<float2*>(a.stat + 2 * (m * rows + row)) = make_float2(sum == 0.f ? INFINITY : run_max[m][s], inv[m]);
+          }
         }
       }
-      if (a.splits > 1) continue;
-      if constexpr (M == 2) {
+      if (query >= a.Lq) continue;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) r[0][j] = fmaf(-lam, r[1][j], r[0][j]);
+      for (int n = 0; n < NV; ++n) {
+        const int dim = n * 16 + q4 * 4;
+        if (dim >= a.DV) continue;
+        float4v r[M];
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          r[m] = o[m][s][n];
+          if (a.splits > 1) {
+            Ops<float>::store4(a.part_o + (((long long)split * M + m) * rows + row) * a.DV + dim, r[m][0], r[m][1], r[m][2], r[m][3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[m][j] *= inv[m];
+            if (a.o32) Ops<float>::store4(a.o32 + b * a.o32s[0] + (long long)query * a.o32s[1] + h * a.o32s[2] + m * a.o32s[3] + dim, r[m][0], r[m][1], r[m][2], r[m][3]);
+          }
+        }
+        if (a.splits > 1) continue;
+        if constexpr (M == 2) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) r[0][j] = fmaf(-lam, r[1][j], r[0][j]);
+        }
+        O::store4(reinterpret_cast<T*>(a.out) + b * a.os[0] + (long long)query * a.os[1] + h * a.os[2] + dim, r[0][0], r[0][1], r[0][2], r[0][3]);
       }
-      O::store4(reinterpret_cast<T*>(a.out) + b * a.os[0] + (long long)query * a.os[1] + h * a.os[2] + dim, r[0][0], r[0][1], r[0][2], r[0][3]);
     }
   }
 }
@@ -254,6 +307,7 @@ __global__ __launch_bounds__(256) void enc_attn_join_kernel(EncAttnArgs a) {
   const int query = (int)(row % a.Lq);
   const long long bh = row / a.Lq;
   const int b = (int)(bh / a.H), h = (int)(bh - (long long)b * a.H);
+  const float sl2 = a.scale * kLog2E;
   float4v r[M];
 #pragma unroll
   for (int m = 0; m < M; ++m) {
@@ -262,11 +316,13 @@ __global__ __launch_bounds__(256) void enc_attn_join_kernel(EncAttnArgs a) {
     const long long step = (long long)M * rows;
     float top = -INFINITY;
     for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[2 * s * step]);
-    const float base = top == -INFINITY ? 0.f : top;
+    const float from = top == -INFINITY ? 0.f : top, base = from * sl2;
     float sum = 0.f;
     float4v acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int s = 0; s < a.splits; ++s) {
-      const float w = __builtin_amdgcn_exp2f(ml[2 * s * step] - base);
+      const float t = ml[2 * s * step];
+      const float w = Exponent::far(base) ? Exponent::far_(t, from, sl2) : __builtin_amdgcn_exp2f(t * sl2 - base);
       const float4v p = *reinterpret_cast<const float4v*>(po + s * step * a.DV);
       sum = fmaf(ml[2 * s * step + 1], w, sum);
 #pragma unroll
@@ -297,35 +353,39 @@ __global__ __launch_bounds__(256) void key_words_kernel(const unsigned char* mas
   if ((threadIdx.x & 63) == 0) words[w] = bits;
 }
 
-template <typename T, int D, int M, int QS, bool BIAS, int PL>
+template <typename T, int D, int M, int QS, bool BIAS, int PL, int NT>
 int launch_fwd_planes(const EncAttnArgs& a, hipStream_t stream) {
   using O = Ops<T>;
   size_t lds = sizeof(T) * (size_t)kTile * (M * O::row_pitch(D) + O::tr_pitch(D * M)) + kTile * sizeof(int);
   if (BIAS) lds += sizeof(float) * (size_t)M * (2 * a.R + 1);
-  const int rc = enc_lds(enc_attn_fwd_kernel<T, D, M, QS, BIAS, PL>, lds);
+  const int rc = enc_lds(enc_attn_fwd_kernel<T, D, M, QS, BIAS, PL, NT>, lds);
   if (rc) return rc;
   const int nqt = (a.Lq + 64 * QS - 1) / (64 * QS);
-  hipLaunchKernelGGL((enc_attn_fwd_kernel<T, D, M, QS, BIAS, PL>), dim3((unsigned)(a.B * a.H * nqt * a.splits)), dim3(256), lds, stream, a);
+  hipLaunchKernelGGL((enc_attn_fwd_kernel<T, D, M, QS, BIAS, PL, NT>), dim3((unsigned)((a.B + a.chunk - 1) / a.chunk * a.H * nqt * a.splits)), dim3(256), lds,
+                     stream, a);
   return hip_err(hipGetLastError());
 }
 
-template <typename T, int D, int M, int QS, bool BIAS>
+template <typename T, int D, int M, int QS, bool BIAS, int NT = 0>
 int launch_fwd(const EncAttnArgs& a, hipStream_t stream) {
   if constexpr (sizeof(T) == 2) {
-    if (a.o32) return launch_fwd_planes<T, D, M, QS, BIAS, 3>(a, stream);
+    if (a.o32) return launch_fwd_planes<T, D, M, QS, BIAS, 3, NT>(a, stream);
   }
-  return launch_fwd_planes<T, D, M, QS, BIAS, 1>(a, stream);
+  return launch_fwd_planes<T, D, M, QS, BIAS, 1, NT>(a, stream);
 }
 
 template <typename T>
 int dispatch_fwd(const EncAttnArgs& a, hipStream_t stream) {
-  const int w = enc_width(a.D);
+  const int w = enc_width(a.D), nt = a.splits == 1 ? enc_board_tiles(a.table ? a.W : 0, a.Lk, a.D, a.M) : 0;
+  const bool two = enc_columns(a.table ? a.W : 0, a.Lq, a.Lk, a.D, a.M, true) == 2;
   if (a.M == 1) {
-    const bool wide = a.Lq > 64;  // two query tiles per wave once they exist: every staged fragment feeds two products
-    if (w == 32) return wide ? launch_fwd<T, 32, 1, 2, true>(a, stream) : launch_fwd<T, 32, 1, 1, true>(a, stream);
-    if (w == 64) return wide ? launch_fwd<T, 64, 1, 2, true>(a, stream) : launch_fwd<T, 64, 1, 1, true>(a, stream);
+    if (nt == 2) return launch_fwd<T, 32, 1, 2, true, 2>(a, stream);
+    if (nt == 4) return launch_fwd<T, 32, 1, 1, true, 4>(a, stream);
+    if (w == 32) return two ? launch_fwd<T, 32, 1, 2, true>(a, stream) : launch_fwd<T, 32, 1, 1, true>(a, stream);
+    if (w == 64) return two ? launch_fwd<T, 64, 1, 2, true>(a, stream) : launch_fwd<T, 64, 1, 1, true>(a, stream);
     return launch_fwd<T, 128, 1, 1, true>(a, stream);
   }
+  if (nt == 2) return launch_fwd<T, 32, 2, 1, true, 2>(a, stream);
   if (w == 32) return a.table ? launch_fwd<T, 32, 2, 1, true>(a, stream) : launch_fwd<T, 32, 2, 1, false>(a, stream);
   return a.table ? launch_fwd<T, 64, 2, 1, true>(a, stream) : launch_fwd<T, 64, 2, 1, false>(a, stream);
 }
@@ -336,15 +396,8 @@ extern "C" {
 
 int atri_sizeof_encattn() { return (int)sizeof(EncAttnArgs); }
 
-// Validity words [B, ceil(Lk / 64)] of a byte mask (nonzero: the key takes part), element strides sb / sk.
-int atri_enc_key_words(const void* mask, long long sb, long long sk, void* words, int B, int Lk, hipStream_t stream) {
-  if (B < 1 || Lk < 1 || !mask || !words) return -10;
-  const long long n = (long long)B * ((Lk + 63) / 64);
-  if ((n + 3) / 4 >= (1LL << 31)) return -15;
-  hipLaunchKernelGGL(key_words_kernel, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, stream, reinterpret_cast<const unsigned char*>(mask), sb, sk,
-                     reinterpret_cast<unsigned long long*>(words), B, Lk);
-  return hip_err(hipGetLastError());
-}
+// Queries per workgroup of the forward (forward != 0) and the query-owned pass, keys per workgroup of the key-owned one.
+int atri_enc_attn_rows(int W, int L, int Lk, int D, int M, int forward) { return 64 * enc_columns(W, L, Lk, D, M, forward != 0); }
 
 // out (and, where the pointers are set, stat and o32) of one attention call.
 int atri_enc_attn_fwd(const EncAttnArgs* args, hipStream_t stream) {
@@ -352,7 +405,15 @@ int atri_enc_attn_fwd(const EncAttnArgs* args, hipStream_t stream) {
   const EncAttnArgs& a = *args;
   const int rc = enc_check(a);
   if (rc) return rc;
-  if (!a.q || !a.k || !a.v || !a.out || a.splits < 1 || (a.splits > 1 && (!a.part_o || !a.part_ml))) return -17;
+  if (!a.q || !a.k || !a.v || !a.out || (a.splits > 1 && (!a.part_o || !a.part_ml))) return -17;
+  if (a.mask) {
+    if (!a.words) return -17;
+    const long long n = ((long long)a.B * ((a.Lk + 63) / 64) + 3) / 4;
+    if (n >= (1LL << 31)) return -15;
+    hipLaunchKernelGGL(key_words_kernel, dim3((unsigned)n), dim3(256), 0, stream, a.mask, a.ms[0], a.ms[1], a.words, a.B, a.Lk);
+    const int rc1 = hip_err(hipGetLastError());
+    if (rc1) return rc1;
+  }
   const int rc2 = a.bf16 ? dispatch_fwd<unsigned short>(a, stream) : dispatch_fwd<float>(a, stream);
   if (rc2 || a.splits == 1) return rc2;
   const long long n = (long long)a.B * a.H * a.Lq * (a.DV / 4);

@@ -14,6 +14,7 @@
 
 using namespace atrihip;
 
+// Filled by ops/residual.py in this order.
 struct ResNormArgs {
   const void* x;        // [N, D] residual stream
   const void* z;        // [N, D] block output
@@ -34,7 +35,7 @@ struct ResNormArgs {
   float* part;          // [workgroups, 5, D] partial sums of dscale, dpost_w, dpost_b, dpre_w, dpre_b
   float* dparams;       // [5, D]
   long long N;
-  int D, gate_mode, groups;
+  int D, gate_mode, groups, x_bf16, z_bf16;
   float eps;
 };
 
@@ -327,7 +328,8 @@ void by_width(const ResNormArgs& a, bool backward, hipStream_t stream) {
   }
 }
 
-int run(const ResNormArgs& a, int x_bf16, int z_bf16, bool backward, hipStream_t stream) {
+int run(const ResNormArgs& a, bool backward, hipStream_t stream) {
+  const bool x_bf16 = a.x_bf16 != 0, z_bf16 = a.z_bf16 != 0;
   // 16-byte accesses: widths in eights (rows then start on 16 bytes; the caller's buffers do)
   const bool vec = a.D % 8 == 0;
   if (x_bf16 && z_bf16) vec ? by_width<unsigned short, unsigned short, true>(a, backward, stream) : by_width<unsigned short, unsigned short, false>(a, backward, stream);
@@ -353,22 +355,22 @@ int atri_sizeof_resnorm() { return (int)sizeof(ResNormArgs); }
 // Rows a workgroup of the kernels for width D takes per step.
 int atri_resnorm_rows(int D) { return threads_of(lanes_of(D)) / lanes_of(D); }
 
-int atri_resnorm_fwd(const ResNormArgs* args, int x_bf16, int z_bf16, hipStream_t stream) {
+int atri_resnorm_fwd(const ResNormArgs* args, hipStream_t stream) {
   if (!args) return -1;
   const int rc = check(*args);
   if (rc) return rc;
   if (!args->y || !args->h || !args->pre_b) return -17;
-  return run(*args, x_bf16, z_bf16, false, stream);
+  return run(*args, false, stream);
 }
 
 // dx, dz, dgate (every element) and dparams [5, D]: dscale, dpost_w, dpost_b, dpre_w, dpre_b.
-int atri_resnorm_bwd(const ResNormArgs* args, int x_bf16, int z_bf16, hipStream_t stream) {
+int atri_resnorm_bwd(const ResNormArgs* args, hipStream_t stream) {
   if (!args) return -1;
   const ResNormArgs& a = *args;
   int rc = check(a);
   if (rc) return rc;
   if (!a.stats || !a.dx || !a.dz || !a.part || !a.dparams || (a.gate_mode && !a.dgate)) return -17;
-  rc = run(a, x_bf16, z_bf16, true, stream);
+  rc = run(a, true, stream);
   if (rc) return rc;
   const int n = 5 * a.D;
   hipLaunchKernelGGL(resnorm_params_kernel, dim3((n + 31) / 32), dim3(1024), 0, stream, a.part, a.dparams, a.groups, n);

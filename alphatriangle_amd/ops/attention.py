@@ -19,7 +19,9 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -143,75 +145,58 @@ def attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: 
 
 
 # ---------------------------------------------------------------------------------------------------------- kernels
-class _ArgsC(C.Structure):
-    _fields_ = (
-        [(n, hb.VP) for n in ("q", "k", "v", "dout", "out", "dq", "dk", "dv", "table", "lut", "lam", "words", "qoff", "stat", "o32",
-                              "delta", "part_o", "part_ml", "hist")]
-        + [(n, C.c_longlong * 3) for n in ("qs", "ks", "vs", "os", "gs", "dqs", "dks", "dvs")]
-        + [("o32s", C.c_longlong * 4)]
-        + [(n, C.c_int) for n in ("B", "Lq", "Lk", "H", "KV", "D", "DV", "M", "R", "W", "q0", "bf16", "splits", "hist_rows")]
-        + [("scale", C.c_float)]
-    )
+# EncAttnArgs of csrc/hip/encoder_attn.hpp: 27 pointers, 8 x 3 + 4 + 2 strides, 21 ints, 1 float.
+_PACK = struct.Struct("=27q30q21if")
+_group_rows: dict[tuple[int, ...], int] = {}
 
 
-_abi_checked = False
-
-
-def _check_abi() -> None:
-    global _abi_checked
-    if not _abi_checked:
-        fn = hb.lib().atri_sizeof_encattn
-        fn.restype = C.c_int
-        if fn() != C.sizeof(_ArgsC):
-            raise hb.HipError(f"ABI mismatch: atri_sizeof_encattn() = {fn()} but ctypes has {C.sizeof(_ArgsC)} bytes")
-        _abi_checked = True
-
-
-def _rows_ok(t: torch.Tensor) -> bool:
-    vec = 16 // t.element_size()
-    return t.data_ptr() % 16 == 0 and (t.stride(3) == 1 or t.shape[3] == 1) and all(t.stride(i) % vec == 0 for i in range(3) if t.shape[i] > 1)
+def _rows_of_group(cols: int, lq: int, lk: int, d: int, maps: int, forward: bool) -> int:
+    """Queries (keys) a workgroup owns; the first call checks the argument struct against the library."""
+    key = (cols, lq, lk, d, maps, forward)
+    rows = _group_rows.get(key)
+    if rows is None:
+        lib = hb.lib()
+        size, per = lib.atri_sizeof_encattn, lib.atri_enc_attn_rows
+        size.restype = per.restype = C.c_int
+        if size() != _PACK.size:
+            raise hb.HipError(f"ABI mismatch: atri_sizeof_encattn() = {size()} but {_PACK.size} bytes are packed")
+        if len(_group_rows) > 4096:
+            _group_rows.clear()
+        rows = _group_rows[key] = int(per(*[C.c_int(int(x)) for x in key]))
+    return rows
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` as the kernels can read it: in place when its rows are contiguous and 16-byte aligned, else a copy."""
-    return t if _rows_ok(t) else t.contiguous()
+    s, n = t.stride(), t.shape
+    vec = 3 if t.dtype == torch.float32 else 7
+    if s[3] == 1 and not t.data_ptr() & 15 and all(not s[i] & vec or n[i] == 1 for i in (0, 1, 2)):
+        return t
+    t = t.contiguous()
+    return t if t.stride(3) == 1 and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
 
 
-def _strides(t: torch.Tensor) -> tuple[int, int, int]:
-    return tuple(0 if t.shape[i] == 1 else t.stride(i) for i in range(3))  # type: ignore[return-value]
-
-
-def _empty_like_rows(t: torch.Tensor, heads: int, width: int, dtype: torch.dtype) -> torch.Tensor:
-    """New ``[B, L, heads, width]`` in the token / batch order of ``t``."""
+def _empty_like_rows(t: torch.Tensor, heads: int, width: int) -> torch.Tensor:
+    """New ``[B, L, heads, width]`` in the type and the token / batch order of ``t``."""
     b, n = t.shape[:2]
-    if b > 1 and n > 1 and t.stride(0) < t.stride(1):
-        return torch.empty(n, b, heads, width, dtype=dtype, device=t.device).transpose(0, 1)
-    return torch.empty(b, n, heads, width, dtype=dtype, device=t.device)
+    if t.stride(0) < t.stride(1) and b > 1 and n > 1:
+        return torch.empty(n, b, heads, width, dtype=t.dtype, device=t.device).transpose(0, 1)
+    return torch.empty(b, n, heads, width, dtype=t.dtype, device=t.device)
 
 
-def _fill(a: _ArgsC, **tensors: tuple[torch.Tensor, str] | torch.Tensor | None) -> None:
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if isinstance(t, tuple):
-            getattr(a, t[1])[:] = _strides(t[0])
-            t = t[0]
-        setattr(a, name, t.data_ptr())
+def _plan(samples: int, groups: int, steps: int, full: int) -> tuple[int, int]:
+    """``(splits, chunk)`` of a launch with ``groups`` workgroups per sample that walk ``steps`` tiles each.
+
+    ``full`` workgroups fill the card.  With fewer the tiles are split, four of them at least to a range (a range's partial
+    sums cost a write, a read and the join); with more a workgroup takes ``chunk`` samples one after the other."""
+    n = samples * groups
+    if 2 * n <= full and steps >= 8:
+        return max(1, min(-(-full // n), steps // 4, 256)), 1
+    return 1, max(1, n // full)
 
 
-def _splits(b: int, h: int, lq: int, lk: int, wide: bool) -> int:
-    """Key ranges per query tile: one unless the (sample, head, query tile) workgroups leave compute units idle, then about
-    four workgroups per CU with at least four key tiles each (a range's partial output costs a write, a read and the join)."""
-    groups = b * h * -(-lq // (128 if wide else 64))
-    tiles = -(-lk // 64)
-    if groups >= 512 or tiles < 8:
-        return 1
-    return max(1, min(-(-1024 // groups), tiles // 4, 256))
-
-
-@dataclass
-class _Call:
-    """What one call fixes besides its tensors."""
+class _Call(NamedTuple):
+    """What one call fixes besides its differentiable tensors."""
 
     buckets: RelativeBuckets | None
     mask: torch.Tensor | None
@@ -221,78 +206,86 @@ class _Call:
     maps: int
 
 
-def _base_args(c: _Call, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor | None, lam: torch.Tensor | None,
-               words: torch.Tensor | None) -> _ArgsC:
-    a = _ArgsC()
-    a.B, a.Lq, a.Lk = q.shape[0], q.shape[1], k.shape[1]
-    a.H, a.KV, a.D, a.DV, a.M = q.shape[2] // c.maps, v.shape[2], q.shape[3], v.shape[3], c.maps
-    a.bf16, a.splits, a.hist_rows, a.q0, a.scale = int(q.dtype == torch.bfloat16), 1, 4, c.q0, c.scale
-    _fill(a, q=(q, "qs"), k=(k, "ks"), v=(v, "vs"), table=table, lam=lam, words=words, qoff=c.qoff)
-    if table is not None and c.buckets is not None:
-        a.R, a.W, a.lut = c.buckets.radius, c.buckets.cols, c.buckets.lut.data_ptr()
-    return a
-
-
 def _forward(c: _Call, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor | None, lam: torch.Tensor | None,
-             train: bool) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
-    """``out`` and, for a backward pass, (stat, o32, words); operands as the kernels read them, fp32 table and lam."""
-    _check_abi()
-    b, lq, hm, _ = q.shape
-    lk, h, dv = k.shape[1], hm // c.maps, v.shape[3]
-    dev = q.device
-    out = _empty_like_rows(q, h, dv, q.dtype)
-    words = None
-    if c.mask is not None:
-        words = torch.empty(b, -(-lk // 64), dtype=torch.int64, device=dev)
-        hb.call("atri_enc_key_words", hb.ptr(c.mask), hb.i64(c.mask.stride(0)), hb.i64(c.mask.stride(1)), hb.ptr(words), hb.i32(b), hb.i32(lk))
-    a = _base_args(c, q, k, v, table, lam, words)
-    _fill(a, out=(out, "os"))
-    stat = o32 = None
-    if train:
-        stat = torch.empty(c.maps, b * h * lq, 2, dtype=torch.float32, device=dev)
-        if c.maps == 2 or q.dtype != torch.float32:  # delta = dO . o needs every map's output in 32 bits
-            o32 = torch.empty(c.maps, b, h, lq, dv, dtype=torch.float32, device=dev)
-            a.o32s[:] = (o32.stride(1), o32.stride(3), o32.stride(2), o32.stride(0))
-        _fill(a, stat=stat, o32=o32)
-    a.splits = _splits(b, h, lq, lk, c.maps == 1 and q.shape[3] <= 64 and lq > 64)
-    part = None
-    if a.splits > 1:
-        rows = a.splits * c.maps * b * h * lq
-        part = torch.empty(rows * (dv + 2), dtype=torch.float32, device=dev)
-        a.part_o, a.part_ml = part.data_ptr(), part.data_ptr() + 4 * rows * dv
-    hb.call("atri_enc_attn_fwd", C.byref(a))
-    return out, stat, o32, words
-
-
-def _backward(c: _Call, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor | None, lam: torch.Tensor | None,
-              o32: torch.Tensor, stat: torch.Tensor, words: torch.Tensor | None, dout: torch.Tensor, dq: torch.Tensor, dk: torch.Tensor,
-              dv: torch.Tensor, want_table: bool, want_lam: bool) -> tuple[torch.Tensor | None, torch.Tensor | None]:
-    """Fills ``dq`` / ``dk`` / ``dv`` (strided, every element) and returns ``(dtable, dlam)`` in fp32.  ``o32`` is the per-map
-    output ``[M, B, H, Lq, DV]`` or, for one fp32 map, the output itself ``[B, Lq, H, DV]``."""
+             train: bool) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """``out`` and, for a backward pass, one buffer of what it keeps: validity words (if masked), (maximum, 1 / sum) of every
+    row and - unless the fp32 output itself will do - every map's output in 32 bits.  Operands as the kernels read them."""
     b, lq, hm, d = q.shape
-    h, dev = hm // c.maps, q.device
-    a = _base_args(c, q, k, v, table, lam, words)
-    delta = torch.empty(c.maps, b * h * lq, dtype=torch.float32, device=dev)
-    _fill(a, dout=(dout, "gs"), dq=(dq, "dqs"), dk=(dk, "dks"), dv=(dv, "dvs"), stat=stat, delta=delta, o32=o32)
-    a.o32s[:] = (o32.stride(1), o32.stride(3), o32.stride(2), o32.stride(0)) if o32.dim() == 5 else (*_strides(o32), 0)
-    hist, nqt, slots = None, 0, 0
-    if want_table and table is not None and c.buckets is not None:
-        per = hb.lib().atri_enc_attn_bwd_queries
-        per.restype = C.c_int
-        nqt, slots = -(-lq // per(C.c_int(d), C.c_int(c.maps))), 2 * c.buckets.radius + 1
-        hist = torch.empty(b * h * nqt, c.maps, slots, dtype=torch.float32, device=dev)
-        a.hist = hist.data_ptr()
-    hb.call("atri_enc_attn_bwd", C.byref(a))
-    dtable = dlam = None
-    if hist is not None and table is not None and c.buckets is not None:
-        shares = max(1, min(64, b * nqt // 16))
-        mid = torch.empty(shares, hm, slots, dtype=torch.float32, device=dev)
-        dtable = torch.empty(c.buckets.num_buckets, hm, dtype=torch.float32, device=dev)
-        hb.call("atri_enc_table_grad", hb.ptr(hist), hb.ptr(mid), hb.ptr(c.buckets.order), hb.ptr(c.buckets.start), hb.ptr(dtable), hb.i32(b),
-                hb.i32(h), hb.i32(c.maps), hb.i32(nqt), hb.i32(slots), hb.i32(c.buckets.num_buckets), hb.i32(shares))
-    if want_lam and lam is not None:
-        dlam = torch.empty(h, dtype=torch.float32, device=dev)
-        hb.call("atri_enc_dlam", hb.ptr(delta[1]), hb.ptr(dlam), hb.i32(b), hb.i32(h), hb.i32(lq))
+    lk, kv, dv = v.shape[1], v.shape[2], v.shape[3]
+    maps, buckets, mask = c.maps, c.buckets, c.mask
+    h = hm // maps
+    bf16 = q.dtype == torch.bfloat16
+    out = _empty_like_rows(q, h, dv)
+    rows = b * h * lq
+    n_words = 2 * b * -(-lk // 64) if mask is not None else 0
+    n_stat = 2 * maps * rows if train else 0
+    n_o32 = maps * rows * dv if train and (bf16 or maps == 2) else 0
+    splits, chunk = _plan(b, h * -(-lq // _rows_of_group(buckets.cols if buckets is not None else 0, lq, lk, d, maps, True)), -(-lk // 64), 1024)
+    n_part = splits * maps * rows * (dv + 2) if splits > 1 else 0
+    n_keep = n_words + (n_words & 2) + n_stat + (n_stat & 2) + n_o32  # each part on 16 bytes
+    keep = torch.empty(n_keep, dtype=torch.float32, device=q.device) if n_keep else None
+    part = torch.empty(n_part, dtype=torch.float32, device=q.device).data_ptr() if n_part else 0
+    at = keep.data_ptr() if keep is not None else 0
+    at_stat = at + 4 * (n_words + (n_words & 2))
+    at_o32 = at_stat + 4 * (n_stat + (n_stat & 2))
+    biased = buckets is not None
+    hb.call_packed("atri_enc_attn_fwd", _PACK.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, out.data_ptr(), 0, 0, 0, table.data_ptr() if biased else 0,
+        buckets.lut.data_ptr() if biased else 0, 0, 0, lam.data_ptr() if maps == 2 else 0, mask.data_ptr() if n_words else 0, at if n_words else 0,
+        c.qoff.data_ptr() if c.qoff is not None else 0, at_stat if train else 0, at_o32 if n_o32 else 0, 0, part, part + 4 * splits * maps * rows * dv, 0, 0, 0, 0, 0, 0,
+        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *_NONE12, h * lq * dv, dv, lq * dv, rows * dv,
+        *(mask.stride() if n_words else (0, 0)), b, lq, lk, h, kv, d, dv, maps, buckets.radius if biased else 0, buckets.cols if biased else 0, c.q0, 0,
+        bf16, 0, 0, splits, chunk, 1, 1, 1, 1, c.scale), q.device.index)
+    return out, keep if train else None
+
+
+_NONE12 = (0,) * 12
+
+
+def _backward(c: _Call, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor | None, lam: torch.Tensor | None, keep: torch.Tensor,
+              out: torch.Tensor | None, dout: torch.Tensor, dq: torch.Tensor, dk: torch.Tensor, dv_: torch.Tensor, want_table: bool,
+              want_lam: bool) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """Fills ``dq`` / ``dk`` / ``dv_`` (strided, every element) and returns ``(dtable, dlam)`` in fp32.  ``keep`` is the forward
+    pass's buffer, ``out`` its output where that is the 32-bit one (one fp32 map)."""
+    b, lq, hm, d = q.shape
+    lk, kv, dv = v.shape[1], v.shape[2], v.shape[3]
+    maps, buckets, dev = c.maps, c.buckets, q.device
+    h = hm // maps
+    rows = b * h * lq
+    n_words = 2 * b * -(-lk // 64) if c.mask is not None else 0
+    at = keep.data_ptr()
+    at_stat = at + 4 * (n_words + (n_words & 2))
+    n_stat = 2 * maps * rows
+    at_o32 = out.data_ptr() if out is not None else at_stat + 4 * (n_stat + (n_stat & 2))
+    biased = buckets is not None
+    want_table = want_table and biased
+    slots = 2 * buckets.radius + 1 if biased else 0
+    per = _rows_of_group(buckets.cols if biased else 0, lq, lk, d, maps, False)
+    nqt, nkt = -(-lq // per), -(-lk // per)
+    q_splits, q_chunk = _plan(b, h * nqt, -(-lk // 64), 512)
+    k_splits, k_chunk = _plan(b, kv * nkt, h // kv * -(-lq // 64), 512)
+    per_head = -(-b // q_chunk) * q_splits * nqt  # query-owned workgroups
+    shares = max(1, min(64, per_head // 16))
+    n_hist, n_mid = (per_head * hm * slots, shares * hm * slots) if want_table else (0, 0)
+    n_dq = q_splits * rows * maps * d if q_splits > 1 else 0
+    n_kv = k_splits * b * kv * lk * (maps * d + dv) if k_splits > 1 else 0
+    n_delta = maps * rows + (-maps * rows & 3)  # the partial gradients on 16 bytes
+    work = torch.empty(n_delta + n_dq + n_kv + n_hist + n_mid, dtype=torch.float32, device=dev)
+    at_work = work.data_ptr()
+    at_dq = at_work + 4 * n_delta
+    at_kv = at_dq + 4 * n_dq
+    at_hist = at_kv + 4 * n_kv
+    dtable = torch.empty(buckets.num_buckets, hm, dtype=torch.float32, device=dev) if want_table else None
+    dlam = torch.empty(h, dtype=torch.float32, device=dev) if want_lam else None
+    hb.call_packed("atri_enc_attn_bwd", _PACK.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), 0, dq.data_ptr(), dk.data_ptr(), dv_.data_ptr(), table.data_ptr() if biased else 0,
+        buckets.lut.data_ptr() if biased else 0, buckets.order.data_ptr() if biased else 0, buckets.start.data_ptr() if biased else 0,
+        lam.data_ptr() if maps == 2 else 0, 0, at if n_words else 0, c.qoff.data_ptr() if c.qoff is not None else 0, at_stat, at_o32, at_work, 0, 0,
+        at_hist if want_table else 0, at_hist + 4 * n_hist if want_table else 0, at_dq, at_kv, dtable.data_ptr() if want_table else 0, dlam.data_ptr() if want_lam else 0,
+        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], 0, 0, 0, *dout.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *dv_.stride()[:3],
+        *((*out.stride()[:3], 0) if out is not None else (h * lq * dv, dv, lq * dv, rows * dv)), 0, 0, b, lq, lk, h, kv, d, dv, maps,
+        buckets.radius if biased else 0, buckets.cols if biased else 0, c.q0, buckets.num_buckets if biased else 0, q.dtype == torch.bfloat16, shares, 4,
+        1, 1, q_splits, q_chunk, k_splits, k_chunk, c.scale), dev.index)
     return dtable, dlam
 
 
@@ -305,21 +298,20 @@ class _EncoderAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, table, lam, call):  # noqa: ANN001
         qr, kr, vr = _rows(q.detach()), _rows(k.detach()), _rows(v.detach())
         t32, l32 = _f32(table), _f32(lam)
-        with torch.cuda.device(q.device):
-            out, stat, o32, words = _forward(call, qr, kr, vr, t32, l32, True)
+        with hb.on_device(q.device.index):
+            out, keep = _forward(call, qr, kr, vr, t32, l32, True)
         ctx.call = call
         ctx.like = (table.dtype if table is not None else None, lam.dtype if lam is not None else None)
-        ctx.save_for_backward(qr, kr, vr, t32, l32, out if o32 is None else o32, stat, words)
+        ctx.save_for_backward(qr, kr, vr, t32, l32, keep, out if call.maps == 1 and q.dtype == torch.float32 else None)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):  # noqa: ANN001
-        q, k, v, table, lam, o32, stat, words = ctx.saved_tensors
-        c = ctx.call
-        with torch.cuda.device(q.device):
-            dq, dk, dv = (_empty_like_rows(t, t.shape[2], t.shape[3], t.dtype) for t in (q, k, v))
-            dtable, dlam = _backward(c, q, k, v, table, lam, o32, stat, words, _rows(dout.to(q.dtype)), dq, dk, dv, ctx.needs_input_grad[3],
+        q, k, v, table, lam, keep, out = ctx.saved_tensors
+        with hb.on_device(q.device.index):
+            dq, dk, dv = (_empty_like_rows(t, t.shape[2], t.shape[3]) for t in (q, k, v))
+            dtable, dlam = _backward(ctx.call, q, k, v, table, lam, keep, out, _rows(dout.to(q.dtype)), dq, dk, dv, ctx.needs_input_grad[3],
                                      ctx.needs_input_grad[4])
             if dtable is not None:
                 dtable = dtable.to(ctx.like[0])
@@ -368,16 +360,18 @@ def _check(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: 
         raise ValueError(f"{name}: query_offset beyond {MAX_OFFSET}")
     if max(q.shape[1], lk) > MAX_OFFSET:
         raise ValueError(f"{name}: sequences of at most {MAX_OFFSET} tokens")
-    others = [t for t in (k, v, table, lam, key_mask, query_offset if torch.is_tensor(query_offset) else None, buckets.lut if buckets else None)
-              if t is not None]
-    if any(t.device != q.device for t in others):
-        raise ValueError(f"{name}: all tensors (and the buckets) on {q.device}, got {[str(t.device) for t in others]}")
+    dev = q.device
+    for t in (k, v, table, lam, key_mask, query_offset if torch.is_tensor(query_offset) else None, buckets.lut if buckets is not None else None):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name}: all tensors (and the buckets) on {dev}, got one on {t.device}")
 
 
 def _attend(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor | None, table: torch.Tensor | None,
             buckets: RelativeBuckets | None, key_mask: torch.Tensor | None, scale: float | None, query_offset: int | torch.Tensor) -> torch.Tensor:
     _check(name, q, k, v, table, lam, buckets, key_mask, query_offset)
     scale = q.shape[3] ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f"{name}: scale is a positive number, got {scale}")
     if not q.is_cuda or q.numel() == 0 or k.numel() == 0:
         return attention_reference(q, k, v, lam, table, buckets, key_mask, scale, query_offset)
     qoff = None
@@ -385,9 +379,10 @@ def _attend(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: t
         qoff = query_offset.expand(q.shape[0]).contiguous()
         query_offset = 0
     call = _Call(buckets, key_mask, qoff, int(query_offset), scale, 1 if lam is None else 2)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table, lam)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (table is not None and table.requires_grad)
+                                    or (lam is not None and lam.requires_grad)):
         return _EncoderAttention.apply(q, k, v, table, lam, call)
-    with torch.cuda.device(q.device):
+    with hb.on_device(q.device.index):
         return _forward(call, _rows(q.detach()), _rows(k.detach()), _rows(v.detach()), _f32(table), _f32(lam), False)[0]
 
 

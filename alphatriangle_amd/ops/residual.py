@@ -10,6 +10,7 @@ order (no atomics).
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -34,16 +35,8 @@ def gated_norm_residual_reference(x: torch.Tensor, z: torch.Tensor, scale: torch
     return y.to(x.dtype), norm(y, pre_weight, pre_bias).to(z.dtype)
 
 
-class _ArgsC(C.Structure):
-    _fields_ = (
-        [(n, hb.VP) for n in ("x", "z", "gate", "scale", "post_w", "post_b", "pre_w", "pre_b", "y", "h", "stats", "dy", "dh", "dx", "dz", "dgate",
-                              "part", "dparams")]
-        + [("N", C.c_longlong)]
-        + [(n, C.c_int) for n in ("D", "gate_mode", "groups")]
-        + [("eps", C.c_float)]
-    )
-
-
+# ResNormArgs of csrc/hip/residual_norm_kernels.hip: 18 pointers, the row count, 5 ints, 1 float.
+_PACK = struct.Struct("=18qq5if")
 _rows_per_step: dict[int, int] = {}  # by width
 
 
@@ -54,44 +47,36 @@ def _workgroups(n: int, d: int, most: int) -> int:
         lib = hb.lib()
         size, rows = lib.atri_sizeof_resnorm, lib.atri_resnorm_rows
         size.restype = rows.restype = C.c_int
-        if size() != C.sizeof(_ArgsC):
-            raise hb.HipError(f"ABI mismatch: atri_sizeof_resnorm() = {size()} but ctypes has {C.sizeof(_ArgsC)} bytes")
+        if size() != _PACK.size:
+            raise hb.HipError(f"ABI mismatch: atri_sizeof_resnorm() = {size()} but {_PACK.size} bytes are packed")
         per = _rows_per_step[d] = int(rows(C.c_int(d)))
     return max(1, min(-(-n // per), most))
 
 
-def _args(x: torch.Tensor, z: torch.Tensor, gate: torch.Tensor | None, params: list[torch.Tensor], eps: float) -> _ArgsC:
-    a = _ArgsC()
-    a.N, a.D, a.eps = x.numel() // x.shape[-1], x.shape[-1], eps
-    a.gate_mode = 0 if gate is None else 2 if gate.shape == z.shape else 1
-    for name, t in zip(("x", "z", "gate", "scale", "post_w", "post_b", "pre_w", "pre_b"), (x, z, gate, *params)):
-        if t is not None:
-            setattr(a, name, t.data_ptr())
-    return a
-
-
-def _types(x: torch.Tensor, z: torch.Tensor) -> tuple[C.c_int, C.c_int]:
-    return hb.i32(x.dtype == torch.bfloat16), hb.i32(z.dtype == torch.bfloat16)
-
-
-def _rows(t: torch.Tensor | None) -> torch.Tensor | None:
+def _rows(t: torch.Tensor) -> torch.Tensor:
     """Contiguous rows on a 16-byte boundary (a copy where they are not)."""
-    if t is None:
-        return None
     t = t.detach().contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t if not t.data_ptr() & 15 else t.clone()
 
 
-def _forward(x, z, gate, params, eps, train):  # noqa: ANN001, ANN202
+def _param(t: torch.Tensor) -> torch.Tensor:
+    return _rows(t if t.dtype == torch.float32 else t.float())
+
+
+def _gate_mode(z: torch.Tensor, gate: torch.Tensor | None) -> int:
+    return 0 if gate is None else 2 if gate.shape == z.shape else 1
+
+
+def _forward(x: torch.Tensor, z: torch.Tensor, gate: torch.Tensor | None, params: tuple[torch.Tensor, ...], eps: float,
+             train: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
     y, h = torch.empty_like(x), torch.empty_like(z)
-    a = _args(x, z, gate, params, eps)
-    a.y, a.h = y.data_ptr(), h.data_ptr()
-    stats = None
-    if train:
-        stats = torch.empty(a.N, 4, dtype=torch.float32, device=x.device)
-        a.stats = stats.data_ptr()
-    a.groups = _workgroups(a.N, a.D, 2048)
-    hb.call("atri_resnorm_fwd", C.byref(a), *_types(x, z))
+    d = x.shape[-1]
+    n = x.numel() // d
+    stats = torch.empty(n, 4, dtype=torch.float32, device=x.device) if train else None
+    hb.call_packed("atri_resnorm_fwd", _PACK.pack(
+        x.data_ptr(), z.data_ptr(), gate.data_ptr() if gate is not None else 0, *[p.data_ptr() for p in params], y.data_ptr(), h.data_ptr(),
+        stats.data_ptr() if stats is not None else 0, 0, 0, 0, 0, 0, 0, 0, n, d, _gate_mode(z, gate), _workgroups(n, d, 2048),
+        x.dtype == torch.bfloat16, z.dtype == torch.bfloat16, eps), x.device.index)
     return y, h, stats
 
 
@@ -99,9 +84,9 @@ class _GatedNormResidual(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, z, scale, post_weight, post_bias, pre_weight, pre_bias, gate, eps):  # noqa: ANN001
         given = (scale, post_weight, post_bias, pre_weight, pre_bias)
-        with torch.cuda.device(x.device):
-            xr, zr, gr = _rows(x), _rows(z), _rows(gate)
-            params = [_rows(p.float()) for p in given]
+        with hb.on_device(x.device.index):
+            xr, zr, gr = _rows(x), _rows(z), _rows(gate) if gate is not None else None
+            params = tuple(_param(p) for p in given)
             y, h, stats = _forward(xr, zr, gr, params, eps, True)
         ctx.save_for_backward(xr, zr, gr, stats, *params)
         ctx.like = [p.dtype for p in given]
@@ -115,21 +100,23 @@ class _GatedNormResidual(torch.autograd.Function):
         if dy is None and dh is None:
             return (None,) * 9
         x, z, gate, stats, *params = ctx.saved_tensors
-        with torch.cuda.device(x.device):
+        with hb.on_device(x.device.index):
             dy = _rows(dy.to(x.dtype)) if dy is not None else None
             dh = _rows(dh.to(z.dtype)) if dh is not None else None
             dx, dz = torch.empty_like(x), torch.empty_like(z)
             dgate = torch.empty_like(gate) if gate is not None else None
-            a = _args(x, z, gate, params, ctx.eps)
+            d = x.shape[-1]
+            n = x.numel() // d
             # many rows per workgroup keep the partial sums small beside the rows: 5 of a row each
-            a.groups = _workgroups(a.N, a.D, 1024 if a.D <= 512 else 512)
-            part = torch.empty(a.groups, 5, a.D, dtype=torch.float32, device=x.device)
-            dparams = torch.empty(5, a.D, dtype=torch.float32, device=x.device)
-            for name, t in (("stats", stats), ("dy", dy), ("dh", dh), ("dx", dx), ("dz", dz), ("dgate", dgate), ("part", part), ("dparams", dparams)):
-                if t is not None:
-                    setattr(a, name, t.data_ptr())
-            hb.call("atri_resnorm_bwd", C.byref(a), *_types(x, z))
-            each = [g.to(t) for g, t in zip(dparams.unbind(0), ctx.like)]
+            groups = _workgroups(n, d, 1024 if d <= 512 else 512)
+            part = torch.empty(groups, 5, d, dtype=torch.float32, device=x.device)
+            dparams = torch.empty(5, d, dtype=torch.float32, device=x.device)
+            hb.call_packed("atri_resnorm_bwd", _PACK.pack(
+                x.data_ptr(), z.data_ptr(), gate.data_ptr() if gate is not None else 0, *[p.data_ptr() for p in params], 0, 0, stats.data_ptr(),
+                dy.data_ptr() if dy is not None else 0, dh.data_ptr() if dh is not None else 0, dx.data_ptr(), dz.data_ptr(),
+                dgate.data_ptr() if gate is not None else 0, part.data_ptr(), dparams.data_ptr(), n, d, _gate_mode(z, gate), groups,
+                x.dtype == torch.bfloat16, z.dtype == torch.bfloat16, ctx.eps), x.device.index)
+            each = [g if t == torch.float32 else g.to(t) for g, t in zip(dparams.unbind(0), ctx.like)]
         return (dx, dz, *each, dgate, None)
 
 
@@ -159,13 +146,15 @@ def gated_norm_residual(x: torch.Tensor, z: torch.Tensor, scale: torch.Tensor, p
         raise ValueError(f"{name}: gate is [..., {d}] or [..., 1] in {z.dtype}, got {tuple(gate.shape)} {gate.dtype}")
     if not eps > 0:
         raise ValueError(f"{name}: eps must be positive, got {eps}")
-    tensors = [t for t in (x, z, scale, post_weight, post_bias, pre_weight, pre_bias, gate) if t is not None]
-    if any(t.device != x.device for t in tensors):
-        raise ValueError(f"{name}: all tensors on {x.device}, got {[str(t.device) for t in tensors]}")
+    params = (scale, post_weight, post_bias, pre_weight, pre_bias)
+    dev = x.device
+    grads = x.requires_grad or z.requires_grad or (gate is not None and gate.requires_grad)
+    for t in (z, *params, gate):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name}: all tensors on {dev}, got one on {t.device}")
     if not x.is_cuda or x.numel() == 0:
-        return gated_norm_residual_reference(x, z, scale, post_weight, post_bias, pre_weight, pre_bias, gate, eps)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        return _GatedNormResidual.apply(x, z, scale, post_weight, post_bias, pre_weight, pre_bias, gate, float(eps))
-    with torch.cuda.device(x.device):
-        params = [_rows(p.float()) for p in (scale, post_weight, post_bias, pre_weight, pre_bias)]
-        return _forward(_rows(x), _rows(z), _rows(gate), params, float(eps), False)[:2]
+        return gated_norm_residual_reference(x, z, *params, gate, eps)
+    if torch.is_grad_enabled() and (grads or any([p.requires_grad for p in params])):
+        return _GatedNormResidual.apply(x, z, *params, gate, float(eps))
+    with hb.on_device(dev.index):
+        return _forward(_rows(x), _rows(z), _rows(gate) if gate is not None else None, tuple(_param(p) for p in params), float(eps), False)[:2]
