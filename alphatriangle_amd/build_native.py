@@ -1,17 +1,20 @@
-"""In-tree builder of the two native libraries.
+"""In-tree builder of the native libraries.
 
 * ``_atri_host``  - host C++ runtime (pybind11, g++): game engine, features,
   host tree search, sum tree, metric ring.
 * ``_atri_host_wide`` - the same sources compiled with 16 occupancy words per
   game state: boards of 257 - 1024 cells (the kernel library holds the
   device engine for them as a second object of ``engine_kernels.hip``).
+* ``_atri_torch`` - host side of the encoder operators as a PyTorch extension (g++):
+  launch planning and autograd nodes in C++; it calls ``libatri_hip`` through
+  addresses it is handed.
 * ``libatri_hip`` - HIP/CDNA4 kernels for gfx950 (hipcc): batched game + tree
   engine, inference network, replay and learner kernels.  Exposed with a C ABI
   and loaded through ctypes after ``import torch`` so that it binds to the same
   HIP runtime as PyTorch.
 
-Both are written next to this file so that they travel with the source tree.
-Run ``python -m alphatriangle_amd.build_native`` (``--host`` / ``--hip`` to pick one).
+All are written next to this file so that they travel with the source tree.
+Run ``python -m alphatriangle_amd.build_native`` (``--host`` / ``--torch`` / ``--hip`` to pick one).
 """
 
 from __future__ import annotations
@@ -29,6 +32,7 @@ _EXT = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
 HOST_SO = PKG_DIR / ("_atri_host" + _EXT)
 HOST_WIDE_SO = PKG_DIR / ("_atri_host_wide" + _EXT)
 WIDE_WORDS = 16  # 64 cells per word: boards of up to 1024 cells
+TORCH_SO = PKG_DIR / ("_atri_torch" + _EXT)
 HIP_SO = PKG_DIR / "libatri_hip.so"
 
 HIP_FLAGS = [
@@ -98,6 +102,45 @@ def build_host(force: bool = False, verbose: bool = True) -> Path:
     return HOST_SO
 
 
+def build_torch(force: bool = False, verbose: bool = True) -> Path:
+    """Build the PyTorch extension (host code only; the HIP headers it includes declare the stream type)."""
+    import torch
+    from torch.utils import cpp_extension
+
+    srcs = sorted((CSRC / "torch").glob("*.cpp"))
+    if not force and _newer(TORCH_SO, srcs + [CSRC / "hip" / "encoder_ops.h", Path(__file__)]):
+        return TORCH_SO
+    rocm = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
+    cmd = [
+        os.environ.get("CXX", "g++"),
+        "-O2",
+        "-std=c++17",
+        "-fPIC",
+        "-shared",
+        "-fvisibility=hidden",
+        "-Wall",
+        "-D__HIP_PLATFORM_AMD__=1",
+        "-DUSE_ROCM=1",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        *[f"-isystem{p}" for p in cpp_extension.include_paths()],
+        f"-isystem{rocm / 'include'}",
+        f"-I{sysconfig.get_paths()['include']}",
+        *[str(s) for s in srcs],
+        "-o",
+        str(TORCH_SO),
+        *[f"-L{p}" for p in cpp_extension.library_paths()],
+        "-lc10",
+        "-lc10_hip",
+        "-ltorch_cpu",
+        "-ltorch",
+        "-ltorch_python",
+    ]
+    if verbose:
+        print("[build_native] torch:", " ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    return TORCH_SO
+
+
 def hip_objects() -> list[tuple[Path, str, list[str]]]:
     """(source, object stem, extra defines) of every object of the kernel library: one per ``.hip`` file, plus the device
     engine a second time with the wide host engine's 16-word game state (boards of 257 - 1024 cells, ``atriw_*`` entries)."""
@@ -165,6 +208,7 @@ def build_selftest(kind: str = "address", verbose: bool = True, wide: bool = Fal
 
 def build_all(force: bool = False, verbose: bool = True) -> None:
     build_host(force, verbose)
+    build_torch(force, verbose)
     build_hip(force, verbose)
 
 
@@ -177,6 +221,8 @@ if __name__ == "__main__":
             print(build_selftest(k))
     elif "--host" in args:
         build_host(force)
+    elif "--torch" in args:
+        build_torch(force)
     elif "--hip" in args:
         build_hip(force)
     else:

@@ -394,11 +394,6 @@ int dispatch_fwd(const EncAttnArgs& a, hipStream_t stream) {
 
 extern "C" {
 
-int atri_sizeof_encattn() { return (int)sizeof(EncAttnArgs); }
-
-// Queries per workgroup of the forward (forward != 0) and the query-owned pass, keys per workgroup of the key-owned one.
-int atri_enc_attn_rows(int W, int L, int Lk, int D, int M, int forward) { return 64 * enc_columns(W, L, Lk, D, M, forward != 0); }
-
 // out (and, where the pointers are set, stat and o32) of one attention call.
 int atri_enc_attn_fwd(const EncAttnArgs* args, hipStream_t stream) {
   if (!args) return -1;

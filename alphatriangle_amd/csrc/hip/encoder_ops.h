@@ -1,0 +1,107 @@
+// What the encoder operators' kernels (encoder_attn_*.hip, residual_norm_kernels.hip) and their host side
+// (csrc/torch/encoder_ops.cpp) share: argument blocks, entry points and the rules that pick a tiling.  No HIP in here.
+#pragma once
+
+struct ihipStream_t;
+
+namespace atrihip {
+
+constexpr int kTile = 64;  // keys (queries in the key-owned pass) staged per step of the attention kernels
+
+struct EncAttnArgs {
+  const void* q;       // [B, Lq, H M, D] by strides
+  const void* k;       // [B, Lk, KV M, D]
+  const void* v;       // [B, Lk, KV, DV]
+  const void* dout;    // [B, Lq, H, DV]
+  void* out;           // [B, Lq, H, DV]
+  void* dq;
+  void* dk;
+  void* dv;
+  const float* table;  // [buckets, H M]; nullptr: no position bias
+  const int* lut;      // [2 R + 1] bucket of every clamped position difference
+  const int* order;    // [2 R + 1] differences by bucket: those of bucket b at start[b] .. start[b + 1] - 1
+  const int* start;
+  const float* lam;    // [H] (M = 2)
+  const unsigned char* mask;  // [B, Lk] bytes by strides (nonzero: the key takes part); nullptr: all keys
+  unsigned long long* words;  // [B, ceil(Lk / 64)] validity bit of every key, made from mask by the forward pass; nullptr: all keys
+  const int* qoff;     // [B] position of the first query, nullptr: q0 for all samples
+  float* stat;         // [M, B H Lq, 2] row maximum of x / scale (+inf: no key) and 1 / sum (0: no key); nullptr: not wanted
+  float* o32;          // [M] x [B, Lq, H, DV] per-map outputs in 32 bits by strides (backward: their product with dO is delta)
+  float* delta;        // [M, B H Lq]
+  float* part_o;       // [splits, M, B H Lq, DV] unnormalised partial outputs (splits > 1)
+  float* part_ml;      // [splits, M, B H Lq, 2] their maxima and sums
+  float* hist;         // [workgroups of the query-owned pass, M, 2 R + 1] sums of dS by position difference; nullptr: not wanted
+  float* mid;          // [shares, H M, 2 R + 1] the same, added up over shares of the samples and query tiles
+  float* dq_part;      // [q_splits, B, H, Lq, M D] partial dQ in 32 bits (q_splits > 1)
+  float* kv_part;      // [k_splits, B, KV, Lk, M D + DV] partial dK and dV (k_splits > 1)
+  float* dtable;       // [buckets, H M]
+  float* dlam;         // [H]; nullptr: not wanted
+  long long qs[3], ks[3], vs[3], os[3], gs[3], dqs[3], dks[3], dvs[3];  // element strides: sample, token, head
+  long long o32s[4];   // o32: sample, token, head, map
+  long long ms[2];     // mask: sample, key
+  int B, Lq, Lk, H, KV, D, DV, M;
+  int R, W, q0;        // clamp of the position difference; board width (0: sequence); position of the first query
+  int buckets, bf16, shares, hist_rows;
+  int splits, chunk;      // forward: key ranges per query tile, samples a workgroup walks one after the other
+  int q_splits, q_chunk;  // query-owned pass: the same
+  int k_splits, k_chunk;  // key-owned pass: query ranges per key tile, samples
+  float scale;
+};
+
+// Boards of 2 to 4 key tiles keep their bias (and the sums of dS by pair) in registers over all samples a workgroup walks: every
+// sample has the same positions.  The tiles are then unrolled: NT of them, with as many 16-row columns per wave as
+// keep 64 registers for each.  0: the general form (sequences, smaller and larger boards).
+inline int enc_board_tiles(int W, int Lk, int D, int M) {
+  const int tiles = (Lk + kTile - 1) / kTile;
+  if (W <= 0 || D > 32 || tiles < 2) return 0;
+  return tiles == 2 ? 2 : tiles <= 4 && M == 1 ? 4 : 0;
+}
+// 16-row columns per wave: queries in the forward and the query-owned pass, keys in the key-owned one.
+inline int enc_columns(int W, int L, int Lk, int D, int M, bool forward) {
+  if (M == 2 || D > 64) return 1;
+  const int nt = enc_board_tiles(W, Lk, D, M);
+  if (nt) return nt == 2 ? 2 : 1;
+  return forward && L <= 64 ? 1 : 2;  // two, once they exist: every staged fragment then feeds two products
+}
+
+// The residual joint: threads that own a row (8 values each) and threads of a workgroup.
+inline int lanes_of(int D) {
+  int lanes = 16;
+  while (lanes * 8 < D) lanes *= 2;
+  return lanes;
+}
+constexpr int threads_of(int lanes) { return lanes < 256 ? 256 : lanes; }
+
+struct ResNormArgs {
+  const void* x;        // [N, D] residual stream
+  const void* z;        // [N, D] block output
+  const void* gate;     // gate logits in z's type: [N, D] (mode 2), [N] (mode 1), nullptr (mode 0)
+  const float* scale;   // [D]
+  const float* post_w;
+  const float* post_b;
+  const float* pre_w;
+  const float* pre_b;
+  void* y;              // [N, D] in x's type
+  void* h;              // [N, D] in z's type
+  float* stats;         // [N, 4]: mean and 1 / deviation of z, of y; nullptr in the forward pass: not wanted
+  const void* dy;       // gradients of y and h; nullptr: zero
+  const void* dh;
+  void* dx;
+  void* dz;
+  void* dgate;
+  float* part;          // [workgroups, 5, D] partial sums of dscale, dpost_w, dpost_b, dpre_w, dpre_b
+  float* dparams;       // [5, D]
+  long long N;
+  int D, gate_mode, groups, x_bf16, z_bf16;
+  float eps;
+};
+
+}  // namespace atrihip
+
+extern "C" {
+// 0, a HIP error code, or a negative code for arguments rejected before any launch.
+int atri_enc_attn_fwd(const atrihip::EncAttnArgs* args, ihipStream_t* stream);
+int atri_enc_attn_bwd(const atrihip::EncAttnArgs* args, ihipStream_t* stream);
+int atri_resnorm_fwd(const atrihip::ResNormArgs* args, ihipStream_t* stream);
+int atri_resnorm_bwd(const atrihip::ResNormArgs* args, ihipStream_t* stream);
+}

@@ -11,33 +11,9 @@
 // apart (any width).  Parameter gradients: a workgroup walks many rows,
 // sums in registers, joins its row groups in a fixed order and writes one partial row; a second launch adds those.
 #include "common.hpp"
+#include "encoder_ops.h"
 
 using namespace atrihip;
-
-// Filled by ops/residual.py in this order.
-struct ResNormArgs {
-  const void* x;        // [N, D] residual stream
-  const void* z;        // [N, D] block output
-  const void* gate;     // gate logits in z's type: [N, D] (mode 2), [N] (mode 1), nullptr (mode 0)
-  const float* scale;   // [D]
-  const float* post_w;
-  const float* post_b;
-  const float* pre_w;
-  const float* pre_b;
-  void* y;              // [N, D] in x's type
-  void* h;              // [N, D] in z's type
-  float* stats;         // [N, 4]: mean and 1 / deviation of z, of y; nullptr in the forward pass: not wanted
-  const void* dy;       // gradients of y and h; nullptr: zero
-  const void* dh;
-  void* dx;
-  void* dz;
-  void* dgate;
-  float* part;          // [workgroups, 5, D] partial sums of dscale, dpost_w, dpost_b, dpre_w, dpre_b
-  float* dparams;       // [5, D]
-  long long N;
-  int D, gate_mode, groups, x_bf16, z_bf16;
-  float eps;
-};
 
 namespace {
 
@@ -94,7 +70,6 @@ struct Share {
   }
 };
 
-constexpr int threads_of(int lanes) { return lanes < 256 ? 256 : lanes; }
 constexpr int kScratch = 8;  // floats per use: one per wave
 
 // Sum over the LANES threads of a row, the same value in all of them.  Rows of several waves meet in `scratch`, a slot of its own
@@ -310,12 +285,6 @@ void launch(const ResNormArgs& a, bool backward, hipStream_t stream) {
   else hipLaunchKernelGGL((resnorm_fwd_kernel<TX, TZ, LANES, VEC>), dim3(a.groups), dim3(threads_of(LANES)), 0, stream, a);
 }
 
-inline int lanes_of(int D) {
-  int lanes = 16;
-  while (lanes * 8 < D) lanes *= 2;
-  return lanes;
-}
-
 template <typename TX, typename TZ, bool VEC>
 void by_width(const ResNormArgs& a, bool backward, hipStream_t stream) {
   switch (lanes_of(a.D)) {
@@ -349,11 +318,6 @@ int check(const ResNormArgs& a) {
 }  // namespace
 
 extern "C" {
-
-int atri_sizeof_resnorm() { return (int)sizeof(ResNormArgs); }
-
-// Rows a workgroup of the kernels for width D takes per step.
-int atri_resnorm_rows(int D) { return threads_of(lanes_of(D)) / lanes_of(D); }
 
 int atri_resnorm_fwd(const ResNormArgs* args, hipStream_t stream) {
   if (!args) return -1;

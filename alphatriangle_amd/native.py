@@ -6,6 +6,7 @@ board of that many cells (the wide build above 256 cells), ``host_of(obj)`` the
 module a bound object came from.  ``hip()`` returns the ctypes handle of the gfx950 kernel
 library; it is never built implicitly on a GPU box and raises loudly when it is
 missing, so that GPU code paths cannot silently fall back to eager PyTorch.
+``torch_ops()`` is the PyTorch extension of the encoder operators, bound to that library.
 """
 
 from __future__ import annotations
@@ -96,3 +97,26 @@ def hip() -> ctypes.CDLL:
             except OSError as exc:
                 raise NativeLibraryError(f"failed to load {path}: {exc}") from exc
     return _hip_lib
+
+
+_torch_ops: ModuleType | None = None
+
+
+def torch_ops() -> ModuleType:
+    """The PyTorch extension of the encoder operators with the kernel library's entry points bound (raises when either is missing)."""
+    global _torch_ops
+    if _torch_ops is None:
+        lib = hip()
+        with _lock:
+            if _torch_ops is None:
+                try:
+                    mod = importlib.import_module("alphatriangle_amd._atri_torch")
+                except ImportError as exc:
+                    raise NativeLibraryError(
+                        f"the encoder operators' PyTorch extension does not load ({exc}). "
+                        "Build it with `python -m alphatriangle_amd.build_native --torch`."
+                    ) from exc
+                names = ("atri_enc_attn_fwd", "atri_enc_attn_bwd", "atri_resnorm_fwd", "atri_resnorm_bwd")
+                mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names})
+                _torch_ops = mod
+    return _torch_ops

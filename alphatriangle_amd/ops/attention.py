@@ -17,16 +17,13 @@
 
 from __future__ import annotations
 
-import ctypes as C
 import math
-import struct
+from collections.abc import Callable
 from dataclasses import dataclass
-from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import hipbind as hb
+from .. import native
 
 MAX_RADIUS = 2047     # largest position difference the kernels keep apart
 MAX_OFFSET = 1 << 29  # positions beyond this would let differences leave 32 bits
@@ -144,182 +141,7 @@ def attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: 
     return torch.matmul(att.contiguous(), vv.contiguous()).permute(0, 2, 1, 3).to(q.dtype)
 
 
-# ---------------------------------------------------------------------------------------------------------- kernels
-# EncAttnArgs of csrc/hip/encoder_attn.hpp: 27 pointers, 8 x 3 + 4 + 2 strides, 21 ints, 1 float.
-_PACK = struct.Struct("=27q30q21if")
-_group_rows: dict[tuple[int, ...], int] = {}
-
-
-def _rows_of_group(cols: int, lq: int, lk: int, d: int, maps: int, forward: bool) -> int:
-    """Queries (keys) a workgroup owns; the first call checks the argument struct against the library."""
-    key = (cols, lq, lk, d, maps, forward)
-    rows = _group_rows.get(key)
-    if rows is None:
-        lib = hb.lib()
-        size, per = lib.atri_sizeof_encattn, lib.atri_enc_attn_rows
-        size.restype = per.restype = C.c_int
-        if size() != _PACK.size:
-            raise hb.HipError(f"ABI mismatch: atri_sizeof_encattn() = {size()} but {_PACK.size} bytes are packed")
-        if len(_group_rows) > 4096:
-            _group_rows.clear()
-        rows = _group_rows[key] = int(per(*[C.c_int(int(x)) for x in key]))
-    return rows
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as the kernels can read it: in place when its rows are contiguous and 16-byte aligned, else a copy."""
-    s, n = t.stride(), t.shape
-    vec = 3 if t.dtype == torch.float32 else 7
-    if s[3] == 1 and not t.data_ptr() & 15 and all(not s[i] & vec or n[i] == 1 for i in (0, 1, 2)):
-        return t
-    t = t.contiguous()
-    return t if t.stride(3) == 1 and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
-
-
-def _empty_like_rows(t: torch.Tensor, heads: int, width: int) -> torch.Tensor:
-    """New ``[B, L, heads, width]`` in the type and the token / batch order of ``t``."""
-    b, n = t.shape[:2]
-    if t.stride(0) < t.stride(1) and b > 1 and n > 1:
-        return torch.empty(n, b, heads, width, dtype=t.dtype, device=t.device).transpose(0, 1)
-    return torch.empty(b, n, heads, width, dtype=t.dtype, device=t.device)
-
-
-def _plan(samples: int, groups: int, steps: int, full: int) -> tuple[int, int]:
-    """``(splits, chunk)`` of a launch with ``groups`` workgroups per sample that walk ``steps`` tiles each.
-
-    ``full`` workgroups fill the card.  With fewer the tiles are split, four of them at least to a range (a range's partial
-    sums cost a write, a read and the join); with more a workgroup takes ``chunk`` samples one after the other."""
-    n = samples * groups
-    if 2 * n <= full and steps >= 8:
-        return max(1, min(-(-full // n), steps // 4, 256)), 1
-    return 1, max(1, n // full)
-
-
-class _Call(NamedTuple):
-    """What one call fixes besides its differentiable tensors."""
-
-    buckets: RelativeBuckets | None
-    mask: torch.Tensor | None
-    qoff: torch.Tensor | None
-    q0: int
-    scale: float
-    maps: int
-
-
-def _forward(c: _Call, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor | None, lam: torch.Tensor | None,
-             train: bool) -> tuple[torch.Tensor, torch.Tensor | None]:
-    """``out`` and, for a backward pass, one buffer of what it keeps: validity words (if masked), (maximum, 1 / sum) of every
-    row and - unless the fp32 output itself will do - every map's output in 32 bits.  Operands as the kernels read them."""
-    b, lq, hm, d = q.shape
-    lk, kv, dv = v.shape[1], v.shape[2], v.shape[3]
-    maps, buckets, mask = c.maps, c.buckets, c.mask
-    h = hm // maps
-    bf16 = q.dtype == torch.bfloat16
-    out = _empty_like_rows(q, h, dv)
-    rows = b * h * lq
-    n_words = 2 * b * -(-lk // 64) if mask is not None else 0
-    n_stat = 2 * maps * rows if train else 0
-    n_o32 = maps * rows * dv if train and (bf16 or maps == 2) else 0
-    splits, chunk = _plan(b, h * -(-lq // _rows_of_group(buckets.cols if buckets is not None else 0, lq, lk, d, maps, True)), -(-lk // 64), 1024)
-    n_part = splits * maps * rows * (dv + 2) if splits > 1 else 0
-    n_keep = n_words + (n_words & 2) + n_stat + (n_stat & 2) + n_o32  # each part on 16 bytes
-    keep = torch.empty(n_keep, dtype=torch.float32, device=q.device) if n_keep else None
-    part = torch.empty(n_part, dtype=torch.float32, device=q.device).data_ptr() if n_part else 0
-    at = keep.data_ptr() if keep is not None else 0
-    at_stat = at + 4 * (n_words + (n_words & 2))
-    at_o32 = at_stat + 4 * (n_stat + (n_stat & 2))
-    biased = buckets is not None
-    hb.call_packed("atri_enc_attn_fwd", _PACK.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, out.data_ptr(), 0, 0, 0, table.data_ptr() if biased else 0,
-        buckets.lut.data_ptr() if biased else 0, 0, 0, lam.data_ptr() if maps == 2 else 0, mask.data_ptr() if n_words else 0, at if n_words else 0,
-        c.qoff.data_ptr() if c.qoff is not None else 0, at_stat if train else 0, at_o32 if n_o32 else 0, 0, part, part + 4 * splits * maps * rows * dv, 0, 0, 0, 0, 0, 0,
-        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *_NONE12, h * lq * dv, dv, lq * dv, rows * dv,
-        *(mask.stride() if n_words else (0, 0)), b, lq, lk, h, kv, d, dv, maps, buckets.radius if biased else 0, buckets.cols if biased else 0, c.q0, 0,
-        bf16, 0, 0, splits, chunk, 1, 1, 1, 1, c.scale), q.device.index)
-    return out, keep if train else None
-
-
-_NONE12 = (0,) * 12
-
-
-def _backward(c: _Call, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor | None, lam: torch.Tensor | None, keep: torch.Tensor,
-              out: torch.Tensor | None, dout: torch.Tensor, dq: torch.Tensor, dk: torch.Tensor, dv_: torch.Tensor, want_table: bool,
-              want_lam: bool) -> tuple[torch.Tensor | None, torch.Tensor | None]:
-    """Fills ``dq`` / ``dk`` / ``dv_`` (strided, every element) and returns ``(dtable, dlam)`` in fp32.  ``keep`` is the forward
-    pass's buffer, ``out`` its output where that is the 32-bit one (one fp32 map)."""
-    b, lq, hm, d = q.shape
-    lk, kv, dv = v.shape[1], v.shape[2], v.shape[3]
-    maps, buckets, dev = c.maps, c.buckets, q.device
-    h = hm // maps
-    rows = b * h * lq
-    n_words = 2 * b * -(-lk // 64) if c.mask is not None else 0
-    at = keep.data_ptr()
-    at_stat = at + 4 * (n_words + (n_words & 2))
-    n_stat = 2 * maps * rows
-    at_o32 = out.data_ptr() if out is not None else at_stat + 4 * (n_stat + (n_stat & 2))
-    biased = buckets is not None
-    want_table = want_table and biased
-    slots = 2 * buckets.radius + 1 if biased else 0
-    per = _rows_of_group(buckets.cols if biased else 0, lq, lk, d, maps, False)
-    nqt, nkt = -(-lq // per), -(-lk // per)
-    q_splits, q_chunk = _plan(b, h * nqt, -(-lk // 64), 512)
-    k_splits, k_chunk = _plan(b, kv * nkt, h // kv * -(-lq // 64), 512)
-    per_head = -(-b // q_chunk) * q_splits * nqt  # query-owned workgroups
-    shares = max(1, min(64, per_head // 16))
-    n_hist, n_mid = (per_head * hm * slots, shares * hm * slots) if want_table else (0, 0)
-    n_dq = q_splits * rows * maps * d if q_splits > 1 else 0
-    n_kv = k_splits * b * kv * lk * (maps * d + dv) if k_splits > 1 else 0
-    n_delta = maps * rows + (-maps * rows & 3)  # the partial gradients on 16 bytes
-    work = torch.empty(n_delta + n_dq + n_kv + n_hist + n_mid, dtype=torch.float32, device=dev)
-    at_work = work.data_ptr()
-    at_dq = at_work + 4 * n_delta
-    at_kv = at_dq + 4 * n_dq
-    at_hist = at_kv + 4 * n_kv
-    dtable = torch.empty(buckets.num_buckets, hm, dtype=torch.float32, device=dev) if want_table else None
-    dlam = torch.empty(h, dtype=torch.float32, device=dev) if want_lam else None
-    hb.call_packed("atri_enc_attn_bwd", _PACK.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), 0, dq.data_ptr(), dk.data_ptr(), dv_.data_ptr(), table.data_ptr() if biased else 0,
-        buckets.lut.data_ptr() if biased else 0, buckets.order.data_ptr() if biased else 0, buckets.start.data_ptr() if biased else 0,
-        lam.data_ptr() if maps == 2 else 0, 0, at if n_words else 0, c.qoff.data_ptr() if c.qoff is not None else 0, at_stat, at_o32, at_work, 0, 0,
-        at_hist if want_table else 0, at_hist + 4 * n_hist if want_table else 0, at_dq, at_kv, dtable.data_ptr() if want_table else 0, dlam.data_ptr() if want_lam else 0,
-        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], 0, 0, 0, *dout.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *dv_.stride()[:3],
-        *((*out.stride()[:3], 0) if out is not None else (h * lq * dv, dv, lq * dv, rows * dv)), 0, 0, b, lq, lk, h, kv, d, dv, maps,
-        buckets.radius if biased else 0, buckets.cols if biased else 0, c.q0, buckets.num_buckets if biased else 0, q.dtype == torch.bfloat16, shares, 4,
-        1, 1, q_splits, q_chunk, k_splits, k_chunk, c.scale), dev.index)
-    return dtable, dlam
-
-
-def _f32(t: torch.Tensor | None) -> torch.Tensor | None:
-    return None if t is None else t.detach().float().contiguous()
-
-
-class _EncoderAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, table, lam, call):  # noqa: ANN001
-        qr, kr, vr = _rows(q.detach()), _rows(k.detach()), _rows(v.detach())
-        t32, l32 = _f32(table), _f32(lam)
-        with hb.on_device(q.device.index):
-            out, keep = _forward(call, qr, kr, vr, t32, l32, True)
-        ctx.call = call
-        ctx.like = (table.dtype if table is not None else None, lam.dtype if lam is not None else None)
-        ctx.save_for_backward(qr, kr, vr, t32, l32, keep, out if call.maps == 1 and q.dtype == torch.float32 else None)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):  # noqa: ANN001
-        q, k, v, table, lam, keep, out = ctx.saved_tensors
-        with hb.on_device(q.device.index):
-            dq, dk, dv = (_empty_like_rows(t, t.shape[2], t.shape[3]) for t in (q, k, v))
-            dtable, dlam = _backward(ctx.call, q, k, v, table, lam, keep, out, _rows(dout.to(q.dtype)), dq, dk, dv, ctx.needs_input_grad[3],
-                                     ctx.needs_input_grad[4])
-            if dtable is not None:
-                dtable = dtable.to(ctx.like[0])
-            if dlam is not None:
-                dlam = dlam.to(ctx.like[1])
-        return dq, dk, dv, dtable, dlam, None
-
-
+# ---------------------------------------------------------------------------------------------------------- operators
 def _check(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor | None, lam: torch.Tensor | None,
            buckets: RelativeBuckets | None, key_mask: torch.Tensor | None, query_offset: int | torch.Tensor) -> None:
     maps = 1 if lam is None else 2
@@ -376,14 +198,22 @@ def _attend(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: t
         return attention_reference(q, k, v, lam, table, buckets, key_mask, scale, query_offset)
     qoff = None
     if torch.is_tensor(query_offset):
-        qoff = query_offset.expand(q.shape[0]).contiguous()
-        query_offset = 0
-    call = _Call(buckets, key_mask, qoff, int(query_offset), scale, 1 if lam is None else 2)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (table is not None and table.requires_grad)
-                                    or (lam is not None and lam.requires_grad)):
-        return _EncoderAttention.apply(q, k, v, table, lam, call)
-    with hb.on_device(q.device.index):
-        return _forward(call, _rows(q.detach()), _rows(k.detach()), _rows(v.detach()), _f32(table), _f32(lam), False)[0]
+        qoff, query_offset = query_offset.expand(q.shape[0]).contiguous(), 0
+    call = _ops or _load()
+    if buckets is None:
+        return call(q, k, v, None, lam, None, None, None, 0, 0, 0, key_mask, None, 0, scale)
+    return call(q, k, v, table, lam, buckets.lut, buckets.order, buckets.start, buckets.radius, buckets.cols, buckets.num_buckets, key_mask, qoff,
+                int(query_offset), scale)
+
+
+_ops: Callable[..., torch.Tensor] | None = None
+
+
+def _load() -> Callable[..., torch.Tensor]:
+    """The kernels' host side (csrc/torch/encoder_ops.cpp)."""
+    global _ops
+    _ops = native.torch_ops().attention
+    return _ops
 
 
 def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, buckets: RelativeBuckets, *,

@@ -10,8 +10,6 @@ path can never fail silently.
 from __future__ import annotations
 
 import ctypes as C
-from collections.abc import Iterator
-from contextlib import contextmanager, nullcontext
 from typing import Any
 
 import numpy as np
@@ -187,36 +185,6 @@ def call(name: str, *args: Any) -> None:
     fn = getattr(lib(), name)
     fn.restype = C.c_int
     check(fn(*args, stream_ptr()), name)
-
-
-_packed_fns: dict[str, Any] = {}
-
-
-def call_packed(name: str, args: bytes, device_index: int) -> None:
-    """Call ``name(args, stream)`` - one C struct packed by the caller - on the current stream of the device, raising on a
-    non-zero return code.  The entry point is bound once: a call costs its launches and little else."""
-    fn = _packed_fns.get(name)
-    if fn is None:
-        fn = getattr(lib(), name)
-        fn.restype, fn.argtypes = C.c_int, [C.c_char_p, VP]
-        _packed_fns[name] = fn
-    code = fn(args, torch._C._cuda_getCurrentRawStream(device_index))
-    if code:
-        check(code, name)
-
-
-@contextmanager
-def _other_device(index: int) -> Iterator[None]:
-    with torch.cuda.device(index):
-        yield
-
-
-_here = nullcontext()
-
-
-def on_device(index: int) -> Any:
-    """Context in which device ``index`` is the current one (free when it already is)."""
-    return _here if torch.cuda.current_device() == index else _other_device(index)
 
 
 def f32(x: float) -> C.c_float:

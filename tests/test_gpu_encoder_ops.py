@@ -326,3 +326,12 @@ def test_empty_calls(maps):
         assert out.shape == inp["dout"].shape and bool((out == 0).all())
         out.sum().backward()
         assert all(x.grad is None or bool((x.grad == 0).all()) for n, x in t.items() if n != "dout" and x is not None)
+
+
+def test_once_differentiable():
+    p = _plan(16)
+    inp = _inputs(torch.float32, 1, 1, 8, 8, 1, 1, 8, p)
+    q = inp["q"].requires_grad_(True)
+    g = torch.autograd.grad(_call(inp, p, None, 0).square().sum(), q, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="once"):
+        g.sum().backward()
