@@ -14,8 +14,6 @@ using namespace atrihip;
 
 namespace {
 
-// Waves per SIMD the register allocation leaves room for: two where 256 registers hold the kernel (32-wide heads), else one.
-constexpr int waves_of(int D) { return D <= 32 ? 2 : 1; }
 constexpr int kDsPitch = kTile + 4;  // row pitch of a wave's 16 x 64 tile of dS on its way to the diagonal sums
 
 __device__ __forceinline__ void wave_lds_fence() {  // orders a wave's own LDS writes before its other lanes' reads
@@ -57,7 +55,7 @@ __device__ __forceinline__ void add_tile(const EncAttnArgs& a, float* sums, cons
 
 // One 4-wave workgroup per (head, 64 QS queries, key range) and q_chunk samples, one after the other.
 template <typename T, int D, int M, int QS, bool BIAS, int NT>
-__global__ __launch_bounds__(256, NT > 0 ? 1 : waves_of(D)) void enc_attn_bwd_q_kernel(EncAttnArgs a) {
+__global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncQueries)) void enc_attn_bwd_q_kernel(EncAttnArgs a) {
   using O = Ops<T>;
   using Frag = typename O::Frag;
   constexpr int DV = D * M, DC = D / O::kDims, VC = DV / O::kDims, ND = D / 16, NKB = 4 / O::kSub;
@@ -66,7 +64,7 @@ __global__ __launch_bounds__(256, NT > 0 ? 1 : waves_of(D)) void enc_attn_bwd_q_
   T* k_lds = reinterpret_cast<T*>(smem);
   T* v_lds = k_lds + M * kTile * PK;
   int* pos_lds = reinterpret_cast<int*>(v_lds + kTile * PV);
-  float* bias_lds = reinterpret_cast<float*>(pos_lds + kTile);
+  float* bias_lds = reinterpret_cast<float*>(pos_lds + (NT ? NT : 1) * kTile);
   const int slots = BIAS ? 2 * a.R + 1 : 0, R2 = 2 * a.R;
   float* ds_lds = bias_lds + ((M * slots + 3) & ~3);
   float* sum_lds = ds_lds + 4 * 16 * kDsPitch;
@@ -121,12 +119,13 @@ __global__ __launch_bounds__(256, NT > 0 ? 1 : waves_of(D)) void enc_attn_bwd_q_
   // Boards: the bias of this wave's pairs, and the sums of their dS over the samples.
   float4v bias_reg[M][QS][NT ? NT * 4 : 1], sum_reg[M][QS][NT ? NT * 4 : 1];
   if constexpr (NT > 0) {
+    if (tid < NT * kTile) pos_lds[tid] = token_pos(tid, a.W);
     __syncthreads();
 #pragma unroll
     for (int kt = 0; kt < NT * 4; ++kt)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int key = kt * 16 + q4 * 4 + j, pos = token_pos(key, a.W);
+        const int key = kt * 16 + q4 * 4 + j, pos = pos_lds[key];
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
@@ -389,7 +388,7 @@ __global__ __launch_bounds__(256, NT > 0 ? 1 : waves_of(D)) void enc_attn_bwd_q_
               for (int kt = 0; kt < 4; ++kt)
                 *reinterpret_cast<float4v*>(buf + l15 * kDsPitch + kt * 16 + q4 * 4) = sum_reg[m][s][tt * 4 + kt];
               wave_lds_fence();
-              add_tile(a, my_sums + m * slots, buf, token_pos(tt * kTile + lane, a.W), token_q[s], 0, 0, lane, lo[m], hi[m]);
+              add_tile(a, my_sums + m * slots, buf, pos_lds[tt * kTile + lane], token_q[s], 0, 0, lane, lo[m], hi[m]);
               wave_lds_fence();
             }
       }
@@ -420,7 +419,7 @@ __global__ __launch_bounds__(256, NT > 0 ? 1 : waves_of(D)) void enc_attn_bwd_q_
 // One 4-wave workgroup per (key / value head, 64 KS keys, query range) and k_chunk samples; a wave owns 16 KS keys and walks the
 // query tiles of every query head that shares them.
 template <typename T, int D, int M, int KS, bool BIAS, int NT>
-__global__ __launch_bounds__(256, waves_of(D)) void enc_attn_bwd_k_kernel(EncAttnArgs a) {
+__global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, sizeof(T) == 2, kEncKeys)) void enc_attn_bwd_k_kernel(EncAttnArgs a) {
   using O = Ops<T>;
   using Frag = typename O::Frag;
   constexpr int DV = D * M, DC = D / O::kDims, VC = DV / O::kDims, ND = D / 16, NV = DV / 16, NKB = 4 / O::kSub;
@@ -429,7 +428,7 @@ __global__ __launch_bounds__(256, waves_of(D)) void enc_attn_bwd_k_kernel(EncAtt
   T* q_lds = reinterpret_cast<T*>(smem);
   T* g_lds = q_lds + M * kTile * PQ;
   int* pos_lds = reinterpret_cast<int*>(g_lds + kTile * PG);
-  float* top_lds = reinterpret_cast<float*>(pos_lds + kTile);
+  float* top_lds = reinterpret_cast<float*>(pos_lds + (NT ? NT : 1) * kTile);
   float* inv_lds = top_lds + M * kTile;
   float* delta_lds = inv_lds + M * kTile;
   int* far_lds = reinterpret_cast<int*>(delta_lds + M * kTile);  // one flag per map (and padding)
@@ -480,12 +479,13 @@ __global__ __launch_bounds__(256, waves_of(D)) void enc_attn_bwd_k_kernel(EncAtt
   if constexpr (NT > 0) {
     fill_bias(a, bias_lds, kvh, M, tid);
     bias_head = kvh;
+    if (tid < NT * kTile) pos_lds[tid] = token_pos(tid, a.W);
     __syncthreads();
 #pragma unroll
     for (int qt = 0; qt < NT * 4; ++qt)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int pos = token_pos(qt * 16 + q4 * 4 + j, a.W);
+        const int pos = pos_lds[qt * 16 + q4 * 4 + j];
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
@@ -785,39 +785,42 @@ __global__ __launch_bounds__(1024) void enc_dlam_kernel(const float* delta2, flo
   }
 }
 
-template <typename T, int D, int M, int S, bool BIAS, int NT = 0>
+template <typename T, int D, int M, bool BIAS, int NT>
+int launch_bwd_k(const EncAttnArgs& a, hipStream_t stream) {
+  using O = Ops<T>;
+  constexpr int KS = enc_columns_of(D, M, NT, kEncKeys);
+  const size_t lds = sizeof(T) * (size_t)kTile * (M * O::row_pitch(D) + O::row_pitch(D * M)) + (NT ? NT : 1) * kTile * sizeof(int) +
+                     sizeof(float) * (3 * M * kTile + 4 + (BIAS ? M * (2 * a.R + 1) : 0));
+  const int rc = enc_lds(enc_attn_bwd_k_kernel<T, D, M, KS, BIAS, NT>, lds);
+  if (rc) return rc;
+  const int nkt = (a.Lk + 64 * KS - 1) / (64 * KS);
+  hipLaunchKernelGGL((enc_attn_bwd_k_kernel<T, D, M, KS, BIAS, NT>), dim3((unsigned)((a.B + a.k_chunk - 1) / a.k_chunk * a.KV * nkt * a.k_splits)), dim3(256),
+                     lds, stream, a);
+  return hip_err(hipGetLastError());
+}
+
+template <typename T, int D, int M, bool BIAS, int NT = 0>
 int launch_bwd(EncAttnArgs a, hipStream_t stream) {
   using O = Ops<T>;
-  constexpr int NK = NT;  // the key-owned pass unrolls the same way where heads are not shared
+  constexpr int QS = enc_columns_of(D, M, NT, kEncQueries);
   const size_t slots = BIAS ? 2 * a.R + 1 : 0;
-  const size_t tiles = sizeof(T) * (size_t)kTile * (M * O::row_pitch(D) + O::row_pitch(D * M)) + kTile * sizeof(int);
-  size_t lds_q = tiles;
-  if (BIAS) lds_q += sizeof(float) * ((M * slots + 3) / 4 * 4 + 4 * 16 * kDsPitch);
+  size_t lds = sizeof(T) * (size_t)kTile * (M * O::row_pitch(D) + O::row_pitch(D * M)) + (NT ? NT : 1) * kTile * sizeof(int);
+  if (BIAS) lds += sizeof(float) * ((M * slots + 3) / 4 * 4 + 4 * 16 * kDsPitch);
   a.hist_rows = 4;
   if (BIAS && a.hist) {
     // a row of sums per wave; one for all where four rows would leave a single workgroup per CU
-    if (lds_q + sizeof(float) * 4 * M * slots > kMaxLds / 2) a.hist_rows = 1;
-    lds_q += sizeof(float) * a.hist_rows * M * slots;
+    if (lds + sizeof(float) * 4 * M * slots > kMaxLds / 2) a.hist_rows = 1;
+    lds += sizeof(float) * a.hist_rows * M * slots;
   }
-  int rc = enc_lds(enc_attn_bwd_q_kernel<T, D, M, S, BIAS, NT>, lds_q);
+  int rc = enc_lds(enc_attn_bwd_q_kernel<T, D, M, QS, BIAS, NT>, lds);
   if (rc) return rc;
-  const int nqt = (a.Lq + 64 * S - 1) / (64 * S), nkt = (a.Lk + 64 * S - 1) / (64 * S);
-  hipLaunchKernelGGL((enc_attn_bwd_q_kernel<T, D, M, S, BIAS, NT>), dim3((unsigned)((a.B + a.q_chunk - 1) / a.q_chunk * a.H * nqt * a.q_splits)), dim3(256),
-                     lds_q, stream, a);
+  const int nqt = (a.Lq + 64 * QS - 1) / (64 * QS);
+  hipLaunchKernelGGL((enc_attn_bwd_q_kernel<T, D, M, QS, BIAS, NT>), dim3((unsigned)((a.B + a.q_chunk - 1) / a.q_chunk * a.H * nqt * a.q_splits)), dim3(256),
+                     lds, stream, a);
   rc = hip_err(hipGetLastError());
   if (rc) return rc;
-  const size_t lds_k = tiles + sizeof(float) * (3 * M * kTile + 4 + M * slots);
-  const dim3 grid((unsigned)((a.B + a.k_chunk - 1) / a.k_chunk * a.KV * nkt * a.k_splits));
-  if (NK > 0 && (a.KV != a.H || a.k_splits > 1)) {
-    rc = enc_lds(enc_attn_bwd_k_kernel<T, D, M, S, BIAS, 0>, lds_k);
-    if (rc) return rc;
-    hipLaunchKernelGGL((enc_attn_bwd_k_kernel<T, D, M, S, BIAS, 0>), grid, dim3(256), lds_k, stream, a);
-  } else {
-    rc = enc_lds(enc_attn_bwd_k_kernel<T, D, M, S, BIAS, NK>, lds_k);
-    if (rc) return rc;
-    hipLaunchKernelGGL((enc_attn_bwd_k_kernel<T, D, M, S, BIAS, NK>), grid, dim3(256), lds_k, stream, a);
-  }
-  return hip_err(hipGetLastError());
+  // the key-owned pass of a board unrolls where no heads are shared
+  return NT > 0 && a.KV == a.H ? launch_bwd_k<T, D, M, BIAS, NT>(a, stream) : launch_bwd_k<T, D, M, BIAS, 0>(a, stream);
 }
 
 template <typename T>
@@ -847,18 +850,18 @@ int join_grads(const EncAttnArgs& a, hipStream_t stream) {
 
 template <typename T>
 int dispatch_bwd(const EncAttnArgs& a, hipStream_t stream) {
-  const int w = enc_width(a.D), nt = a.q_splits == 1 ? enc_board_tiles(a.table ? a.W : 0, a.Lk, a.D, a.M) : 0;
+  const int w = enc_width(a.D), nt = enc_board_tiles(a.table ? a.W : 0, a.Lk, a.D, a.M);
+  if (nt > 0 && (a.q_splits > 1 || (a.KV == a.H && a.k_splits > 1))) return -18;
   if (a.M == 1) {
-    if (nt == 2) return launch_bwd<T, 32, 1, 2, true, 2>(a, stream);
-    if (nt == 4) return launch_bwd<T, 32, 1, 1, true, 4>(a, stream);
-    if (w == 32 && enc_columns(a.W, a.Lq, a.Lk, a.D, a.M, false) == 1) return launch_bwd<T, 32, 1, 1, true>(a, stream);
-    if (w == 32) return launch_bwd<T, 32, 1, 2, true>(a, stream);
-    if (w == 64) return launch_bwd<T, 64, 1, 2, true>(a, stream);
-    return launch_bwd<T, 128, 1, 1, true>(a, stream);
+    if (nt == 2) return launch_bwd<T, 32, 1, true, 2>(a, stream);
+    if (nt == 4) return launch_bwd<T, 32, 1, true, 4>(a, stream);
+    if (w == 32) return launch_bwd<T, 32, 1, true>(a, stream);
+    if (w == 64) return launch_bwd<T, 64, 1, true>(a, stream);
+    return launch_bwd<T, 128, 1, true>(a, stream);
   }
-  if (nt == 2) return launch_bwd<T, 32, 2, 1, true, 2>(a, stream);
-  if (w == 32) return a.table ? launch_bwd<T, 32, 2, 1, true>(a, stream) : launch_bwd<T, 32, 2, 1, false>(a, stream);
-  return a.table ? launch_bwd<T, 64, 2, 1, true>(a, stream) : launch_bwd<T, 64, 2, 1, false>(a, stream);
+  if (nt == 2) return launch_bwd<T, 32, 2, true, 2>(a, stream);
+  if (w == 32) return a.table ? launch_bwd<T, 32, 2, true>(a, stream) : launch_bwd<T, 32, 2, false>(a, stream);
+  return a.table ? launch_bwd<T, 64, 2, true>(a, stream) : launch_bwd<T, 64, 2, false>(a, stream);
 }
 
 }  // namespace
@@ -886,7 +889,7 @@ int atri_enc_attn_bwd(const EncAttnArgs* args, hipStream_t stream) {
   rc = a.bf16 ? join_grads<unsigned short>(a, stream) : join_grads<float>(a, stream);
   if (rc) return rc;
   if (a.hist) {
-    const int per = 64 * enc_columns(a.table ? a.W : 0, a.Lq, a.Lk, a.D, a.M, false), nqt = (a.Lq + per - 1) / per;
+    const int per = 64 * enc_columns(a.table ? a.W : 0, a.Lq, a.Lk, a.D, a.M, kEncQueries), nqt = (a.Lq + per - 1) / per;
     hipLaunchKernelGGL(enc_hist_sum_kernel, dim3((slots + 63) / 64, hm, a.shares), dim3(256), 0, stream, a.hist, a.mid,
                        (a.B + a.q_chunk - 1) / a.q_chunk, a.H, nqt * a.q_splits, a.M, slots, a.shares);
     rc = hip_err(hipGetLastError());

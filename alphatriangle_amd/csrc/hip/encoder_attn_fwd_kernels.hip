@@ -15,7 +15,7 @@ namespace {
 // pass follows, for delta = dO . o has to match dP = dO V^T to 32 bits: the gradients of the table and of lam are sums
 // of p (dP - delta) in which everything but the error of delta cancels (with one fragment they were 1e-3 off).
 template <typename T, int D, int M, int QS, bool BIAS, int PL, int NT>
-__global__ __launch_bounds__(256, NT > 0 ? 2 : 1) void enc_attn_fwd_kernel(EncAttnArgs a) {
+__global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncForward)) void enc_attn_fwd_kernel(EncAttnArgs a) {
   using O = Ops<T>;
   using Frag = typename O::Frag;
   constexpr int DV = D * M, DC = D / O::kDims, NV = DV / 16, NKB = 4 / O::kSub;
@@ -24,7 +24,7 @@ __global__ __launch_bounds__(256, NT > 0 ? 2 : 1) void enc_attn_fwd_kernel(EncAt
   T* k_lds = reinterpret_cast<T*>(smem);
   T* v_lds = k_lds + M * kTile * PK;
   int* pos_lds = reinterpret_cast<int*>(v_lds + kTile * PV);
-  float* bias_lds = reinterpret_cast<float*>(pos_lds + kTile);
+  float* bias_lds = reinterpret_cast<float*>(pos_lds + (NT ? NT : 1) * kTile);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, q4 = lane >> 4;
   const int nqt = (a.Lq + 64 * QS - 1) / (64 * QS);
@@ -79,12 +79,13 @@ __global__ __launch_bounds__(256, NT > 0 ? 2 : 1) void enc_attn_fwd_kernel(EncAt
   for (int s = 0; s < QS; ++s) token_q[s] = BIAS ? token_pos(q_first + s * 16 + l15, a.W) : 0;
   float4v bias_reg[M][QS][NT ? NT * 4 : 1];
   if constexpr (NT > 0) {
+    if (tid < NT * kTile) pos_lds[tid] = token_pos(tid, a.W);
     __syncthreads();
 #pragma unroll
     for (int kt = 0; kt < NT * 4; ++kt)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int key = kt * 16 + q4 * 4 + j, pos = token_pos(key, a.W);
+        const int key = kt * 16 + q4 * 4 + j, pos = pos_lds[key];
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
@@ -356,7 +357,7 @@ __global__ __launch_bounds__(256) void key_words_kernel(const unsigned char* mas
 template <typename T, int D, int M, int QS, bool BIAS, int PL, int NT>
 int launch_fwd_planes(const EncAttnArgs& a, hipStream_t stream) {
   using O = Ops<T>;
-  size_t lds = sizeof(T) * (size_t)kTile * (M * O::row_pitch(D) + O::tr_pitch(D * M)) + kTile * sizeof(int);
+  size_t lds = sizeof(T) * (size_t)kTile * (M * O::row_pitch(D) + O::tr_pitch(D * M)) + (NT ? NT : 1) * kTile * sizeof(int);
   if (BIAS) lds += sizeof(float) * (size_t)M * (2 * a.R + 1);
   const int rc = enc_lds(enc_attn_fwd_kernel<T, D, M, QS, BIAS, PL, NT>, lds);
   if (rc) return rc;
@@ -376,8 +377,9 @@ int launch_fwd(const EncAttnArgs& a, hipStream_t stream) {
 
 template <typename T>
 int dispatch_fwd(const EncAttnArgs& a, hipStream_t stream) {
-  const int w = enc_width(a.D), nt = a.splits == 1 ? enc_board_tiles(a.table ? a.W : 0, a.Lk, a.D, a.M) : 0;
-  const bool two = enc_columns(a.table ? a.W : 0, a.Lq, a.Lk, a.D, a.M, true) == 2;
+  const int w = enc_width(a.D), nt = enc_board_tiles(a.table ? a.W : 0, a.Lk, a.D, a.M);
+  if (nt > 0 && a.splits > 1) return -18;
+  const bool two = enc_columns(a.table ? a.W : 0, a.Lq, a.Lk, a.D, a.M, kEncForward) == 2;
   if (a.M == 1) {
     if (nt == 2) return launch_fwd<T, 32, 1, 2, true, 2>(a, stream);
     if (nt == 4) return launch_fwd<T, 32, 1, 1, true, 4>(a, stream);

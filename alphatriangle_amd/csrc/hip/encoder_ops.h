@@ -4,6 +4,12 @@
 
 struct ihipStream_t;
 
+#ifndef ENC_Q2
+#define ENC_Q2 2
+#endif
+#ifndef ENC_Q2W
+#define ENC_Q2W 2
+#endif
 namespace atrihip {
 
 constexpr int kTile = 64;  // keys (queries in the key-owned pass) staged per step of the attention kernels
@@ -56,12 +62,23 @@ inline int enc_board_tiles(int W, int Lk, int D, int M) {
   if (W <= 0 || D > 32 || tiles < 2) return 0;
   return tiles == 2 ? 2 : tiles <= 4 && M == 1 ? 4 : 0;
 }
+enum EncPass { kEncForward = 0, kEncQueries = 1, kEncKeys = 2 };  // forward, query-owned and key-owned backward pass
 // 16-row columns per wave: queries in the forward and the query-owned pass, keys in the key-owned one.
-inline int enc_columns(int W, int L, int Lk, int D, int M, bool forward) {
-  if (M == 2 || D > 64) return 1;
+constexpr int enc_columns_of(int D, int M, int nt, int pass) {
+  if (M == 2 || D > 64 || nt == 4) return 1;
+  return nt == 2 && pass == kEncQueries ? ENC_Q2 : 2;  // two: every staged fragment feeds two products
+}
+inline int enc_columns(int W, int L, int Lk, int D, int M, int pass) {
   const int nt = enc_board_tiles(W, Lk, D, M);
-  if (nt) return nt == 2 ? 2 : 1;
-  return forward && L <= 64 ? 1 : 2;  // two, once they exist: every staged fragment then feeds two products
+  return nt == 0 && pass == kEncForward && L <= 64 ? 1 : enc_columns_of(D, M, nt, pass);
+}
+// Waves per SIMD the register allocation of a kernel leaves room for.  These kernels wait on LDS and on the matrix and
+// exponential pipes, so a second wave is worth some spilled registers (two 4095-token sequences in bf16, both backward
+// passes: 857 us with one, 466 us with two); a third is not, except where the kernel nearly fits anyway.
+constexpr int enc_waves(int D, int M, int nt, int columns, bool bf16, int pass) {
+  if (pass == kEncForward) return nt == 4 || (bf16 && M == 1 && D == 64 && columns == 2) ? 3 : 2;
+  if (pass == kEncQueries && nt == 2 && M == 2) return 1;
+  return pass == kEncQueries && nt == 2 ? ENC_Q2W : 2;
 }
 
 // The residual joint: threads that own a row (8 values each) and threads of a workgroup.

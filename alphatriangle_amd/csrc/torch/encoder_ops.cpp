@@ -96,13 +96,27 @@ void strides(long long (&s)[3], const Tensor& t) {
 }
 
 // Key (query) ranges per workgroup row and samples per workgroup of a launch with `groups` workgroups per sample that walk
-// `steps` tiles each.  `full` workgroups fill the card.  With fewer the tiles are split, four of them at least to a
-// range (a range's partial sums cost a write, a read and the join); with more a workgroup takes several samples.
-void plan(int64_t samples, int64_t groups, int64_t steps, int64_t full, int& splits, int& chunk) {
+// `steps` tiles each, on a card that holds `resident` of them at a time.
+//   more than fit: every workgroup takes several samples (its bias is laid out once, loads run ahead across samples), so that
+//   one round of them covers the batch;
+//   fewer: the tiles are split where that shortens the rounds.  A workgroup costs its tiles and two more for its ends, a
+//   split the write and join of its partial sums.
+void plan(int64_t samples, int64_t groups, int64_t steps, int64_t resident, int& splits, int& chunk) {
   const int64_t n = samples * groups;
-  splits = chunk = 1;
-  if (2 * n <= full && steps >= 8) splits = static_cast<int>(std::clamp<int64_t>(up(full, n), 1, std::min<int64_t>(steps / 4, 256)));
-  else chunk = static_cast<int>(std::max<int64_t>(1, n / full));
+  splits = 1;
+  chunk = static_cast<int>(std::max<int64_t>(1, n / resident));
+  if (chunk > 1) return;
+  const auto cost = [&](int64_t s) { return static_cast<double>(up(n * s, resident) * (up(steps, s) + 2)) + (s > 1 ? 2.0 + 0.05 * static_cast<double>(s) : 0.0); };
+  double best = cost(1);
+  for (int64_t s = 2; s <= std::min<int64_t>(steps / 2, 128); ++s)
+    if (cost(s) < 0.95 * best) best = cost(s), splits = static_cast<int>(s);
+}
+
+// Workgroups of one pass that the card's 256 compute units hold at a time (four waves each, one per SIMD).
+int64_t resident(const EncAttnArgs& a, int pass) {
+  const int nt = atrihip::enc_board_tiles(a.W, a.Lk, a.D, a.M);
+  const int width = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
+  return 256 * atrihip::enc_waves(width, a.M, nt, atrihip::enc_columns(a.W, a.Lq, a.Lk, a.D, a.M, pass), a.bf16 != 0, pass);
 }
 
 struct Sizes {
@@ -168,8 +182,9 @@ Tensor attention_forward(const Call& c, const Tensor& q, const Tensor& k, const 
     if (s.n_stat) a.stat = at_keep + s.n_words;
     if (s.n_o32) a.o32 = at_keep + s.n_words + s.n_stat;
   }
-  const int64_t per = 64 * atrihip::enc_columns(a.W, a.Lq, a.Lk, a.D, a.M, true);
-  plan(s.b, s.h * up(s.lq, per), up(s.lk, atrihip::kTile), 1024, a.splits, a.chunk);
+  const bool board = atrihip::enc_board_tiles(a.W, a.Lk, a.D, a.M) > 0;  // unrolled over its tiles: never split
+  const int64_t per = 64 * atrihip::enc_columns(a.W, a.Lq, a.Lk, a.D, a.M, atrihip::kEncForward);
+  plan(s.b, s.h * up(s.lq, per), board ? 1 : up(s.lk, atrihip::kTile), resident(a, atrihip::kEncForward), a.splits, a.chunk);
   Tensor part;
   if (a.splits > 1) {
     const int64_t n = a.splits * s.maps * s.rows;
@@ -228,9 +243,12 @@ struct Attention : torch::autograd::Function<Attention> {
     }
     // edges: q, k, v, then the table and lam where they are given
     const bool want_table = table.defined() && ctx->needs_input_grad(3), want_lam = lam.defined() && ctx->needs_input_grad(table.defined() ? 4 : 3);
-    const int64_t per = 64 * atrihip::enc_columns(a.W, a.Lq, a.Lk, a.D, a.M, false), nqt = up(s.lq, per), nkt = up(s.lk, per);
-    plan(s.b, s.h * nqt, up(s.lk, atrihip::kTile), 512, a.q_splits, a.q_chunk);
-    plan(s.b, s.kv * nkt, s.h / s.kv * up(s.lq, atrihip::kTile), 512, a.k_splits, a.k_chunk);
+    const int64_t nqt = up(s.lq, 64 * atrihip::enc_columns(a.W, a.Lq, a.Lk, a.D, a.M, atrihip::kEncQueries));
+    // shared heads take the general form of the key-owned pass
+    const int64_t nkt = up(s.lk, 64 * atrihip::enc_columns(s.h == s.kv ? a.W : 0, a.Lq, a.Lk, a.D, a.M, atrihip::kEncKeys));
+    const bool board = atrihip::enc_board_tiles(a.W, a.Lk, a.D, a.M) > 0;  // unrolled over its tiles: never split
+    plan(s.b, s.h * nqt, board ? 1 : up(s.lk, atrihip::kTile), resident(a, atrihip::kEncQueries), a.q_splits, a.q_chunk);
+    plan(s.b, s.kv * nkt, board && s.h == s.kv ? 1 : s.h / s.kv * up(s.lq, atrihip::kTile), resident(a, atrihip::kEncKeys), a.k_splits, a.k_chunk);
     const int64_t hm = s.h * s.maps, slots = 2 * c.radius + 1, per_head = up(s.b, a.q_chunk) * a.q_splits * nqt;
     a.shares = static_cast<int>(std::clamp<int64_t>(per_head / 16, 1, 64));
     const int64_t n_delta = up(s.maps * s.rows, 4) * 4, n_dq = a.q_splits > 1 ? a.q_splits * s.rows * s.maps * s.d : 0;
