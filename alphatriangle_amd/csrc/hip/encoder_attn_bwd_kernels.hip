@@ -113,6 +113,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncQu
   float lo[M], hi[M];
 #pragma unroll
   for (int m = 0; m < M; ++m) lo[m] = hi[m] = 0.f;
+  float delta2_sum = 0.f;  // of this lane's queries over the samples
   int token_q[QS];
 #pragma unroll
   for (int s = 0; s < QS; ++s) token_q[s] = BIAS ? token_pos(q_first + s * 16 + l15, a.W) : 0;
@@ -169,7 +170,10 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncQu
           dot += O::dot(dof[s][c], v);
         }
         delta[m][s] = quad_row_sum(dot);
-        if (valid && q4 == 0 && split == 0) a.delta[m * rows + row0 + query] = delta[m][s];
+        if (valid && q4 == 0 && split == 0) {
+          a.delta[m * rows + row0 + query] = delta[m][s];
+          if (M == 2 && m == 1) delta2_sum += delta[m][s];
+        }
       }
     }
     float4v dq[M][QS][ND];
@@ -372,6 +376,10 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncQu
         }
       }
     }
+  }
+  if (M == 2 && a.dlam) {
+    const float all = wave_sum(delta2_sum);
+    if (lane == 0) a.dlam_part[(size_t)group_id * 4 + wave] = all;
   }
   if (!want_sums) return;
   if constexpr (NT > 0) {  // the board's pairs, once for all samples
@@ -722,7 +730,19 @@ __global__ __launch_bounds__(256) void enc_grad_join_kernel(const float* part, i
   Ops<T>::store4(dest + b * sb + token * st + ((long long)g * maps + m) * sh + (col - m * width), s[0], s[1], s[2], s[3]);
 }
 
-// mid[z][h M + m][slot] = sum of hist over a share of head h's workgroups, `per_head` for each of `outer` sample chunks, in order.
+// The small gradients, in a fixed order and (beyond one workgroup's share) 64 bits: the terms of these sums cancel.
+struct SmallGrads {
+  const float* sums;   // [outer, H, per_head, M, slots] sums of dS by position difference
+  const int* order;    // differences by bucket
+  const int* start;
+  float* dtable;       // [buckets, H M]
+  const float* delta2; // [outer, H, per_head, 4] sums of delta_2 by wave
+  float* dlam;         // [H]
+  int outer, H, per_head, M, slots, buckets, table_groups;
+};
+
+// mid[z][h][m][slot] = sum over a share of head h's rows: the first of two steps where there are many sums (SmallGrads then has
+// outer = shares and per_head = 1).
 __global__ __launch_bounds__(256) void enc_hist_sum_kernel(const float* hist, float* mid, int outer, int H, int per_head, int M, int slots, int shares) {
   __shared__ float part[4][64];
   const int slot = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
@@ -745,44 +765,43 @@ __global__ __launch_bounds__(256) void enc_hist_sum_kernel(const float* hist, fl
   }
 }
 
-// dtable[bucket][h M + m]: one wave per (bucket, column) adds the slots of the bucket (order[start[b]] .. order[start[b + 1] - 1]) over
-// all shares, in 64 bits (the terms of these sums cancel).
-__global__ __launch_bounds__(256) void enc_bucket_sum_kernel(const float* mid, const int* order, const int* start, float* dtable, int buckets, int hm,
-                                                             int slots, int shares) {
-  const int w = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (w >= buckets * hm) return;
-  const int bucket = w / hm, col = w - bucket * hm;
-  const int first = start[bucket], n = start[bucket + 1] - first;
-  double s = 0.0;
-  for (int i = lane; i < n * shares; i += 64) {
-    const int z = i / n, e = i - z * n;
-    s += (double)mid[((size_t)z * hm + col) * slots + order[first + e]];
-  }
+__device__ __forceinline__ double wave_sum_d(double s) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off, 64);
-  if (lane == 0) dtable[(size_t)bucket * hm + col] = (float)s;
+  return s;
 }
 
-// dlam[h] = -sum of delta_2 over samples and queries: one workgroup per head, fixed order, 64-bit sums.
-__global__ __launch_bounds__(1024) void enc_dlam_kernel(const float* delta2, float* dlam, int B, int H, int Lq) {
-  __shared__ double part[16];
-  const int h = blockIdx.x, tid = threadIdx.x;
-  const long long n = (long long)B * Lq;
+// One wave per (bucket, head and map) adds the bucket's differences over all rows; the workgroups behind them, one per head, lam's
+// gradient -sum delta_2.
+__global__ __launch_bounds__(256) void enc_small_grads_kernel(SmallGrads a) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if ((int)blockIdx.x < a.table_groups) {
+    const int hm = a.H * a.M, w = blockIdx.x * 4 + wave;
+    if (w >= a.buckets * hm) return;
+    const int bucket = w / hm, col = w - bucket * hm, h = col / a.M, m = col - h * a.M;
+    const int first = a.start[bucket], n = a.start[bucket + 1] - first, rows = a.outer * a.per_head;
+    double s = 0.0;
+#pragma unroll 4
+    for (int i = lane; i < n * rows; i += 64) {
+      const int r = i / n, e = i - r * n, o = r / a.per_head;
+      s += (double)a.sums[((((size_t)o * a.H + h) * a.per_head + (r - o * a.per_head)) * a.M + m) * a.slots + a.order[first + e]];
+    }
+    s = wave_sum_d(s);
+    if (lane == 0) a.dtable[(size_t)bucket * hm + col] = (float)s;
+    return;
+  }
+  __shared__ double part[4];
+  const int h = blockIdx.x - a.table_groups, n = a.per_head * 4;
   double s = 0.0;
 #pragma unroll 4
-  for (long long i = tid; i < n; i += 1024) {
-    const long long b = i / Lq;
-    s += (double)delta2[(b * H + h) * Lq + (i - b * Lq)];
+  for (int i = threadIdx.x; i < a.outer * n; i += 256) {
+    const int o = i / n;
+    s += (double)a.delta2[((size_t)o * a.H + h) * n + (i - o * n)];
   }
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off, 64);
-  if ((tid & 63) == 0) part[tid >> 6] = s;
+  s = wave_sum_d(s);
+  if (lane == 0) part[wave] = s;
   __syncthreads();
-  if (tid == 0) {
-    double all = 0.0;
-    for (int i = 0; i < 16; ++i) all += part[i];
-    dlam[h] = (float)-all;
-  }
+  if (threadIdx.x == 0) a.dlam[h] = (float)-((part[0] + part[1]) + (part[2] + part[3]));
 }
 
 template <typename T, int D, int M, bool BIAS, int NT>
@@ -882,28 +901,36 @@ int atri_enc_attn_bwd(const EncAttnArgs* args, hipStream_t stream) {
         (long long)slots * a.shares >= (1LL << 31))
       return -15;
   }
-  if (a.dlam && a.M != 2) return -14;
+  if (a.dlam && (a.M != 2 || !a.dlam_part)) return -14;
   if ((a.q_splits > 1 && !a.dq_part) || (a.k_splits > 1 && !a.kv_part)) return -17;
   rc = a.bf16 ? dispatch_bwd<unsigned short>(a, stream) : dispatch_bwd<float>(a, stream);
   if (rc) return rc;
   rc = a.bf16 ? join_grads<unsigned short>(a, stream) : join_grads<float>(a, stream);
   if (rc) return rc;
+  if (!a.hist && !a.dlam) return 0;
+  const int per = 64 * enc_columns(a.table ? a.W : 0, a.Lq, a.Lk, a.D, a.M, kEncQueries), nqt = (a.Lq + per - 1) / per;
+  SmallGrads g{a.hist, a.order, a.start, a.dtable, a.dlam_part, a.dlam, (a.B + a.q_chunk - 1) / a.q_chunk, a.H, nqt * a.q_splits, a.M, slots, a.buckets, 0};
   if (a.hist) {
-    const int per = 64 * enc_columns(a.table ? a.W : 0, a.Lq, a.Lk, a.D, a.M, kEncQueries), nqt = (a.Lq + per - 1) / per;
-    hipLaunchKernelGGL(enc_hist_sum_kernel, dim3((slots + 63) / 64, hm, a.shares), dim3(256), 0, stream, a.hist, a.mid,
-                       (a.B + a.q_chunk - 1) / a.q_chunk, a.H, nqt * a.q_splits, a.M, slots, a.shares);
-    rc = hip_err(hipGetLastError());
-    if (rc) return rc;
-    hipLaunchKernelGGL(enc_bucket_sum_kernel, dim3((unsigned)((a.buckets * hm + 3) / 4)), dim3(256), 0, stream, a.mid, a.order, a.start, a.dtable, a.buckets, hm,
-                       slots, a.shares);
-    rc = hip_err(hipGetLastError());
-    if (rc) return rc;
+    g.table_groups = (a.buckets * hm + 3) / 4;
+    // in one step while the sums are few enough to be read slot by slot from L2; each step is a launch of 4.5 us
+    if ((long long)g.outer * g.per_head * hm * slots > (1 << 20)) {
+      hipLaunchKernelGGL(enc_hist_sum_kernel, dim3((slots + 63) / 64, hm, a.shares), dim3(256), 0, stream, a.hist, a.mid, g.outer, a.H, g.per_head, a.M, slots,
+                         a.shares);
+      rc = hip_err(hipGetLastError());
+      if (rc) return rc;
+      SmallGrads t = g;
+      t.sums = a.mid;
+      t.outer = a.shares;
+      t.per_head = 1;
+      hipLaunchKernelGGL(enc_small_grads_kernel, dim3(g.table_groups), dim3(256), 0, stream, t);
+      rc = hip_err(hipGetLastError());
+      if (rc || !a.dlam) return rc;
+      g.table_groups = 0;
+    }
   }
-  if (a.dlam) {
-    hipLaunchKernelGGL(enc_dlam_kernel, dim3(a.H), dim3(1024), 0, stream, a.delta + (long long)a.B * a.H * a.Lq, a.dlam, a.B, a.H, a.Lq);
-    rc = hip_err(hipGetLastError());
-  }
-  return rc;
+  const int groups = g.table_groups + (a.dlam ? a.H : 0);
+  hipLaunchKernelGGL(enc_small_grads_kernel, dim3(groups), dim3(256), 0, stream, g);
+  return hip_err(hipGetLastError());
 }
 
 }  // extern "C"

@@ -296,32 +296,36 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncFo
   }
 }
 
-// Joins the partial softmaxes of `splits` key ranges: one thread per four output values of a row.
-template <typename T, int M>
+// Joins the partial softmaxes of `splits` key ranges, four output values of a row at a time.  SHARES = 4: by four threads, each with a
+// quarter of the ranges, whose loads are under way together - with few rows the kernel is a chain of latencies (one token
+// of four sequences: 7 -> 4.5 us); one thread reads whole lines (two maps of 12004 rows: 19 us with four, 11 us with one).
+template <typename T, int M, int SHARES>
 __global__ __launch_bounds__(256) void enc_attn_join_kernel(EncAttnArgs a) {
   const long long rows = (long long)a.B * a.H * a.Lq;
-  const int quads = a.DV / 4;
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * quads) return;
-  const long long row = i / quads;
-  const int dim = (int)(i - row * quads) * 4;
+  const int quads = a.DV / 4, share = SHARES == 4 ? (threadIdx.x >> 4) & 3 : 0;
+  const long long i = SHARES == 4 ? ((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16 + (threadIdx.x & 15) : (long long)blockIdx.x * 256 + threadIdx.x;
+  const bool on = i < rows * quads;
+  const long long row = on ? i / quads : 0;
+  const int dim = on ? (int)(i - row * quads) * 4 : 0;
   const int query = (int)(row % a.Lq);
   const long long bh = row / a.Lq;
   const int b = (int)(bh / a.H), h = (int)(bh - (long long)b * a.H);
   const float sl2 = a.scale * kLog2E;
+  const long long step = (long long)M * rows;
   float4v r[M];
 #pragma unroll
   for (int m = 0; m < M; ++m) {
     const float* ml = a.part_ml + 2 * (m * rows + row);
     const float* po = a.part_o + (m * rows + row) * a.DV + dim;
-    const long long step = (long long)M * rows;
     float top = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[2 * s * step]);
+#pragma unroll 4
+    for (int s = share; s < a.splits; s += SHARES) top = fmaxf(top, ml[2 * s * step]);
+    if constexpr (SHARES == 4) top = quad_row_max(top);
     const float from = top == -INFINITY ? 0.f : top, base = from * sl2;
     float sum = 0.f;
     float4v acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int s = 0; s < a.splits; ++s) {
+    for (int s = share; s < a.splits; s += SHARES) {
       const float t = ml[2 * s * step];
       const float w = Exponent::far(base) ? Exponent::far_(t, from, sl2) : __builtin_amdgcn_exp2f(t * sl2 - base);
       const float4v p = *reinterpret_cast<const float4v*>(po + s * step * a.DV);
@@ -329,12 +333,15 @@ __global__ __launch_bounds__(256) void enc_attn_join_kernel(EncAttnArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[j] = fmaf(p[j], w, acc[j]);
     }
+    if constexpr (SHARES == 4) sum = quad_row_sum(sum);
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[m][j] = acc[j] * inv;
+    for (int j = 0; j < 4; ++j) r[m][j] = (SHARES == 4 ? quad_row_sum(acc[j]) : acc[j]) * inv;
+    if (!on || share != 0) continue;
     if (a.stat && dim == 0) *reinterpret_cast<float2*>(a.stat + 2 * (m * rows + row)) = make_float2(sum == 0.f ? INFINITY : top, inv);
     if (a.o32) Ops<float>::store4(a.o32 + b * a.o32s[0] + (long long)query * a.o32s[1] + h * a.o32s[2] + m * a.o32s[3] + dim, r[m][0], r[m][1], r[m][2], r[m][3]);
   }
+  if (!on || share != 0) return;
   if constexpr (M == 2) {
     const float lam = a.lam[h];
 #pragma unroll
@@ -381,7 +388,7 @@ int dispatch_fwd(const EncAttnArgs& a, hipStream_t stream) {
   if (nt > 0 && a.splits > 1) return -18;
   const bool two = enc_columns(a.table ? a.W : 0, a.Lq, a.Lk, a.D, a.M, kEncForward) == 2;
   if (a.M == 1) {
-    if (nt == 2) return launch_fwd<T, 32, 1, 2, true, 2>(a, stream);
+    if (nt == 2) return launch_fwd<T, 32, 1, enc_columns_of(32, 1, 2, kEncForward), true, 2>(a, stream);
     if (nt == 4) return launch_fwd<T, 32, 1, 1, true, 4>(a, stream);
     if (w == 32) return two ? launch_fwd<T, 32, 1, 2, true>(a, stream) : launch_fwd<T, 32, 1, 1, true>(a, stream);
     if (w == 64) return two ? launch_fwd<T, 64, 1, 2, true>(a, stream) : launch_fwd<T, 64, 1, 1, true>(a, stream);
@@ -390,6 +397,19 @@ int dispatch_fwd(const EncAttnArgs& a, hipStream_t stream) {
   if (nt == 2) return launch_fwd<T, 32, 2, 1, true, 2>(a, stream);
   if (w == 32) return a.table ? launch_fwd<T, 32, 2, 1, true>(a, stream) : launch_fwd<T, 32, 2, 1, false>(a, stream);
   return a.table ? launch_fwd<T, 64, 2, 1, true>(a, stream) : launch_fwd<T, 64, 2, 1, false>(a, stream);
+}
+
+template <typename T, int M>
+int launch_join(const EncAttnArgs& a, hipStream_t stream) {
+  const long long n = (long long)a.B * a.H * a.Lq * (a.DV / 4);
+  if ((n + 255) / 256 >= (1LL << 31)) return -15;
+  if (n <= 65536) hipLaunchKernelGGL((enc_attn_join_kernel<T, M, 4>), dim3((unsigned)((n + 63) / 64)), dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((enc_attn_join_kernel<T, M, 1>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
+  return hip_err(hipGetLastError());
+}
+template <typename T>
+int join(const EncAttnArgs& a, hipStream_t stream) {
+  return a.M == 1 ? launch_join<T, 1>(a, stream) : launch_join<T, 2>(a, stream);
 }
 
 }  // namespace
@@ -413,17 +433,7 @@ int atri_enc_attn_fwd(const EncAttnArgs* args, hipStream_t stream) {
   }
   const int rc2 = a.bf16 ? dispatch_fwd<unsigned short>(a, stream) : dispatch_fwd<float>(a, stream);
   if (rc2 || a.splits == 1) return rc2;
-  const long long n = (long long)a.B * a.H * a.Lq * (a.DV / 4);
-  if ((n + 255) / 256 >= (1LL << 31)) return -15;
-  const dim3 grid((unsigned)((n + 255) / 256));
-  if (a.bf16) {
-    if (a.M == 1) hipLaunchKernelGGL((enc_attn_join_kernel<unsigned short, 1>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((enc_attn_join_kernel<unsigned short, 2>), grid, dim3(256), 0, stream, a);
-  } else {
-    if (a.M == 1) hipLaunchKernelGGL((enc_attn_join_kernel<float, 1>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((enc_attn_join_kernel<float, 2>), grid, dim3(256), 0, stream, a);
-  }
-  return hip_err(hipGetLastError());
+  return a.bf16 ? join<unsigned short>(a, stream) : join<float>(a, stream);
 }
 
 }  // extern "C"

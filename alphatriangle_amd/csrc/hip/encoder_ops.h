@@ -4,12 +4,6 @@
 
 struct ihipStream_t;
 
-#ifndef ENC_Q2
-#define ENC_Q2 2
-#endif
-#ifndef ENC_Q2W
-#define ENC_Q2W 2
-#endif
 namespace atrihip {
 
 constexpr int kTile = 64;  // keys (queries in the key-owned pass) staged per step of the attention kernels
@@ -41,6 +35,7 @@ struct EncAttnArgs {
   float* dq_part;      // [q_splits, B, H, Lq, M D] partial dQ in 32 bits (q_splits > 1)
   float* kv_part;      // [k_splits, B, KV, Lk, M D + DV] partial dK and dV (k_splits > 1)
   float* dtable;       // [buckets, H M]
+  float* dlam_part;    // [workgroups of the query-owned pass, 4] sums of delta_2 by wave
   float* dlam;         // [H]; nullptr: not wanted
   long long qs[3], ks[3], vs[3], os[3], gs[3], dqs[3], dks[3], dvs[3];  // element strides: sample, token, head
   long long o32s[4];   // o32: sample, token, head, map
@@ -66,7 +61,9 @@ enum EncPass { kEncForward = 0, kEncQueries = 1, kEncKeys = 2 };  // forward, qu
 // 16-row columns per wave: queries in the forward and the query-owned pass, keys in the key-owned one.
 constexpr int enc_columns_of(int D, int M, int nt, int pass) {
   if (M == 2 || D > 64 || nt == 4) return 1;
-  return nt == 2 && pass == kEncQueries ? ENC_Q2 : 2;  // two: every staged fragment feeds two products
+  // two: every staged fragment feeds two products; one where bias and sums of dS share the registers (256 boards of 120 cells,
+  // fp32, query-owned pass: 68 us with two, 51 us with one; forward and key-owned pass: no difference within 3 %)
+  return nt == 2 && pass == kEncQueries ? 1 : 2;
 }
 inline int enc_columns(int W, int L, int Lk, int D, int M, int pass) {
   const int nt = enc_board_tiles(W, Lk, D, M);
@@ -76,9 +73,8 @@ inline int enc_columns(int W, int L, int Lk, int D, int M, int pass) {
 // exponential pipes, so a second wave is worth some spilled registers (two 4095-token sequences in bf16, both backward
 // passes: 857 us with one, 466 us with two); a third is not, except where the kernel nearly fits anyway.
 constexpr int enc_waves(int D, int M, int nt, int columns, bool bf16, int pass) {
-  if (pass == kEncForward) return nt == 4 || (bf16 && M == 1 && D == 64 && columns == 2) ? 3 : 2;
-  if (pass == kEncQueries && nt == 2 && M == 2) return 1;
-  return pass == kEncQueries && nt == 2 ? ENC_Q2W : 2;
+  if (pass == kEncForward) return nt == 4 || (nt == 0 && bf16 && M == 1 && D == 64 && columns == 2) ? 3 : 2;
+  return pass == kEncQueries && nt == 2 && M == 2 ? 1 : 2;
 }
 
 // The residual joint: threads that own a row (8 values each) and threads of a workgroup.

@@ -21,20 +21,6 @@ __device__ __forceinline__ float read1(const float* p) { return *p; }
 __device__ __forceinline__ float read1(const unsigned short* p) { return bf16_to_float(*p); }
 __device__ __forceinline__ void write1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void write1(unsigned short* p, float v) { *p = float_to_bf16(v); }
-__device__ __forceinline__ void read8(const float* p, float* v) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void read8(const unsigned short* p, float* v) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const unsigned w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-  }
-}
 __device__ __forceinline__ void write8(float* p, const float* v) {
   reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -43,20 +29,61 @@ __device__ __forceinline__ void write8(unsigned short* p, const float* v) {
   *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
-// A thread's share of a row: the column of its value e, and whole-share transfers (zeros beyond the row).
+// A thread's share of a row as it lies in memory: 16-byte pieces (VEC) or single values, zeros beyond the row.  Rows are read into
+// these one step ahead of their use, so that a workgroup always has loads under way.
+template <typename T, int LANES, bool VEC>
+struct Raw {
+  static constexpr int kPieces = sizeof(T) / 2;  // of 16 bytes
+  uint4 v[VEC ? kPieces : 1];
+  T one[VEC ? 1 : 8];
+  static __device__ __forceinline__ int col(int lane, int e) { return VEC ? lane * 8 + e : e * LANES + lane; }
+  __device__ __forceinline__ void read(const T* row, int D, int lane) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        v[i] = make_uint4(0, 0, 0, 0);
+        if (lane * 8 < D) v[i] = reinterpret_cast<const uint4*>(row + lane * 8)[i];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) one[e] = col(lane, e) < D ? row[col(lane, e)] : T(0);
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < (VEC ? kPieces : 1); ++i) v[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int e = 0; e < (VEC ? 1 : 8); ++e) one[e] = T(0);
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    if constexpr (VEC && sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f[4 * i] = __uint_as_float(v[i].x); f[4 * i + 1] = __uint_as_float(v[i].y);
+        f[4 * i + 2] = __uint_as_float(v[i].z); f[4 * i + 3] = __uint_as_float(v[i].w);
+      }
+    } else if constexpr (VEC) {
+      const unsigned w[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = read1(&one[e]);
+    }
+  }
+};
+
 template <int LANES, bool VEC>
 struct Share {
   static __device__ __forceinline__ int col(int lane, int e) { return VEC ? lane * 8 + e : e * LANES + lane; }
   template <typename T>
   static __device__ __forceinline__ void read(const T* row, int D, int lane, float (&v)[8]) {
-    if constexpr (VEC) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
-      if (lane * 8 < D) read8(row + lane * 8, v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = col(lane, e) < D ? read1(row + col(lane, e)) : 0.f;
-    }
+    Raw<T, LANES, VEC> r;
+    r.read(row, D, lane);
+    r.get(v);
   }
   template <typename T>
   static __device__ __forceinline__ void write(T* row, int D, int lane, const float (&v)[8]) {
@@ -70,24 +97,36 @@ struct Share {
   }
 };
 
-constexpr int kScratch = 8;  // floats per use: one per wave
-
-// Sum over the LANES threads of a row, the same value in all of them.  Rows of several waves meet in `scratch`, a slot of its own
-// for every sum of a step and two sets of slots in turn, so that one barrier per sum is enough.
-template <int LANES>
-__device__ __forceinline__ float row_sum(float v, float* scratch) {
+// Sums over the LANES threads of a row, the same values in all of them.  Rows of several waves meet in `scratch` (N floats per wave):
+// slots of their own for every set of sums of a step and two sets of slots in turn, so that one barrier per set is enough.
+constexpr int kScratch = 8 * 3;
+template <int LANES, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float* scratch) {
 #pragma unroll
-  for (int off = (LANES < 64 ? LANES : 64) / 2; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+  for (int off = (LANES < 64 ? LANES : 64) / 2; off >= 1; off >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], off, 64);
   if constexpr (LANES > 64) {
     constexpr int kWaves = LANES / 64;
-    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-    __syncthreads();
-    const float* mine = scratch + threadIdx.x / LANES * kWaves;
-    v = mine[0];
+    if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-    for (int i = 1; i < kWaves; ++i) v += mine[i];
+      for (int i = 0; i < N; ++i) scratch[(threadIdx.x >> 6) * N + i] = v[i];
+    }
+    __syncthreads();
+    const float* mine = scratch + threadIdx.x / LANES * kWaves * N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = mine[i];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) v[i] += mine[w * N + i];
+    }
   }
-  return v;
+}
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v, float* scratch) {
+  float a[1] = {v};
+  row_sums<LANES>(a, scratch);
+  return a[0];
 }
 
 template <int LANES, bool VEC>
@@ -120,16 +159,30 @@ __global__ __launch_bounds__(threads_of(LANES)) void resnorm_fwd_kernel(ResNormA
   S::read(a.post_b, D, lane, pb);
   S::read(a.pre_w, D, lane, qw);
   S::read(a.pre_b, D, lane, qb);
+  Raw<TX, LANES, VEC> raw_x;
+  Raw<TZ, LANES, VEC> raw_z, raw_g;
+  float open_next = 1.0f;
+  const long long step = (long long)gridDim.x * kRows;
+  // a row group behind the last row computes that one again and writes nothing
+  auto fetch = [&](long long r) {
+    r = r < a.N ? r : a.N - 1;
+    raw_z.read(reinterpret_cast<const TZ*>(a.z) + r * D, D, lane);
+    raw_x.read(reinterpret_cast<const TX*>(a.x) + r * D, D, lane);
+    if (a.gate_mode == 2) raw_g.read(reinterpret_cast<const TZ*>(a.gate) + r * D, D, lane);
+    if (a.gate_mode == 1) open_next = read1(reinterpret_cast<const TZ*>(a.gate) + r);
+  };
+  fetch((long long)blockIdx.x * kRows + group);
   int turn = 0;
-  for (long long r0 = (long long)blockIdx.x * kRows; r0 < a.N; r0 += (long long)gridDim.x * kRows, turn ^= 1) {
+  for (long long r0 = (long long)blockIdx.x * kRows; r0 < a.N; r0 += step, turn ^= 1) {
     const long long row = r0 + group;
-    const bool on = row < a.N;  // a row group behind the last row computes that one again and writes nothing
-    const long long at = (on ? row : a.N - 1) * D;
+    const bool on = row < a.N;
+    const long long at = row * D;
     float x[8], z[8], g[8];
-    S::read(reinterpret_cast<const TZ*>(a.z) + at, D, lane, z);
-    S::read(reinterpret_cast<const TX*>(a.x) + at, D, lane, x);
-    if (a.gate_mode == 2) S::read(reinterpret_cast<const TZ*>(a.gate) + at, D, lane, g);
-    const float open_row = a.gate_mode == 1 ? sigmoid(read1(reinterpret_cast<const TZ*>(a.gate) + (on ? row : a.N - 1))) : 1.0f;
+    raw_z.get(z);
+    raw_x.get(x);
+    if (a.gate_mode == 2) raw_g.get(g);
+    const float open_row = a.gate_mode == 1 ? sigmoid(open_next) : 1.0f;
+    if (r0 + step < a.N) fetch(row + step);
     float mean, rstd, mean_y, rstd_y;
     moments<LANES, VEC>(z, D, inv_d, a.eps, lane, scratch[turn], mean, rstd);
 #pragma unroll
@@ -153,7 +206,7 @@ template <typename TX, typename TZ, int LANES, bool VEC>
 __global__ __launch_bounds__(threads_of(LANES)) void resnorm_bwd_kernel(ResNormArgs a) {
   using S = Share<LANES, VEC>;
   constexpr int kRows = threads_of(LANES) / LANES;
-  __shared__ float scratch[2][5 * kScratch];
+  __shared__ float scratch[2][2 * kScratch];
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, D = a.D;
   const float inv_d = 1.0f / (float)D;
   float sc[8], pw[8], pb[8], qw[8];
@@ -166,22 +219,40 @@ __global__ __launch_bounds__(threads_of(LANES)) void resnorm_bwd_kernel(ResNormA
   for (int i = 0; i < 5; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum[i][e] = 0.f;
+  Raw<TX, LANES, VEC> raw_x, raw_dy;
+  Raw<TZ, LANES, VEC> raw_z, raw_g, raw_dh;
+  float4 st_next;
+  float open_next = 0.f;
+  const long long step = (long long)gridDim.x * kRows;
+  auto fetch = [&](long long r) {
+    const bool on = r < a.N;
+    r = on ? r : a.N - 1;
+    raw_z.read(reinterpret_cast<const TZ*>(a.z) + r * D, D, lane);
+    raw_x.read(reinterpret_cast<const TX*>(a.x) + r * D, D, lane);
+    if (a.gate_mode == 2) raw_g.read(reinterpret_cast<const TZ*>(a.gate) + r * D, D, lane);
+    if (a.gate_mode == 1) open_next = read1(reinterpret_cast<const TZ*>(a.gate) + r);
+    raw_dy.zero();
+    raw_dh.zero();
+    if (a.dy && on) raw_dy.read(reinterpret_cast<const TX*>(a.dy) + r * D, D, lane);
+    if (a.dh && on) raw_dh.read(reinterpret_cast<const TZ*>(a.dh) + r * D, D, lane);
+    st_next = *reinterpret_cast<const float4*>(a.stats + 4 * r);
+  };
+  fetch((long long)blockIdx.x * kRows + group);
   int turn = 0;
-  for (long long r0 = (long long)blockIdx.x * kRows; r0 < a.N; r0 += (long long)gridDim.x * kRows, turn ^= 1) {
+  for (long long r0 = (long long)blockIdx.x * kRows; r0 < a.N; r0 += step, turn ^= 1) {
     const long long row = r0 + group;
     const bool on = row < a.N;
-    const long long at = (on ? row : a.N - 1) * D;
+    const long long at = row * D;
     float x[8], z[8], g[8], dy[8], dh[8];
-    S::read(reinterpret_cast<const TZ*>(a.z) + at, D, lane, z);
-    S::read(reinterpret_cast<const TX*>(a.x) + at, D, lane, x);
-    if (a.gate_mode == 2) S::read(reinterpret_cast<const TZ*>(a.gate) + at, D, lane, g);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) dy[e] = dh[e] = 0.f;
-    if (a.dy && on) S::read(reinterpret_cast<const TX*>(a.dy) + at, D, lane, dy);
-    if (a.dh && on) S::read(reinterpret_cast<const TZ*>(a.dh) + at, D, lane, dh);
-    const float4 st = *reinterpret_cast<const float4*>(a.stats + 4 * (on ? row : a.N - 1));
-    const float open_row = a.gate_mode == 1 ? sigmoid(read1(reinterpret_cast<const TZ*>(a.gate) + (on ? row : a.N - 1))) : 1.0f;
-    float s1 = 0.f, s2 = 0.f;
+    raw_z.get(z);
+    raw_x.get(x);
+    if (a.gate_mode == 2) raw_g.get(g);
+    raw_dy.get(dy);
+    raw_dh.get(dh);
+    const float4 st = st_next;
+    const float open_row = a.gate_mode == 1 ? sigmoid(open_next) : 1.0f;
+    if (r0 + step < a.N) fetch(row + step);
+    float s12[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const bool in = S::col(lane, e) < D;
@@ -192,12 +263,12 @@ __global__ __launch_bounds__(threads_of(LANES)) void resnorm_bwd_kernel(ResNormA
       sum[4][e] += dh[e];
       sum[3][e] = fmaf(dh[e], x[e], sum[3][e]);
       dh[e] *= qw[e];
-      s1 += dh[e];
-      s2 = fmaf(dh[e], x[e], s2);
+      s12[0] += dh[e];
+      s12[1] = fmaf(dh[e], x[e], s12[1]);
     }
-    s1 = row_sum<LANES>(s1, scratch[turn]) * inv_d;
-    s2 = row_sum<LANES>(s2, scratch[turn] + kScratch) * inv_d;
-    float t1 = 0.f, t2 = 0.f, tg = 0.f;
+    row_sums<LANES>(s12, scratch[turn]);
+    const float s1 = s12[0] * inv_d, s2 = s12[1] * inv_d;
+    float t12[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float d = on ? fmaf(st.w, dh[e] - s1 - x[e] * s2, dy[e]) : 0.f;  // whole gradient of y
@@ -209,18 +280,17 @@ __global__ __launch_bounds__(threads_of(LANES)) void resnorm_bwd_kernel(ResNormA
       sum[2][e] += dn;
       sum[1][e] = fmaf(dn, z[e], sum[1][e]);
       g[e] = dn * n * (1.0f - g[e]);           // gradient of the gate's logit
-      tg += g[e];
+      t12[2] += g[e];
       x[e] = dn * pw[e];
-      t1 += x[e];
-      t2 = fmaf(x[e], z[e], t2);
+      t12[0] += x[e];
+      t12[1] = fmaf(x[e], z[e], t12[1]);
     }
-    t1 = row_sum<LANES>(t1, scratch[turn] + 2 * kScratch) * inv_d;
-    t2 = row_sum<LANES>(t2, scratch[turn] + 3 * kScratch) * inv_d;
-    if (a.gate_mode == 1) tg = row_sum<LANES>(tg, scratch[turn] + 4 * kScratch);
+    row_sums<LANES>(t12, scratch[turn] + kScratch);
+    const float t1 = t12[0] * inv_d, t2 = t12[1] * inv_d;
     if (!on) continue;
     S::write(reinterpret_cast<TX*>(a.dx) + at, D, lane, dy);
     if (a.gate_mode == 2) S::write(reinterpret_cast<TZ*>(a.dgate) + at, D, lane, g);
-    if (a.gate_mode == 1 && lane == 0) write1(reinterpret_cast<TZ*>(a.dgate) + row, tg);
+    if (a.gate_mode == 1 && lane == 0) write1(reinterpret_cast<TZ*>(a.dgate) + row, t12[2]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = st.y * (x[e] - t1 - z[e] * t2);
     S::write(reinterpret_cast<TZ*>(a.dz) + at, D, lane, x);

@@ -104,9 +104,9 @@ void strides(long long (&s)[3], const Tensor& t) {
 void plan(int64_t samples, int64_t groups, int64_t steps, int64_t resident, int& splits, int& chunk) {
   const int64_t n = samples * groups;
   splits = 1;
-  chunk = static_cast<int>(std::max<int64_t>(1, n / resident));
+  chunk = static_cast<int>(up(n, resident));
   if (chunk > 1) return;
-  const auto cost = [&](int64_t s) { return static_cast<double>(up(n * s, resident) * (up(steps, s) + 2)) + (s > 1 ? 2.0 + 0.05 * static_cast<double>(s) : 0.0); };
+  const auto cost = [&](int64_t s) { return static_cast<double>(up(n * s, resident) * (up(steps, s) + 2)) + (s > 1 ? 2.0 + 0.5 * static_cast<double>(s) : 0.0); };
   double best = cost(1);
   for (int64_t s = 2; s <= std::min<int64_t>(steps / 2, 128); ++s)
     if (cost(s) < 0.95 * best) best = cost(s), splits = static_cast<int>(s);
@@ -255,7 +255,8 @@ struct Attention : torch::autograd::Function<Attention> {
     const int64_t n_kv = a.k_splits > 1 ? a.k_splits * s.b * s.kv * s.lk * (s.maps * s.d + s.dv) : 0;
     const int64_t n_hist = want_table ? per_head * hm * slots : 0, n_mid = want_table ? a.shares * hm * slots : 0;
     const auto f = q.options().dtype(at::kFloat);
-    const Tensor work = at::empty({n_delta + n_dq + n_kv + n_hist + n_mid}, f);
+    const int64_t n_dlam = want_lam ? per_head * s.h * 4 : 0;
+    const Tensor work = at::empty({n_delta + n_dq + n_kv + n_hist + n_mid + n_dlam}, f);
     a.delta = f32(work);
     if (n_dq) a.dq_part = a.delta + n_delta;
     if (n_kv) a.kv_part = a.delta + n_delta + n_dq;
@@ -269,6 +270,7 @@ struct Attention : torch::autograd::Function<Attention> {
     if (want_lam) {
       dlam = at::empty({s.h}, f);
       a.dlam = f32(dlam);
+      a.dlam_part = a.delta + n_delta + n_dq + n_kv + n_hist + n_mid;
     }
     launch(lib.attn_bwd, a, "atri_enc_attn_bwd", q);
     if (want_table) dtable = dtable.to(static_cast<at::ScalarType>(ints[6]));
@@ -377,7 +379,8 @@ struct GatedNormResidual : torch::autograd::Function<GatedNormResidual> {
     launch(lib.norm_bwd, a, "atri_resnorm_bwd", x);
     const auto types = ctx->saved_data["types"].toIntVector();
     variable_list all = {dx, dz};
-    for (int i = 0; i < 5; ++i) all.push_back(dparams.select(0, i).to(static_cast<at::ScalarType>(types[i])));
+    const auto each = dparams.unbind(0);
+    for (int i = 0; i < 5; ++i) all.push_back(each[i].to(static_cast<at::ScalarType>(types[i])));
     all.push_back(dgate);
     all.emplace_back();
     return all;
