@@ -81,6 +81,8 @@ def train(
     train_steps_per_round: Annotated[int | None, typer.Option(help="Split layout: learner steps between two polls for shipments and weight requests.")] = None,
     gpus: Annotated[int, typer.Option(help="Number of GPUs of this node to use: one process per GPU, started by this command.")] = 1,
     dtype: Annotated[str | None, typer.Option(help="Leaf-evaluation precision of the GPU engine: fp32 (reference precision) or bf16 (fast).")] = None,
+    attention: Annotated[str | None, typer.Option(help="Encoder attention: softmax, relative (learned board position bias) or differential.")] = None,
+    encoder_norm: Annotated[str | None, typer.Option(help="Encoder residual blocks: pre (norm) or sandwich (norms around, gate and residual scale).")] = None,
     dist_backend: Annotated[str, typer.Option(help="Process-group backend: auto, nccl (= RCCL) or gloo (CPU rehearsals).")] = "auto",
 ) -> None:
     """Run the headless training pipeline.  `--gpus N` starts N ranks (one per GPU) from this one command."""
@@ -122,6 +124,14 @@ def train(
         if dtype not in ("fp32", "bf16"):
             raise typer.BadParameter("--dtype must be 'fp32' or 'bf16'")
         sys_cfg.INFERENCE_DTYPE = dtype  # type: ignore[assignment]
+    if attention is not None or encoder_norm is not None:
+        from .config import ModelConfig
+
+        chosen = {k: v for k, v in (("TRANSFORMER_ATTENTION", attention), ("TRANSFORMER_NORM", encoder_norm)) if v is not None}
+        try:
+            model_cfg = ModelConfig(**{**model_cfg.model_dump(), **chosen})
+        except ValueError as exc:
+            raise typer.BadParameter(f"--attention / --encoder-norm: {exc}") from exc
     if dist_backend not in ("auto", "nccl", "gloo"):
         raise typer.BadParameter("--dist-backend must be auto, nccl or gloo")
     sys_cfg.DIST_BACKEND = dist_backend  # type: ignore[assignment]

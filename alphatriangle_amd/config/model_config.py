@@ -30,6 +30,9 @@ class ModelConfig(BaseModel):
     TRANSFORMER_HEADS: int = Field(default=4, gt=0)
     TRANSFORMER_LAYERS: int = Field(default=2, ge=0)
     TRANSFORMER_FC_DIM: int = Field(default=256, gt=0)
+    # encoder variants (models/encoder.py); the defaults are the reference's layer
+    TRANSFORMER_ATTENTION: Literal["softmax", "relative", "differential"] = Field(default="softmax")
+    TRANSFORMER_NORM: Literal["pre", "sandwich"] = Field(default="pre")
 
     FC_DIMS_SHARED: list[int] = Field(default=[128])
     POLICY_HEAD_DIMS: list[int] = Field(default=[128])
@@ -69,6 +72,14 @@ class ModelConfig(BaseModel):
                     )
                 if self.TRANSFORMER_FC_DIM <= 0:
                     raise ValueError("TRANSFORMER_FC_DIM must be positive when TRANSFORMER_LAYERS > 0.")
+                head = self.TRANSFORMER_DIM // self.TRANSFORMER_HEADS
+                if self.TRANSFORMER_ATTENTION == "relative" and (head % 8 != 0 or head > 128):
+                    raise ValueError(f"relative attention needs heads of a multiple of 8 up to 128 values, got {head}.")
+                if self.TRANSFORMER_ATTENTION == "differential" and (head % 8 != 0 or head > 64 or self.TRANSFORMER_HEADS % 2 != 0):
+                    raise ValueError(
+                        f"differential attention needs an even number of heads of a multiple of 8 up to 64 values, "
+                        f"got {self.TRANSFORMER_HEADS} of {head}."
+                    )
         return self
 
     @model_validator(mode="after")

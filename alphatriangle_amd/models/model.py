@@ -892,7 +892,7 @@ class AlphaTriangleNet(nn.Module):
         self.res_body = nn.Sequential(*res)
         self.cnn_output_channels = channels
 
-        self.transformer_body: nn.TransformerEncoder | None = None
+        self.transformer_body: nn.Module | None = None
         self.pos_encoder: PositionalEncoding | None = None
         self.input_proj: nn.Module = nn.Identity()
         self.transformer_output_size = 0
@@ -909,7 +909,7 @@ class AlphaTriangleNet(nn.Module):
             if channels != d:
                 self.input_proj = GemmConv2d(channels, d, kernel_size=1)
             self.pos_encoder = PositionalEncoding(d, dropout=0.1)
-            layer = EncoderLayer(
+            kind = dict(
                 d_model=d,
                 nhead=mc.TRANSFORMER_HEADS,
                 dim_feedforward=mc.TRANSFORMER_FC_DIM,
@@ -917,9 +917,14 @@ class AlphaTriangleNet(nn.Module):
                 batch_first=False,
                 norm_first=True,
             )
-            self.transformer_body = nn.TransformerEncoder(
-                layer, num_layers=mc.TRANSFORMER_LAYERS, norm=FastLayerNorm(d), enable_nested_tensor=False
-            )
+            if mc.TRANSFORMER_ATTENTION == "softmax" and mc.TRANSFORMER_NORM == "pre":
+                self.transformer_body = nn.TransformerEncoder(
+                    EncoderLayer(**kind), num_layers=mc.TRANSFORMER_LAYERS, norm=FastLayerNorm(d), enable_nested_tensor=False
+                )
+            else:
+                from .encoder import BoardEncoder
+
+                self.transformer_body = BoardEncoder(self.body_hw, mc.TRANSFORMER_LAYERS, mc.TRANSFORMER_ATTENTION, mc.TRANSFORMER_NORM == "sandwich", **kind)
             self.transformer_output_size = self.body_hw[0] * self.body_hw[1] * d
             feat = self.transformer_output_size
         else:
@@ -1018,7 +1023,7 @@ class AlphaTriangleNet(nn.Module):
                 tokens = self.pos_encoder(x.flatten(2).permute(2, 1, 0).contiguous())  # [H*W, B, D]
             body = self.transformer_body
             norm = body.norm
-            if fused and isinstance(norm, FastLayerNorm) and norm.fast_ok(tokens):
+            if fused and isinstance(body, nn.TransformerEncoder) and isinstance(norm, FastLayerNorm) and norm.fast_ok(tokens):
                 for layer in body.layers:  # the stack written out, so that the final LayerNorm can write [B, H*W*D] itself
                     tokens = layer(tokens)
                 return _LayerNormFn.apply(tokens, norm.weight, norm.bias, norm.eps, True)

@@ -76,6 +76,8 @@ def engine_supports(mc: ModelConfig, ec: EnvConfig, dtype: str = "bf16") -> tupl
     """Whether the HIP engine implements this architecture at this precision (else callers use the PyTorch module)."""
     if dtype not in ("bf16", "fp32"):
         return False, f"no {dtype} kernels"
+    if mc.USE_TRANSFORMER and mc.TRANSFORMER_LAYERS > 0 and (mc.TRANSFORMER_ATTENTION != "softmax" or mc.TRANSFORMER_NORM != "pre"):
+        return False, "the engine's encoder kernels implement softmax attention and pre-norm residuals"
     if dtype == "fp32":
         # The fp32-grade kernels (csrc/hip/split_*.hip) are written for the reference's default architecture family:
         # 3x3 stem 1 -> 32 -> 64 -> 128, 128-channel residual blocks, d_model 128 / 4 heads, 128-wide dense tail.
