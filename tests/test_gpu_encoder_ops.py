@@ -335,3 +335,156 @@ def test_once_differentiable():
     g = torch.autograd.grad(_call(inp, p, None, 0).square().sum(), q, create_graph=True)[0]
     with pytest.raises(RuntimeError, match="once"):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("maps,kind,lq,lk,h,kv,d,b", [
+    (1, (8, 15), 120, 120, 4, 4, 32, 301),  # two key tiles, bias and sums in registers
+    (2, (8, 15), 120, 120, 2, 2, 32, 601),
+    (1, (10, 16), 160, 160, 4, 4, 24, 203),  # three of the four tiles of the widest register form
+    (1, (12, 21), 252, 252, 2, 2, 32, 303),  # a last tile of 60 keys
+    (1, (8, 15), 120, 120, 4, 2, 32, 301),  # shared heads: register form for the queries, general form for the keys
+    (1, (3, 5), 15, 15, 4, 4, 32, 301),  # one tile
+    (1, (8, 15), 120, 120, 4, 4, 64, 301),  # wide heads: general form on a board
+    (1, 40, 33, 130, 4, 1, 32, 301),  # sequences
+    (2, 40, 70, 65, 2, 1, 64, 601),
+])
+def test_workgroups_walk_several_samples(dtype, maps, kind, lq, lk, h, kv, d, b):
+    """More samples than the card holds workgroups, with masks of every kind; masked rows hold NaN and infinities, and values of
+    one sample must not reach the next."""
+    p = _plan(kind)
+    inp = _inputs(dtype, maps, b, lq, lk, h, kv, d, p, std=0.7)
+    g = torch.Generator().manual_seed(3)
+    mask = torch.rand(b, lk, generator=g) < torch.rand(b, 1, generator=g)
+    mask[1::7] = False  # no key at all
+    mask[2::7] = True
+    mask[3::7, lk // 2 :] = False
+    mask = mask.cuda()
+    clean_out, clean = _compare(inp, p, mask)
+    assert bool((clean_out[1::7] == 0).all())
+    bad = dict(inp)
+    for n, x in (("k", math.nan), ("v", math.inf)):
+        bad[n] = inp[n].clone()
+        bad[n][~mask] = x
+    names = [n for n in ("q", "k", "v", "table", "lam") if inp[n] is not None]
+    t = {**bad, **{n: bad[n].detach().clone().requires_grad_(True) for n in names}}
+    out = _call(t, p, mask, 0)
+    grads = torch.autograd.grad(out, [t[n] for n in names], inp["dout"])
+    assert torch.equal(out, clean_out)
+    for n, x in zip(names, grads):
+        assert torch.equal(x, clean[n]), n
+
+
+def test_many_positions_and_many_sums():
+    """4095 relative positions under hundreds of workgroups: the sums by position are joined in two steps."""
+    p = _plan(2047)
+    _compare(_inputs(torch.bfloat16, 1, 3, 1500, 2100, 6, 2, 32, p), p)
+    board = _plan((20, 30))
+    _compare(_inputs(torch.float32, 1, 24, 600, 600, 4, 4, 16, board), board)
+
+
+def test_offsets_beyond_32_bits():
+    """Rows 2^25 elements apart: element offsets pass 2^31 and byte offsets 2^32."""
+    p = _plan(32)
+    n, step = 70, 1 << 25
+    for dtype in BOTH:
+        store = torch.empty(n * step + (1 << 24), dtype=dtype, device="cuda")
+        view = {}
+        base = _inputs(dtype, 1, 2, n, n, 1, 1, 32, p)
+        for i, name in enumerate(("q", "k", "v", "dout")):
+            x = store[i << 20 :].as_strided((2, n, 1, 32), (1 << 22, step, 32, 1), store.storage_offset() + (i << 20))
+            x.copy_(base[name])
+            view[name] = x
+        want, grads = _compare(base, p)
+        t = {k: view[k].detach().requires_grad_(True) for k in ("q", "k", "v")}
+        out = _call({**base, **t}, p, None, 0)
+        got = torch.autograd.grad(out, list(t.values()), view["dout"])
+        assert torch.equal(out, want)
+        for k, x in zip(t, got):
+            assert torch.equal(x, grads[k]), k
+        del store, view, t, out, got, x
+        torch.cuda.empty_cache()
+
+
+def test_two_calls_at_once():
+    """Calls on two streams share no scratch memory."""
+    p, w = _plan((8, 15)), _plan(64)
+    a = _inputs(torch.float32, 1, 64, 120, 120, 4, 4, 32, p, seed=1)
+    c = _inputs(torch.bfloat16, 2, 2, 150, 1900, 4, 2, 64, w, seed=2)
+
+    def step(inp, plan):  # noqa: ANN001, ANN202
+        names = [n for n in ("q", "k", "v", "table", "lam") if inp[n] is not None]
+        t = {**inp, **{n: inp[n].detach().requires_grad_(True) for n in names}}
+        out = _call(t, plan, None, 0)
+        return (out.detach(), *torch.autograd.grad(out, [t[n] for n in names], inp["dout"]))
+
+    want_a, want_c = step(a, p), step(c, w)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    got_a, got_c = [], []
+    for _ in range(4):
+        with torch.cuda.stream(s1):
+            got_a.append(step(a, p))
+        with torch.cuda.stream(s2):
+            got_c.append(step(c, w))
+    torch.cuda.synchronize()
+    for got, want in ((got_a, want_a), (got_c, want_c)):
+        for r in got:
+            for x, y in zip(r, want):
+                assert torch.equal(x, y)
+
+
+def test_two_graphs_of_two_maps():
+    """Two captured training calls of different shapes, replayed in turn beside eager ones, on new inputs."""
+    p = _plan((8, 15))
+    shapes = ((3, 120, 4, 4), (40, 120, 2, 2))
+    graphs = []
+    for b, l, h, kv in shapes:
+        static = {n: (x.clone() if x is not None else None) for n, x in _inputs(torch.bfloat16, 2, b, l, l, h, kv, 32, p).items()}
+        names = ("q", "k", "v", "table", "lam")
+
+        def step(static=static, names=names):  # noqa: ANN202
+            t = {**static, **{n: static[n].detach().requires_grad_(True) for n in names}}
+            out = _call(t, p, None, 0)
+            return (out.detach(), *torch.autograd.grad(out, [t[n] for n in names], static["dout"]))
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = step()
+        graphs.append((graph, held, static, step))
+    for seed in range(3):
+        for (b, l, h, kv), (graph, _, static, _) in zip(shapes, graphs):
+            for n, x in _inputs(torch.bfloat16, 2, b, l, l, h, kv, 32, p, seed=seed).items():
+                if x is not None:
+                    static[n].copy_(x)
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, held, _, step in graphs:
+            for x, y in zip([x.clone() for x in held], step()):
+                assert torch.equal(x, y)
+
+
+def test_inputs_changed_in_place_are_noticed():
+    p = _plan(16)
+    inp = _inputs(torch.float32, 1, 1, 20, 20, 1, 1, 32, p)
+    for name in ("k", "table"):
+        t = {**inp, name: inp[name].clone(), "q": inp["q"].clone().requires_grad_(True)}
+        out = _call(t, p, None, 0)
+        t[name].mul_(2)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
+
+
+def test_half_of_a_batch_equals_the_whole():
+    """Results do not depend on how many samples share a launch (no sum runs over samples except the table's)."""
+    p = _plan((8, 15))
+    for dtype in BOTH:
+        inp = _inputs(dtype, 1, 400, 120, 120, 4, 4, 32, p)
+        whole = _call(inp, p, None, 0)
+        part = {n: (x[390:] if n in ("q", "k", "v") else x) for n, x in inp.items()}
+        assert torch.equal(_call(part, p, None, 0), whole[390:])
