@@ -117,7 +117,7 @@ __device__ __forceinline__ int query_origin(const EncAttnArgs& a, int b) {
   const int o = a.qoff ? a.qoff[b] : a.q0;
   return o < -(1 << 29) ? -(1 << 29) : o > (1 << 29) ? (1 << 29) : o;  // differences stay within 32 bits
 }
-__device__ __forceinline__ int clamp_slot(int d, int R2) { return d < 0 ? 0 : d > R2 ? R2 : d; }
+__device__ __forceinline__ int clamp_slot(int d, int R2) { return max(0, min(d, R2)); }
 
 // exp2 of (x - top) sl2, x and top in units of 1 / scale, sl2 = scale log2 e.  One fused multiply-add: base = top sl2 is rounded
 // once, and every value of a row carries the same base, so its rounding cancels against the sum.  Far rows (|base| of a

@@ -69,7 +69,8 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncQu
   float* ds_lds = bias_lds + ((M * slots + 3) & ~3);
   float* sum_lds = ds_lds + 4 * 16 * kDsPitch;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, q4 = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, q4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // what follows from it (owned rows, clamped sides) stays in scalar registers
   const int nqt = (a.Lq + 64 * QS - 1) / (64 * QS);
   const int group_id = xcd_order(blockIdx.x, gridDim.x);
   int id = group_id;
@@ -442,7 +443,8 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, sizeof(T) == 2, kEncKe
   int* far_lds = reinterpret_cast<int*>(delta_lds + M * kTile);  // one flag per map (and padding)
   float* bias_lds = reinterpret_cast<float*>(far_lds + 4);
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, q4 = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, q4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // what follows from it (owned rows, clamped sides) stays in scalar registers
   const int nkt = (a.Lk + 64 * KS - 1) / (64 * KS);
   int id = xcd_order(blockIdx.x, gridDim.x);
   const int kt_ = id % nkt;

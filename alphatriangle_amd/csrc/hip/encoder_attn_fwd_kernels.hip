@@ -26,7 +26,8 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncFo
   int* pos_lds = reinterpret_cast<int*>(v_lds + kTile * PV);
   float* bias_lds = reinterpret_cast<float*>(pos_lds + (NT ? NT : 1) * kTile);
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, q4 = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, q4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // what follows from it (owned rows, clamped sides) stays in scalar registers
   const int nqt = (a.Lq + 64 * QS - 1) / (64 * QS);
   int id = xcd_order(blockIdx.x, gridDim.x);
   const int qt = id % nqt;
