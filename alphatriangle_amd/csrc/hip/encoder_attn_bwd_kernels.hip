@@ -223,83 +223,99 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncQu
           const int qa = q_first + s * 16 + origin;
           side[s] = BIAS && NT == 0 ? clamped_side(a, t0, t0 + kTile - 1, qa, qa + 15) : 0;
         }
+        // PLAIN: no far row and no masked key, one basic block
+        auto scores = [&](auto plain_) {
+          constexpr bool PLAIN = decltype(plain_)::value;
 #pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) {
+          for (int kb = 0; kb < NKB; ++kb) {
+            // where the scores start
 #pragma unroll
-          for (int u = 0; u < O::kSub; ++u) {
-            const int kt = kb * O::kSub + u;
-            float4v dp[QS];
-#pragma unroll
-            for (int s = 0; s < QS; ++s) dp[s] = float4v{-delta[0][s], -delta[0][s], -delta[0][s], -delta[0][s]};  // dP - delta of the first map
-#pragma unroll
-            for (int c = 0; c < VC; ++c) {
-              const Frag vf = O::row_frag(v_lds, PV, kt * 16 + l15, c, q4);
-#pragma unroll
-              for (int s = 0; s < QS; ++s) dp[s] = O::mma(vf, dof[s][c], dp[s]);
-            }
-            int4 p4 = make_int4(0, 0, 0, 0);
-            if constexpr (BIAS && NT == 0) p4 = *reinterpret_cast<const int4*>(pos_lds + kt * 16 + q4 * 4);
-            const int pj[4] = {p4.x, p4.y, p4.z, p4.w};
-#pragma unroll
-            for (int m = 0; m < M; ++m) {
-              float4v x[QS];
+            for (int m = 0; m < M; ++m)
 #pragma unroll
               for (int s = 0; s < QS; ++s) {
+                float4v* x = &ds[m][s][kb * O::kSub];
                 if constexpr (NT > 0) {
-                  x[s] = bias_reg[m][s][kt0 + kt];
+#pragma unroll
+                  for (int u = 0; u < O::kSub; ++u) x[u] = bias_reg[m][s][kt0 + kb * O::kSub + u];
                 } else if constexpr (BIAS) {
                   const float* bias = bias_lds + m * slots;
                   if (side[s] != 0) {
                     const float c = bias[side[s] > 0 ? R2 : 0];
-                    x[s] = float4v{c, c, c, c};
+#pragma unroll
+                    for (int u = 0; u < O::kSub; ++u) x[u] = float4v{c, c, c, c};
                   } else {
                     const int off = a.R - token_q[s] - origin;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x[s][j] = bias[clamp_slot(pj[j] + off, R2)];
+                    for (int u = 0; u < O::kSub; ++u) {
+                      const int4 p4 = *reinterpret_cast<const int4*>(pos_lds + (kb * O::kSub + u) * 16 + q4 * 4);
+                      const int pj[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+                      for (int j = 0; j < 4; ++j) x[u][j] = bias[clamp_slot(pj[j] + off, R2)];
+                    }
                   }
                 } else {
-                  x[s] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                  for (int u = 0; u < O::kSub; ++u) x[u] = float4v{0.f, 0.f, 0.f, 0.f};
                 }
               }
 #pragma unroll
-              for (int c = 0; c < DC; ++c) {
-                const Frag kf = O::row_frag(k_lds + m * kTile * PK, PK, kt * 16 + l15, c, q4);
+            for (int u = 0; u < O::kSub; ++u) {
+              const int kt = kb * O::kSub + u;
+              float4v dp[QS];
 #pragma unroll
-                for (int s = 0; s < QS; ++s) x[s] = O::mma(kf, qf[m][s][c], x[s]);
+              for (int s = 0; s < QS; ++s) dp[s] = float4v{-delta[0][s], -delta[0][s], -delta[0][s], -delta[0][s]};  // dP - delta of the first map
+#pragma unroll
+              for (int c = 0; c < VC; ++c) {
+                const Frag vf = O::row_frag(v_lds, PV, kt * 16 + l15, c, q4);
+#pragma unroll
+                for (int s = 0; s < QS; ++s) dp[s] = O::mma(vf, dof[s][c], dp[s]);
               }
 #pragma unroll
-              for (int s = 0; s < QS; ++s) {
-                const float shift = m == 0 ? 0.f : delta[0][s] - delta[m][s];
-                if (far) {
+              for (int m = 0; m < M; ++m) {
 #pragma unroll
-                  for (int j = 0; j < 4; ++j) x[s][j] = Exponent::far_(x[s][j], top[m][s], sl2);
-                } else {
+                for (int c = 0; c < DC; ++c) {
+                  const Frag kf = O::row_frag(k_lds + m * kTile * PK, PK, kt * 16 + l15, c, q4);
 #pragma unroll
-                  for (int j = 0; j < 4; ++j) x[s][j] = Exponent::near_(x[s][j], base[m][s], sl2);
+                  for (int s = 0; s < QS; ++s) ds[m][s][kt] = O::mma(kf, qf[m][s][c], ds[m][s][kt]);
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) ds[m][s][kt][j] = x[s][j] * (m == 0 ? dp[s][j] : dp[s][j] + shift);
-                if (word != ~0ULL) {
-                  const unsigned bits = (unsigned)(word >> (kt * 16 + q4 * 4));
+                for (int s = 0; s < QS; ++s) {
+                  const float shift = m == 0 ? 0.f : delta[0][s] - delta[m][s];
+                  float4v x = ds[m][s][kt];
+                  if (!PLAIN && far) {
 #pragma unroll
-                  for (int j = 0; j < 4; ++j) ds[m][s][kt][j] = (bits >> j) & 1 ? ds[m][s][kt][j] : 0.f;
+                    for (int j = 0; j < 4; ++j) x[j] = Exponent::far_(x[j], top[m][s], sl2);
+                  } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[j] = Exponent::near_(x[j], base[m][s], sl2);
+                  }
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) x[j] *= m == 0 ? dp[s][j] : dp[s][j] + shift;
+                  if (!PLAIN && word != ~0ULL) {
+                    const unsigned bits = (unsigned)(word >> (kt * 16 + q4 * 4));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[j] = (bits >> j) & 1 ? x[j] : 0.f;
+                  }
+                  ds[m][s][kt] = x;
                 }
               }
             }
-          }
 #pragma unroll
-          for (int m = 0; m < M; ++m) {
-            Frag sf[QS];
+            for (int m = 0; m < M; ++m) {
+              Frag sf[QS];
 #pragma unroll
-            for (int s = 0; s < QS; ++s) sf[s] = O::acc_frag(&ds[m][s][kb * O::kSub]);
+              for (int s = 0; s < QS; ++s) sf[s] = O::acc_frag(&ds[m][s][kb * O::kSub]);
 #pragma unroll
-            for (int n = 0; n < ND; ++n) {
-              const Frag kf = O::tr_frag(k_lds + m * kTile * PK, PK, kb, n, l15, q4);
+              for (int n = 0; n < ND; ++n) {
+                const Frag kf = O::tr_frag(k_lds + m * kTile * PK, PK, kb, n, l15, q4);
 #pragma unroll
-              for (int s = 0; s < QS; ++s) dq[m][s][n] = O::mma(kf, sf[s], dq[m][s][n]);
+                for (int s = 0; s < QS; ++s) dq[m][s][n] = O::mma(kf, sf[s], dq[m][s][n]);
+              }
             }
           }
-        }
+        };
+        if (far || word != ~0ULL) scores(std::false_type{});
+        else scores(std::true_type{});
         if constexpr (NT > 0) {
 #pragma unroll
           for (int m = 0; m < M; ++m)

@@ -130,87 +130,111 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncFo
       if (walk.sample < b_last) fetch(walk);  // the next tile's loads (this sample's or the next one's) run under this tile's products
       if (!busy) return;
 
+      // Few and wide basic blocks per map: the start of the scores, all products, one branch each for masked keys, far rows and
+      // new maxima.
       float4v st[M][QS][4];
 #pragma unroll
       for (int m = 0; m < M; ++m) {
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
+        for (int s = 0; s < QS; ++s) {
+          float4v* x = st[m][s];
           if constexpr (NT > 0) {
 #pragma unroll
-            for (int s = 0; s < QS; ++s) st[m][s][kt] = bias_reg[m][s][kt0 + kt];
+            for (int kt = 0; kt < 4; ++kt) x[kt] = bias_reg[m][s][kt0 + kt];
           } else if constexpr (BIAS) {
             const float* bias = bias_lds + m * (R2 + 1);
-            const int4 p = *reinterpret_cast<const int4*>(pos_lds + kt * 16 + q4 * 4);
-            const int pj[4] = {p.x, p.y, p.z, p.w};
+            const int qa = q_first + s * 16 + origin;
+            const int side = clamped_side(a, t0, t0 + kTile - 1, qa, qa + 15);
+            if (side != 0) {
+              const float c = bias[side > 0 ? R2 : 0];
 #pragma unroll
-            for (int s = 0; s < QS; ++s) {
-              const int qa = q_first + s * 16 + origin;
-              const int side = clamped_side(a, t0, t0 + kTile - 1, qa, qa + 15);
-              if (side != 0) {
-                const float c = bias[side > 0 ? R2 : 0];
-                st[m][s][kt] = float4v{c, c, c, c};
-              } else {
-                const int off = a.R - token_q[s] - origin;
+              for (int kt = 0; kt < 4; ++kt) x[kt] = float4v{c, c, c, c};
+            } else {
+              const int off = a.R - token_q[s] - origin;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) st[m][s][kt][j] = bias[clamp_slot(pj[j] + off, R2)];
+              for (int kt = 0; kt < 4; ++kt) {
+                const int4 p = *reinterpret_cast<const int4*>(pos_lds + kt * 16 + q4 * 4);
+                const int pj[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[kt][j] = bias[clamp_slot(pj[j] + off, R2)];
               }
             }
           } else {
 #pragma unroll
-            for (int s = 0; s < QS; ++s) st[m][s][kt] = float4v{0.f, 0.f, 0.f, 0.f};
+            for (int kt = 0; kt < 4; ++kt) x[kt] = float4v{0.f, 0.f, 0.f, 0.f};
           }
+        }
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
           for (int c = 0; c < DC; ++c) {
             const Frag kf = O::row_frag(k_lds + m * kTile * PK, PK, kt * 16 + l15, c, q4);
 #pragma unroll
             for (int s = 0; s < QS; ++s) st[m][s][kt] = O::mma(kf, qf[m][s][c], st[m][s][kt]);
           }
+        if (word != ~0ULL) {
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt) {
+            const unsigned bits = (unsigned)(word >> (kt * 16 + q4 * 4));
+#pragma unroll
+            for (int s = 0; s < QS; ++s)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) st[m][s][kt][j] = (bits >> j) & 1 ? st[m][s][kt][j] : -INFINITY;
+          }
         }
+        float from[QS], fade[QS];
+        bool far = false;
 #pragma unroll
         for (int s = 0; s < QS; ++s) {
-          float4v* x = st[m][s];
-          if (word != ~0ULL) {
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt) {
-              const unsigned bits = (unsigned)(word >> (kt * 16 + q4 * 4));
-#pragma unroll
-              for (int j = 0; j < 4; ++j) x[kt][j] = (bits >> j) & 1 ? x[kt][j] : -INFINITY;
-            }
-          }
           float top = run_max[m][s];
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) top = fmaxf(top, x[kt][j]);
+            for (int j = 0; j < 4; ++j) top = fmaxf(top, st[m][s][kt][j]);
           top = quad_row_max(top);
-          const float from = top == -INFINITY ? 0.f : top;  // nothing seen yet: exp2(-inf - 0) = 0, never inf - inf
-          const float base = from * sl2;
-          float fade, sum = 0.f;
-          if (__any(Exponent::far(base))) {
-            fade = Exponent::far_(run_max[m][s], from, sl2);
+          from[s] = top == -INFINITY ? 0.f : top;  // nothing seen yet: exp2(-inf - 0) = 0, never inf - inf
+          fade[s] = run_max[m][s];
+          run_max[m][s] = top;
+          far |= Exponent::far(from[s] * sl2);
+        }
+        if (__any(far)) {
+#pragma unroll
+          for (int s = 0; s < QS; ++s) {
+            fade[s] = Exponent::far_(fade[s], from[s], sl2);
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) x[kt][j] = Exponent::far_(x[kt][j], from, sl2);
-          } else {
-            fade = __builtin_amdgcn_exp2f(run_max[m][s] * sl2 - base);
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) x[kt][j] = Exponent::near_(x[kt][j], base, sl2);
+              for (int j = 0; j < 4; ++j) st[m][s][kt][j] = Exponent::far_(st[m][s][kt][j], from[s], sl2);
           }
+        } else {
+#pragma unroll
+          for (int s = 0; s < QS; ++s) {
+            const float base = from[s] * sl2;
+            fade[s] = __builtin_amdgcn_exp2f(fade[s] * sl2 - base);
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) st[m][s][kt][j] = Exponent::near_(st[m][s][kt][j], base, sl2);
+          }
+        }
+        bool faded = false;
+#pragma unroll
+        for (int s = 0; s < QS; ++s) {
+          float sum = 0.f;
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum += x[kt][j];
-          run_max[m][s] = top;
-          run_sum[m][s] = fmaf(run_sum[m][s], fade, sum);
-          if (__any(fade != 1.0f)) {
+            for (int j = 0; j < 4; ++j) sum += st[m][s][kt][j];
+          run_sum[m][s] = fmaf(run_sum[m][s], fade[s], sum);
+          faded |= fade[s] != 1.0f;
+        }
+        if (__any(faded)) {
+#pragma unroll
+          for (int s = 0; s < QS; ++s)
 #pragma unroll
             for (int n = 0; n < NV; ++n)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) o[m][s][n][j] *= fade;
-          }
+              for (int j = 0; j < 4; ++j) o[m][s][n][j] *= fade[s];
         }
       }
 #pragma unroll
