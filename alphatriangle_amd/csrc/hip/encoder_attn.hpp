@@ -9,10 +9,13 @@
 // and its gradients.  The bias, divided by the scale, is where the matrix product's accumulator starts, so the scores cost
 // no vector instruction until the exponential, exp2(fma(x, scale log2 e, -base)): see Exponent.
 //
-// Matrix operands.  bf16 rows use v_mfma_f32_16x16x32_bf16 as they are; fp32 rows use v_mfma_f32_16x16x4_f32, true fp32
-// products: three bf16 passes over (hi, lo) splits carry 16 bits per operand, 30 times the rounding of an fp32 product.
+// Matrix operands.  bf16 rows use v_mfma_f32_16x16x32_bf16 as they are.  fp32 rows are cut into three bf16 values that
+// carry all 24 bits (Split), and a product is the six of the nine partial products that reach above 2^-25 of it: 96 cycles for
+// a depth of 32, where eight v_mfma_f32_16x16x4_f32 take 256 (two 2048-token sequences of eight 32-wide heads: forward 107 ->
+// 82 us, backward 349 -> 258 us).  Two parts and three products would carry 16 bits, 30 times the rounding of an fp32 product.
+// Where three parts do not fit, the fp32 instruction stays (see the dispatch).
 // A fragment covers kDims values of the contraction: lane (l15 = lane & 15, q4 = lane >> 4) holds, for row / column l15,
-//   bf16: values 8 q4 .. 8 q4 + 7 of 32;   fp32: values 4 q4 .. 4 q4 + 3 of 16 (four 4-deep instructions, one value each);
+//   bf16, Split: values 8 q4 .. 8 q4 + 7 of 32;   fp32: values 4 q4 .. 4 q4 + 3 of 16 (four 4-deep instructions, one value each);
 // an accumulator gives the lane C[4 q4 + j][l15], j = 0..3.  With the owned rows (queries in the forward and the dQ pass,
 // keys in the dK / dV pass) as COLUMNS of every product, softmax sums stay inside a lane plus one exchange over q4, and
 // an accumulator (two of them for bf16) is the B fragment of the product that follows, without any exchange: the
@@ -30,15 +33,25 @@ constexpr float kLog2E = 1.4426950408889634f;
 template <typename T>
 struct Ops;
 
+struct Split {};  // tag: fp32 rows as three bf16 parts
+
 template <>
 struct Ops<unsigned short> {
   using Frag = short8;
+  using Mem = unsigned short;        // element in memory
+  using Lds = unsigned short;        // element of a staged tile
+  static constexpr bool kBf16 = true;
   static constexpr int kDims = 32;   // contraction values per fragment
-  static constexpr int kVec = 8;     // elements per 16 bytes
+  static constexpr int kLane = 8;    // of them in a lane
+  static constexpr int kVec = 8;     // elements in memory per 16 bytes
   static constexpr int kSub = 2;     // 16-row accumulators per B fragment
+  static constexpr int kParts = 1;   // tiles of [kTile][pitch] that make a staged one
   static constexpr int row_pitch(int d) { return d + 8; }   // 16-lane b128 row reads: all 64 banks once
   static constexpr int tr_pitch(int d) { return d + 16; }   // transposing reads: eight 32-byte rows on distinct banks
-  static __device__ __forceinline__ Frag zero() { return Frag{}; }
+  static __device__ __forceinline__ Frag from_memory(const unsigned short* p) { return *reinterpret_cast<const short8*>(p); }
+  static __device__ __forceinline__ void stage(unsigned short* t, int pitch, int row, int col, const uint4& v) {
+    *reinterpret_cast<uint4*>(t + row * pitch + col) = v;
+  }
   static __device__ __forceinline__ Frag row_frag(const unsigned short* t, int pitch, int row, int c, int q4) {
     return *reinterpret_cast<const short8*>(t + row * pitch + c * 32 + q4 * 8);
   }
@@ -76,12 +89,20 @@ struct Ops<unsigned short> {
 template <>
 struct Ops<float> {
   using Frag = float4v;
+  using Mem = float;
+  using Lds = float;
+  static constexpr bool kBf16 = false;
   static constexpr int kDims = 16;
+  static constexpr int kLane = 4;
   static constexpr int kVec = 4;
   static constexpr int kSub = 1;
+  static constexpr int kParts = 1;
   static constexpr int row_pitch(int d) { return d + 4; }
   static constexpr int tr_pitch(int d) { return d + 4; }
-  static __device__ __forceinline__ Frag zero() { return Frag{}; }
+  static __device__ __forceinline__ Frag from_memory(const float* p) { return *reinterpret_cast<const float4v*>(p); }
+  static __device__ __forceinline__ void stage(float* t, int pitch, int row, int col, const uint4& v) {
+    *reinterpret_cast<uint4*>(t + row * pitch + col) = v;
+  }
   static __device__ __forceinline__ Frag row_frag(const float* t, int pitch, int row, int c, int q4) {
     return *reinterpret_cast<const float4v*>(t + row * pitch + c * 16 + q4 * 4);
   }
@@ -102,6 +123,82 @@ struct Ops<float> {
   static __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
     *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
   }
+};
+
+template <>
+struct Ops<Split> {
+  using One = Ops<unsigned short>;
+  struct Frag {
+    short8 part[3];
+  };
+  using Mem = float;
+  using Lds = unsigned short;
+  static constexpr bool kBf16 = false;
+  static constexpr int kDims = 32;
+  static constexpr int kLane = 8;
+  static constexpr int kVec = 4;
+  static constexpr int kSub = 2;
+  static constexpr int kParts = 3;
+  static constexpr int row_pitch(int d) { return One::row_pitch(d); }
+  static constexpr int tr_pitch(int d) { return One::tr_pitch(d); }
+  // Eight values, each the sum of its three parts: bf16(x), bf16 of the rest, and what then remains, at most 8 bits.
+  static __device__ __forceinline__ Frag cut(float4v a, float4v b) {
+    Frag f;
+    float4v s[2] = {a, b};
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      f.part[p] = One::acc_frag(s);
+      if (p < 2) One::take(s, f.part[p]);
+    }
+    return f;
+  }
+  static __device__ __forceinline__ Frag from_memory(const float* p) {
+    return cut(*reinterpret_cast<const float4v*>(p), *reinterpret_cast<const float4v*>(p + 4));
+  }
+  static __device__ __forceinline__ void stage(unsigned short* t, int pitch, int row, int col, const uint4& v) {
+    float4v s = __builtin_bit_cast(float4v, v);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      const uint2 w = make_uint2(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]));
+      *reinterpret_cast<uint2*>(t + (p * kTile + row) * pitch + col) = w;
+      s[0] -= __uint_as_float(w.x << 16);
+      s[1] -= __uint_as_float(w.x & 0xffff0000u);
+      s[2] -= __uint_as_float(w.y << 16);
+      s[3] -= __uint_as_float(w.y & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ Frag row_frag(const unsigned short* t, int pitch, int row, int c, int q4) {
+    Frag f;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) f.part[p] = One::row_frag(t + p * kTile * pitch, pitch, row, c, q4);
+    return f;
+  }
+  static __device__ __forceinline__ Frag tr_frag(const unsigned short* t, int pitch, int kb, int n, int l15, int q4) {
+    Frag f;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) f.part[p] = One::tr_frag(t + p * kTile * pitch, pitch, kb, n, l15, q4);
+    return f;
+  }
+  static __device__ __forceinline__ Frag acc_frag(const float4v* s) { return cut(s[0], s[1]); }
+  static __device__ __forceinline__ void take(float4v*, const Frag&) {}
+  static __device__ __forceinline__ float4v mma(const Frag& a, const Frag& b, float4v c) {  // smallest terms first
+    c = One::mma(a.part[2], b.part[0], c);
+    c = One::mma(a.part[0], b.part[2], c);
+    c = One::mma(a.part[1], b.part[1], c);
+    c = One::mma(a.part[1], b.part[0], c);
+    c = One::mma(a.part[0], b.part[1], c);
+    return One::mma(a.part[0], b.part[0], c);
+  }
+  static __device__ __forceinline__ float dot(const Frag& a, const float* o) {
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = (bf16_to_float((unsigned short)a.part[0][e]) + bf16_to_float((unsigned short)a.part[1][e])) + bf16_to_float((unsigned short)a.part[2][e]);
+      s = fmaf(x, o[e], s);
+    }
+    return s;
+  }
+  static __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) { Ops<float>::store4(p, a, b, c, d); }
 };
 
 // Consecutive logical workgroups on the same XCD (the hardware deals blockIdx out round robin over eight), so that the query
@@ -147,35 +244,35 @@ __device__ __forceinline__ void fill_bias(const EncAttnArgs& a, float* bias, int
 // bit in `word` is clear (whatever the masked row holds) and beyond the matrix's width.
 template <typename T, int D>
 struct Stage {
-  static constexpr int kVecsPerRow = D / Ops<T>::kVec;
+  using O = Ops<T>;
+  static constexpr int kVecsPerRow = D / O::kVec;
   static constexpr int kN = kTile * kVecsPerRow / 256;
   uint4 r[kN];
-  __device__ __forceinline__ void load(const T* base, long long pitch, int t0, unsigned long long word, int width, int tid) {
+  __device__ __forceinline__ void load(const typename O::Mem* base, long long pitch, int t0, unsigned long long word, int width, int tid) {
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int vi = tid + i * 256, row = vi / kVecsPerRow, col = (vi % kVecsPerRow) * Ops<T>::kVec;
+      const int vi = tid + i * 256, row = vi / kVecsPerRow, col = (vi % kVecsPerRow) * O::kVec;
       r[i] = make_uint4(0, 0, 0, 0);
       if (((word >> row) & 1) && col < width) r[i] = *reinterpret_cast<const uint4*>(base + (long long)(t0 + row) * pitch + col);
     }
   }
-  __device__ __forceinline__ void store(T* lds, int pitch, int tid) const {
+  __device__ __forceinline__ void store(typename O::Lds* lds, int pitch, int tid) const {
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int vi = tid + i * 256, row = vi / kVecsPerRow, col = (vi % kVecsPerRow) * Ops<T>::kVec;
-      *reinterpret_cast<uint4*>(lds + row * pitch + col) = r[i];
+      const int vi = tid + i * 256;
+      O::stage(lds, pitch, vi / kVecsPerRow, (vi % kVecsPerRow) * O::kVec, r[i]);
     }
   }
 };
 
 // Row fragments of up to 16 owned tokens straight from memory (each value is read by one lane).
 template <typename T, int C>
-__device__ __forceinline__ void load_rows(typename Ops<T>::Frag (&f)[C], const T* row, bool valid, int width, int q4) {
-  using Frag = typename Ops<T>::Frag;
+__device__ __forceinline__ void load_rows(typename Ops<T>::Frag (&f)[C], const typename Ops<T>::Mem* row, bool valid, int width, int q4) {
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int col = c * Ops<T>::kDims + q4 * Ops<T>::kVec;
-    f[c] = Ops<T>::zero();
-    if (valid && col < width) f[c] = *reinterpret_cast<const Frag*>(row + col);
+    const int col = c * Ops<T>::kDims + q4 * Ops<T>::kLane;
+    f[c] = typename Ops<T>::Frag{};
+    if (valid && col < width) f[c] = Ops<T>::from_memory(row + col);
   }
 }
 

@@ -55,15 +55,15 @@ __device__ __forceinline__ void add_tile(const EncAttnArgs& a, float* sums, cons
 
 // One 4-wave workgroup per (head, 64 QS queries, key range) and q_chunk samples, one after the other.
 template <typename T, int D, int M, int QS, bool BIAS, int NT>
-__global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncQueries)) void enc_attn_bwd_q_kernel(EncAttnArgs a) {
+__global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncQueries)) void enc_attn_bwd_q_kernel(EncAttnArgs a) {
   using O = Ops<T>;
   using Frag = typename O::Frag;
   constexpr int DV = D * M, DC = D / O::kDims, VC = DV / O::kDims, ND = D / 16, NKB = 4 / O::kSub;
-  constexpr int PK = O::row_pitch(D), PV = O::row_pitch(DV);
+  constexpr int PK = O::row_pitch(D), PV = O::row_pitch(DV), TK = O::kParts * kTile * PK;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  T* k_lds = reinterpret_cast<T*>(smem);
-  T* v_lds = k_lds + M * kTile * PK;
-  int* pos_lds = reinterpret_cast<int*>(v_lds + kTile * PV);
+  typename O::Lds* k_lds = reinterpret_cast<typename O::Lds*>(smem);
+  typename O::Lds* v_lds = k_lds + M * TK;
+  int* pos_lds = reinterpret_cast<int*>(v_lds + O::kParts * kTile * PV);
   float* bias_lds = reinterpret_cast<float*>(pos_lds + (NT ? NT : 1) * kTile);
   const int slots = BIAS ? 2 * a.R + 1 : 0, R2 = 2 * a.R;
   float* ds_lds = bias_lds + ((M * slots + 3) & ~3);
@@ -94,10 +94,10 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncQu
   Stage<T, D> sk[M];
   Stage<T, DV> sv;
   auto fetch = [&](const TileWalk& w) {
-    const T* kb = reinterpret_cast<const T*>(a.k) + w.sample * a.ks[0] + (long long)kvh * M * a.ks[2];
+    const typename O::Mem* kb = reinterpret_cast<const typename O::Mem*>(a.k) + w.sample * a.ks[0] + (long long)kvh * M * a.ks[2];
 #pragma unroll
     for (int m = 0; m < M; ++m) sk[m].load(kb + m * a.ks[2], a.ks[1], w.tile * kTile, w.word, a.D, tid);
-    sv.load(reinterpret_cast<const T*>(a.v) + w.sample * a.vs[0] + kvh * a.vs[2], a.vs[1], w.tile * kTile, w.word, a.DV, tid);
+    sv.load(reinterpret_cast<const typename O::Mem*>(a.v) + w.sample * a.vs[0] + kvh * a.vs[2], a.vs[1], w.tile * kTile, w.word, a.DV, tid);
   };
   TileWalk walk;
   if constexpr (NT == 0) {
@@ -147,10 +147,10 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncQu
     for (int s = 0; s < QS; ++s) {
       const int query = q_first + s * 16 + l15;
       const bool valid = query < a.Lq;
-      load_rows<T, VC>(dof[s], reinterpret_cast<const T*>(a.dout) + b * a.gs[0] + (long long)query * a.gs[1] + h * a.gs[2], valid, a.DV, q4);
+      load_rows<T, VC>(dof[s], reinterpret_cast<const typename O::Mem*>(a.dout) + b * a.gs[0] + (long long)query * a.gs[1] + h * a.gs[2], valid, a.DV, q4);
 #pragma unroll
       for (int m = 0; m < M; ++m) {
-        load_rows<T, DC>(qf[m][s], reinterpret_cast<const T*>(a.q) + b * a.qs[0] + (long long)query * a.qs[1] + (long long)(h * M + m) * a.qs[2], valid,
+        load_rows<T, DC>(qf[m][s], reinterpret_cast<const typename O::Mem*>(a.q) + b * a.qs[0] + (long long)query * a.qs[1] + (long long)(h * M + m) * a.qs[2], valid,
                          a.D, q4);
         float2 st = make_float2(INFINITY, 0.f);
         if (valid) st = *reinterpret_cast<const float2*>(a.stat + 2 * (m * rows + row0 + query));
@@ -160,11 +160,11 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncQu
         float dot = 0.f;
 #pragma unroll
         for (int c = 0; c < VC; ++c) {
-          const int col = c * O::kDims + q4 * O::kVec;
+          const int col = c * O::kDims + q4 * O::kLane;
           if (!valid || col >= a.DV) continue;
-          float v[O::kVec];
+          float v[O::kLane];
 #pragma unroll
-          for (int e = 0; e < O::kVec; e += 4) {
+          for (int e = 0; e < O::kLane; e += 4) {
             const float4 u = *reinterpret_cast<const float4*>(o + col + e);
             v[e] = u.x; v[e + 1] = u.y; v[e + 2] = u.z; v[e + 3] = u.w;
           }
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncQu
       const int t0 = walk.tile * kTile;
       __syncthreads();
 #pragma unroll
-      for (int m = 0; m < M; ++m) sk[m].store(k_lds + m * kTile * PK, PK, tid);
+      for (int m = 0; m < M; ++m) sk[m].store(k_lds + m * TK, PK, tid);
       sv.store(v_lds, PV, tid);
       if (BIAS && NT == 0 && tid < kTile) pos_lds[tid] = token_pos(t0 + tid, a.W);
       __syncthreads();
@@ -274,7 +274,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncQu
               for (int m = 0; m < M; ++m) {
 #pragma unroll
                 for (int c = 0; c < DC; ++c) {
-                  const Frag kf = O::row_frag(k_lds + m * kTile * PK, PK, kt * 16 + l15, c, q4);
+                  const Frag kf = O::row_frag(k_lds + m * TK, PK, kt * 16 + l15, c, q4);
 #pragma unroll
                   for (int s = 0; s < QS; ++s) ds[m][s][kt] = O::mma(kf, qf[m][s][c], ds[m][s][kt]);
                 }
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncQu
               for (int s = 0; s < QS; ++s) sf[s] = O::acc_frag(&ds[m][s][kb * O::kSub]);
 #pragma unroll
               for (int n = 0; n < ND; ++n) {
-                const Frag kf = O::tr_frag(k_lds + m * kTile * PK, PK, kb, n, l15, q4);
+                const Frag kf = O::tr_frag(k_lds + m * TK, PK, kb, n, l15, q4);
 #pragma unroll
                 for (int s = 0; s < QS; ++s) dq[m][s][n] = O::mma(kf, sf[s], dq[m][s][n]);
               }
@@ -381,7 +381,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncQu
 #pragma unroll
       for (int m = 0; m < M; ++m) {
         const float c = a.scale * (m == 0 ? inv[m][s] : -lam * inv[m][s]);
-        T* row = reinterpret_cast<T*>(a.dq) + b * a.dqs[0] + (long long)query * a.dqs[1] + (long long)(h * M + m) * a.dqs[2];
+        typename O::Mem* row = reinterpret_cast<typename O::Mem*>(a.dq) + b * a.dqs[0] + (long long)query * a.dqs[1] + (long long)(h * M + m) * a.dqs[2];
         float* part = a.dq_part + ((split * rows + row0 + query) * M + m) * a.D;
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
@@ -444,15 +444,15 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncQu
 // One 4-wave workgroup per (key / value head, 64 KS keys, query range) and k_chunk samples; a wave owns 16 KS keys and walks the
 // query tiles of every query head that shares them.
 template <typename T, int D, int M, int KS, bool BIAS, int NT>
-__global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, sizeof(T) == 2, kEncKeys)) void enc_attn_bwd_k_kernel(EncAttnArgs a) {
+__global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, Ops<T>::kBf16, kEncKeys)) void enc_attn_bwd_k_kernel(EncAttnArgs a) {
   using O = Ops<T>;
   using Frag = typename O::Frag;
   constexpr int DV = D * M, DC = D / O::kDims, VC = DV / O::kDims, ND = D / 16, NV = DV / 16, NKB = 4 / O::kSub;
-  constexpr int PQ = O::row_pitch(D), PG = O::row_pitch(DV);
+  constexpr int PQ = O::row_pitch(D), PG = O::row_pitch(DV), TQ = O::kParts * kTile * PQ;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  T* q_lds = reinterpret_cast<T*>(smem);
-  T* g_lds = q_lds + M * kTile * PQ;
-  int* pos_lds = reinterpret_cast<int*>(g_lds + kTile * PG);
+  typename O::Lds* q_lds = reinterpret_cast<typename O::Lds*>(smem);
+  typename O::Lds* g_lds = q_lds + M * TQ;
+  int* pos_lds = reinterpret_cast<int*>(g_lds + O::kParts * kTile * PG);
   float* top_lds = reinterpret_cast<float*>(pos_lds + (NT ? NT : 1) * kTile);
   float* inv_lds = top_lds + M * kTile;
   float* delta_lds = inv_lds + M * kTile;
@@ -488,8 +488,8 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, sizeof(T) == 2, kEncKe
     const unsigned long long word = range_word(t0, a.Lq);
 #pragma unroll
     for (int m = 0; m < M; ++m)
-      sq[m].load(reinterpret_cast<const T*>(a.q) + b * a.qs[0] + (long long)(h * M + m) * a.qs[2], a.qs[1], t0, word, a.D, tid);
-    sg.load(reinterpret_cast<const T*>(a.dout) + b * a.gs[0] + h * a.gs[2], a.gs[1], t0, word, a.DV, tid);
+      sq[m].load(reinterpret_cast<const typename O::Mem*>(a.q) + b * a.qs[0] + (long long)(h * M + m) * a.qs[2], a.qs[1], t0, word, a.D, tid);
+    sg.load(reinterpret_cast<const typename O::Mem*>(a.dout) + b * a.gs[0] + h * a.gs[2], a.gs[1], t0, word, a.DV, tid);
     const int which = tid >> 6, i = t0 + (tid & 63);
     const long long row = ((long long)b * a.H + h) * a.Lq + i;
     if (which < M) {
@@ -531,9 +531,9 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, sizeof(T) == 2, kEncKe
       any |= live[s];
 #pragma unroll
       for (int m = 0; m < M; ++m)
-        load_rows<T, DC>(kf[m][s], reinterpret_cast<const T*>(a.k) + b * a.ks[0] + (long long)key * a.ks[1] + (long long)(kvh * M + m) * a.ks[2],
+        load_rows<T, DC>(kf[m][s], reinterpret_cast<const typename O::Mem*>(a.k) + b * a.ks[0] + (long long)key * a.ks[1] + (long long)(kvh * M + m) * a.ks[2],
                          live[s], a.D, q4);
-      load_rows<T, VC>(vf[s], reinterpret_cast<const T*>(a.v) + b * a.vs[0] + (long long)key * a.vs[1] + kvh * a.vs[2], live[s], a.DV, q4);
+      load_rows<T, VC>(vf[s], reinterpret_cast<const typename O::Mem*>(a.v) + b * a.vs[0] + (long long)key * a.vs[1] + kvh * a.vs[2], live[s], a.DV, q4);
     }
     float4v dk[M][KS][ND], dv[KS][NV];
 #pragma unroll
@@ -554,7 +554,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, sizeof(T) == 2, kEncKe
       const float lam = M == 2 ? a.lam[h] : 0.f;
       __syncthreads();
 #pragma unroll
-      for (int m = 0; m < M; ++m) sq[m].store(q_lds + m * kTile * PQ, PQ, tid);
+      for (int m = 0; m < M; ++m) sq[m].store(q_lds + m * TQ, PQ, tid);
       sg.store(g_lds, PG, tid);
       if (tid < M * kTile) {
         top_lds[tid] = stat.x;
@@ -620,7 +620,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, sizeof(T) == 2, kEncKe
             }
 #pragma unroll
             for (int c = 0; c < DC; ++c) {
-              const Frag qf = O::row_frag(q_lds + m * kTile * PQ, PQ, qt * 16 + l15, c, q4);
+              const Frag qf = O::row_frag(q_lds + m * TQ, PQ, qt * 16 + l15, c, q4);
 #pragma unroll
               for (int s = 0; s < KS; ++s) x[s] = O::mma(qf, kf[m][s][c], x[s]);
             }
@@ -670,7 +670,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, sizeof(T) == 2, kEncKe
           for (int s = 0; s < KS; ++s) sf[s] = O::acc_frag(ds[m][s]);
 #pragma unroll
           for (int n = 0; n < ND; ++n) {
-            const Frag qf = O::tr_frag(q_lds + m * kTile * PQ, PQ, kb, n, l15, q4);
+            const Frag qf = O::tr_frag(q_lds + m * TQ, PQ, kb, n, l15, q4);
 #pragma unroll
             for (int s = 0; s < KS; ++s) dk[m][s][n] = O::mma(qf, sf[s], dk[m][s][n]);
           }
@@ -705,7 +705,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, sizeof(T) == 2, kEncKe
       if (key >= a.Lk) continue;
       const long long krow = ((long long)b * a.KV + kvh) * a.Lk + key;
       float* part = a.kv_part + (split * ((long long)a.B * a.KV * a.Lk) + krow) * (M * a.D + a.DV);
-      T* dv_row = reinterpret_cast<T*>(a.dv) + b * a.dvs[0] + (long long)key * a.dvs[1] + kvh * a.dvs[2];
+      typename O::Mem* dv_row = reinterpret_cast<typename O::Mem*>(a.dv) + b * a.dvs[0] + (long long)key * a.dvs[1] + kvh * a.dvs[2];
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         const int dim = n * 16 + q4 * 4;
@@ -716,7 +716,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, sizeof(T) == 2, kEncKe
       }
 #pragma unroll
       for (int m = 0; m < M; ++m) {
-        T* dk_row = reinterpret_cast<T*>(a.dk) + b * a.dks[0] + (long long)key * a.dks[1] + (long long)(kvh * M + m) * a.dks[2];
+        typename O::Mem* dk_row = reinterpret_cast<typename O::Mem*>(a.dk) + b * a.dks[0] + (long long)key * a.dks[1] + (long long)(kvh * M + m) * a.dks[2];
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
           const int dim = n * 16 + q4 * 4;
@@ -825,8 +825,8 @@ __global__ __launch_bounds__(256) void enc_small_grads_kernel(SmallGrads a) {
 template <typename T, int D, int M, bool BIAS, int NT>
 int launch_bwd_k(const EncAttnArgs& a, hipStream_t stream) {
   using O = Ops<T>;
-  constexpr int KS = enc_columns_of(D, M, NT, kEncKeys);
-  const size_t lds = sizeof(T) * (size_t)kTile * (M * O::row_pitch(D) + O::row_pitch(D * M)) + (NT ? NT : 1) * kTile * sizeof(int) +
+  constexpr int KS = enc_columns_of(D, M, NT, Ops<T>::kBf16, kEncKeys);
+  const size_t lds = sizeof(typename O::Lds) * (size_t)(O::kParts * kTile) * (M * O::row_pitch(D) + O::row_pitch(D * M)) + (NT ? NT : 1) * kTile * sizeof(int) +
                      sizeof(float) * (3 * M * kTile + 4 + (BIAS ? M * (2 * a.R + 1) : 0));
   const int rc = enc_lds(enc_attn_bwd_k_kernel<T, D, M, KS, BIAS, NT>, lds);
   if (rc) return rc;
@@ -836,23 +836,24 @@ int launch_bwd_k(const EncAttnArgs& a, hipStream_t stream) {
   return hip_err(hipGetLastError());
 }
 
-template <typename T, int D, int M, bool BIAS, int NT = 0>
+// TQ: rows of the query-owned pass
+template <typename TQ, typename T, int D, int M, bool BIAS, int NT = 0>
 int launch_bwd(EncAttnArgs a, hipStream_t stream) {
-  using O = Ops<T>;
-  constexpr int QS = enc_columns_of(D, M, NT, kEncQueries);
+  using O = Ops<TQ>;
+  constexpr int QS = enc_columns_of(D, M, NT, O::kBf16, kEncQueries);
   const size_t slots = BIAS ? 2 * a.R + 1 : 0;
-  size_t lds = sizeof(T) * (size_t)kTile * (M * O::row_pitch(D) + O::row_pitch(D * M)) + (NT ? NT : 1) * kTile * sizeof(int);
+  size_t lds = sizeof(typename O::Lds) * (size_t)(O::kParts * kTile) * (M * O::row_pitch(D) + O::row_pitch(D * M)) + (NT ? NT : 1) * kTile * sizeof(int);
   if (BIAS) lds += sizeof(float) * ((M * slots + 3) / 4 * 4 + 4 * 16 * kDsPitch);
   a.hist_rows = 4;
   if (BIAS && a.hist) {
-    // a row of sums per wave; one for all where four rows would leave a single workgroup per CU
-    if (lds + sizeof(float) * 4 * M * slots > kMaxLds / 2) a.hist_rows = 1;
+    // a row of sums per wave; one for all where four rows would leave fewer workgroups per CU than the registers allow
+    if (lds + sizeof(float) * 4 * M * slots > kMaxLds / enc_waves(D, M, NT, QS, O::kBf16, kEncQueries)) a.hist_rows = 1;
     lds += sizeof(float) * a.hist_rows * M * slots;
   }
-  int rc = enc_lds(enc_attn_bwd_q_kernel<T, D, M, QS, BIAS, NT>, lds);
+  int rc = enc_lds(enc_attn_bwd_q_kernel<TQ, D, M, QS, BIAS, NT>, lds);
   if (rc) return rc;
   const int nqt = (a.Lq + 64 * QS - 1) / (64 * QS);
-  hipLaunchKernelGGL((enc_attn_bwd_q_kernel<T, D, M, QS, BIAS, NT>), dim3((unsigned)((a.B + a.q_chunk - 1) / a.q_chunk * a.H * nqt * a.q_splits)), dim3(256),
+  hipLaunchKernelGGL((enc_attn_bwd_q_kernel<TQ, D, M, QS, BIAS, NT>), dim3((unsigned)((a.B + a.q_chunk - 1) / a.q_chunk * a.H * nqt * a.q_splits)), dim3(256),
                      lds, stream, a);
   rc = hip_err(hipGetLastError());
   if (rc) return rc;
@@ -885,20 +886,23 @@ int join_grads(const EncAttnArgs& a, hipStream_t stream) {
   return 0;
 }
 
-template <typename T>
+// T: bf16 rows, or Split; W: fp32 rows with the fp32 matrix instruction, where the parts would not fit: two 64-wide maps into LDS
+// (128-wide heads: 1081 us in parts, 1544 us without), the query-owned pass of a two-map board into registers (256 boards of
+// 120 cells: 84 us in parts, 70 us without).
+template <typename T, typename W>
 int dispatch_bwd(const EncAttnArgs& a, hipStream_t stream) {
   const int w = enc_width(a.D), nt = enc_board_tiles(a.table ? a.W : 0, a.Lk, a.D, a.M);
   if (nt > 0 && (a.q_splits > 1 || (a.KV == a.H && a.k_splits > 1))) return -18;
   if (a.M == 1) {
-    if (nt == 2) return launch_bwd<T, 32, 1, true, 2>(a, stream);
-    if (nt == 4) return launch_bwd<T, 32, 1, true, 4>(a, stream);
-    if (w == 32) return launch_bwd<T, 32, 1, true>(a, stream);
-    if (w == 64) return launch_bwd<T, 64, 1, true>(a, stream);
-    return launch_bwd<T, 128, 1, true>(a, stream);
+    if (nt == 2) return launch_bwd<T, T, 32, 1, true, 2>(a, stream);
+    if (nt == 4) return launch_bwd<T, T, 32, 1, true, 4>(a, stream);
+    if (w == 32) return launch_bwd<T, T, 32, 1, true>(a, stream);
+    if (w == 64) return launch_bwd<T, T, 64, 1, true>(a, stream);
+    return launch_bwd<T, T, 128, 1, true>(a, stream);
   }
-  if (nt == 2) return launch_bwd<T, 32, 2, true, 2>(a, stream);
-  if (w == 32) return a.table ? launch_bwd<T, 32, 2, true>(a, stream) : launch_bwd<T, 32, 2, false>(a, stream);
-  return a.table ? launch_bwd<T, 64, 2, true>(a, stream) : launch_bwd<T, 64, 2, false>(a, stream);
+  if (nt == 2) return launch_bwd<W, T, 32, 2, true, 2>(a, stream);
+  if (w == 32) return a.table ? launch_bwd<T, T, 32, 2, true>(a, stream) : launch_bwd<T, T, 32, 2, false>(a, stream);
+  return a.table ? launch_bwd<W, W, 64, 2, true>(a, stream) : launch_bwd<W, W, 64, 2, false>(a, stream);
 }
 
 }  // namespace
@@ -921,12 +925,12 @@ int atri_enc_attn_bwd(const EncAttnArgs* args, hipStream_t stream) {
   }
   if (a.dlam && (a.M != 2 || !a.dlam_part)) return -14;
   if ((a.q_splits > 1 && !a.dq_part) || (a.k_splits > 1 && !a.kv_part)) return -17;
-  rc = a.bf16 ? dispatch_bwd<unsigned short>(a, stream) : dispatch_bwd<float>(a, stream);
+  rc = a.bf16 ? dispatch_bwd<unsigned short, unsigned short>(a, stream) : dispatch_bwd<Split, float>(a, stream);
   if (rc) return rc;
   rc = a.bf16 ? join_grads<unsigned short>(a, stream) : join_grads<float>(a, stream);
   if (rc) return rc;
   if (!a.hist && !a.dlam) return 0;
-  const int per = 64 * enc_columns(a.table ? a.W : 0, a.Lq, a.Lk, a.D, a.M, kEncQueries), nqt = (a.Lq + per - 1) / per;
+  const int per = 64 * enc_columns(a.table ? a.W : 0, a.Lq, a.Lk, a.D, a.M, a.bf16 != 0, kEncQueries), nqt = (a.Lq + per - 1) / per;
   SmallGrads g{a.hist, a.order, a.start, a.dtable, a.dlam_part, a.dlam, (a.B + a.q_chunk - 1) / a.q_chunk, a.H, nqt * a.q_splits, a.M, slots, a.buckets, 0};
   if (a.hist) {
     g.table_groups = (a.buckets * hm + 3) / 4;

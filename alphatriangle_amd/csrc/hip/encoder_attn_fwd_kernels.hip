@@ -15,15 +15,15 @@ namespace {
 // pass follows, for delta = dO . o has to match dP = dO V^T to 32 bits: the gradients of the table and of lam are sums
 // of p (dP - delta) in which everything but the error of delta cancels (with one fragment they were 1e-3 off).
 template <typename T, int D, int M, int QS, bool BIAS, int PL, int NT>
-__global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncForward)) void enc_attn_fwd_kernel(EncAttnArgs a) {
+__global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncForward)) void enc_attn_fwd_kernel(EncAttnArgs a) {
   using O = Ops<T>;
   using Frag = typename O::Frag;
   constexpr int DV = D * M, DC = D / O::kDims, NV = DV / 16, NKB = 4 / O::kSub;
-  constexpr int PK = O::row_pitch(D), PV = O::tr_pitch(DV);
+  constexpr int PK = O::row_pitch(D), PV = O::tr_pitch(DV), TK = O::kParts * kTile * PK;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  T* k_lds = reinterpret_cast<T*>(smem);
-  T* v_lds = k_lds + M * kTile * PK;
-  int* pos_lds = reinterpret_cast<int*>(v_lds + kTile * PV);
+  typename O::Lds* k_lds = reinterpret_cast<typename O::Lds*>(smem);
+  typename O::Lds* v_lds = k_lds + M * TK;
+  int* pos_lds = reinterpret_cast<int*>(v_lds + O::kParts * kTile * PV);
   float* bias_lds = reinterpret_cast<float*>(pos_lds + (NT ? NT : 1) * kTile);
 
   const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, q4 = lane >> 4;
@@ -48,10 +48,10 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncFo
   Stage<T, D> sk[M];
   Stage<T, DV> sv;
   auto fetch = [&](const TileWalk& w) {
-    const T* kb = reinterpret_cast<const T*>(a.k) + w.sample * a.ks[0] + (long long)kvh * M * a.ks[2];
+    const typename O::Mem* kb = reinterpret_cast<const typename O::Mem*>(a.k) + w.sample * a.ks[0] + (long long)kvh * M * a.ks[2];
 #pragma unroll
     for (int m = 0; m < M; ++m) sk[m].load(kb + m * a.ks[2], a.ks[1], w.tile * kTile, w.word, a.D, tid);
-    sv.load(reinterpret_cast<const T*>(a.v) + w.sample * a.vs[0] + kvh * a.vs[2], a.vs[1], w.tile * kTile, w.word, a.DV, tid);
+    sv.load(reinterpret_cast<const typename O::Mem*>(a.v) + w.sample * a.vs[0] + kvh * a.vs[2], a.vs[1], w.tile * kTile, w.word, a.DV, tid);
   };
   Frag qf[M][QS][DC];
   auto fetch_queries = [&](int b) {
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncFo
       const int query = q_first + s * 16 + l15;
 #pragma unroll
       for (int m = 0; m < M; ++m)
-        load_rows<T, DC>(qf[m][s], reinterpret_cast<const T*>(a.q) + b * a.qs[0] + (long long)query * a.qs[1] + (long long)(h * M + m) * a.qs[2],
+        load_rows<T, DC>(qf[m][s], reinterpret_cast<const typename O::Mem*>(a.q) + b * a.qs[0] + (long long)query * a.qs[1] + (long long)(h * M + m) * a.qs[2],
                          query < a.Lq, a.D, q4);
     }
   };
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncFo
       const int t0 = walk.tile * kTile;
       __syncthreads();  // every wave is past its reads of the previous tile
 #pragma unroll
-      for (int m = 0; m < M; ++m) sk[m].store(k_lds + m * kTile * PK, PK, tid);
+      for (int m = 0; m < M; ++m) sk[m].store(k_lds + m * TK, PK, tid);
       sv.store(v_lds, PV, tid);
       if (BIAS && NT == 0 && tid < kTile) pos_lds[tid] = token_pos(t0 + tid, a.W);
       __syncthreads();
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncFo
         for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
           for (int c = 0; c < DC; ++c) {
-            const Frag kf = O::row_frag(k_lds + m * kTile * PK, PK, kt * 16 + l15, c, q4);
+            const Frag kf = O::row_frag(k_lds + m * TK, PK, kt * 16 + l15, c, q4);
 #pragma unroll
             for (int s = 0; s < QS; ++s) st[m][s][kt] = O::mma(kf, qf[m][s][c], st[m][s][kt]);
           }
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, sizeof(T) == 2, kEncFo
 #pragma unroll
           for (int j = 0; j < 4; ++j) r[0][j] = fmaf(-lam, r[1][j], r[0][j]);
         }
-        O::store4(reinterpret_cast<T*>(a.out) + b * a.os[0] + (long long)query * a.os[1] + h * a.os[2] + dim, r[0][0], r[0][1], r[0][2], r[0][3]);
+        O::store4(reinterpret_cast<typename O::Mem*>(a.out) + b * a.os[0] + (long long)query * a.os[1] + h * a.os[2] + dim, r[0][0], r[0][1], r[0][2], r[0][3]);
       }
     }
   }
@@ -389,7 +389,7 @@ __global__ __launch_bounds__(256) void key_words_kernel(const unsigned char* mas
 template <typename T, int D, int M, int QS, bool BIAS, int PL, int NT>
 int launch_fwd_planes(const EncAttnArgs& a, hipStream_t stream) {
   using O = Ops<T>;
-  size_t lds = sizeof(T) * (size_t)kTile * (M * O::row_pitch(D) + O::tr_pitch(D * M)) + (NT ? NT : 1) * kTile * sizeof(int);
+  size_t lds = sizeof(typename O::Lds) * (size_t)(O::kParts * kTile) * (M * O::row_pitch(D) + O::tr_pitch(D * M)) + (NT ? NT : 1) * kTile * sizeof(int);
   if (BIAS) lds += sizeof(float) * (size_t)M * (2 * a.R + 1);
   const int rc = enc_lds(enc_attn_fwd_kernel<T, D, M, QS, BIAS, PL, NT>, lds);
   if (rc) return rc;
@@ -401,27 +401,29 @@ int launch_fwd_planes(const EncAttnArgs& a, hipStream_t stream) {
 
 template <typename T, int D, int M, int QS, bool BIAS, int NT = 0>
 int launch_fwd(const EncAttnArgs& a, hipStream_t stream) {
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (Ops<T>::kBf16) {
     if (a.o32) return launch_fwd_planes<T, D, M, QS, BIAS, 3, NT>(a, stream);
   }
   return launch_fwd_planes<T, D, M, QS, BIAS, 1, NT>(a, stream);
 }
 
-template <typename T>
+// T: bf16 rows, or Split; W: the widest fp32 heads, whose staged parts would leave one workgroup per CU (128-wide: 336 us in
+// parts, 320 us with the fp32 instruction) or fill the LDS (two 64-wide maps).
+template <typename T, typename W>
 int dispatch_fwd(const EncAttnArgs& a, hipStream_t stream) {
   const int w = enc_width(a.D), nt = enc_board_tiles(a.table ? a.W : 0, a.Lk, a.D, a.M);
   if (nt > 0 && a.splits > 1) return -18;
-  const bool two = enc_columns(a.table ? a.W : 0, a.Lq, a.Lk, a.D, a.M, kEncForward) == 2;
+  const bool two = enc_columns(a.table ? a.W : 0, a.Lq, a.Lk, a.D, a.M, a.bf16 != 0, kEncForward) == 2;
   if (a.M == 1) {
-    if (nt == 2) return launch_fwd<T, 32, 1, enc_columns_of(32, 1, 2, kEncForward), true, 2>(a, stream);
+    if (nt == 2) return launch_fwd<T, 32, 1, enc_columns_of(32, 1, 2, Ops<T>::kBf16, kEncForward), true, 2>(a, stream);
     if (nt == 4) return launch_fwd<T, 32, 1, 1, true, 4>(a, stream);
     if (w == 32) return two ? launch_fwd<T, 32, 1, 2, true>(a, stream) : launch_fwd<T, 32, 1, 1, true>(a, stream);
     if (w == 64) return two ? launch_fwd<T, 64, 1, 2, true>(a, stream) : launch_fwd<T, 64, 1, 1, true>(a, stream);
-    return launch_fwd<T, 128, 1, 1, true>(a, stream);
+    return launch_fwd<W, 128, 1, 1, true>(a, stream);
   }
   if (nt == 2) return launch_fwd<T, 32, 2, 1, true, 2>(a, stream);
   if (w == 32) return a.table ? launch_fwd<T, 32, 2, 1, true>(a, stream) : launch_fwd<T, 32, 2, 1, false>(a, stream);
-  return a.table ? launch_fwd<T, 64, 2, 1, true>(a, stream) : launch_fwd<T, 64, 2, 1, false>(a, stream);
+  return a.table ? launch_fwd<W, 64, 2, 1, true>(a, stream) : launch_fwd<W, 64, 2, 1, false>(a, stream);
 }
 
 template <typename T, int M>
@@ -456,7 +458,7 @@ int atri_enc_attn_fwd(const EncAttnArgs* args, hipStream_t stream) {
     const int rc1 = hip_err(hipGetLastError());
     if (rc1) return rc1;
   }
-  const int rc2 = a.bf16 ? dispatch_fwd<unsigned short>(a, stream) : dispatch_fwd<float>(a, stream);
+  const int rc2 = a.bf16 ? dispatch_fwd<unsigned short, unsigned short>(a, stream) : dispatch_fwd<Split, float>(a, stream);
   if (rc2 || a.splits == 1) return rc2;
   return a.bf16 ? join<unsigned short>(a, stream) : join<float>(a, stream);
 }

@@ -59,21 +59,26 @@ inline int enc_board_tiles(int W, int Lk, int D, int M) {
 }
 enum EncPass { kEncForward = 0, kEncQueries = 1, kEncKeys = 2 };  // forward, query-owned and key-owned backward pass
 // 16-row columns per wave: queries in the forward and the query-owned pass, keys in the key-owned one.
-constexpr int enc_columns_of(int D, int M, int nt, int pass) {
+constexpr int enc_columns_of(int D, int M, int nt, bool bf16, int pass) {
   if (M == 2 || D > 64 || nt == 4) return 1;
+  // fp32 operands take three times the registers: one where two spill (two 2048-token sequences of eight 64-wide heads, backward:
+  // 574 us with two, 408 us with one; 32-wide heads: 258 and 316 us)
+  if (!bf16 && D > 32 && pass != kEncForward) return 1;
   // two: every staged fragment feeds two products; one where bias and sums of dS share the registers (256 boards of 120 cells,
   // fp32, query-owned pass: 68 us with two, 51 us with one; forward and key-owned pass: no difference within 3 %)
   return nt == 2 && pass == kEncQueries ? 1 : 2;
 }
-inline int enc_columns(int W, int L, int Lk, int D, int M, int pass) {
+inline int enc_columns(int W, int L, int Lk, int D, int M, bool bf16, int pass) {
   const int nt = enc_board_tiles(W, Lk, D, M);
-  return nt == 0 && pass == kEncForward && L <= 64 ? 1 : enc_columns_of(D, M, nt, pass);
+  return nt == 0 && pass == kEncForward && L <= 64 ? 1 : enc_columns_of(D, M, nt, bf16, pass);
 }
 // Waves per SIMD the register allocation of a kernel leaves room for.  These kernels wait on LDS and on the matrix and
 // exponential pipes, so a second wave is worth some spilled registers (two 4095-token sequences in bf16, both backward
-// passes: 857 us with one, 466 us with two); a third is not, except where the kernel nearly fits anyway.
+// passes: 857 us with one, 466 us with two); a third is not, except where the kernel nearly fits anyway.  One where a
+// workgroup fills the LDS or keeps the sums of two maps.
 constexpr int enc_waves(int D, int M, int nt, int columns, bool bf16, int pass) {
-  if (pass == kEncForward) return nt == 4 || (nt == 0 && bf16 && M == 1 && D == 64 && columns == 2) ? 3 : 2;
+  if (pass == kEncForward) return bf16 && (nt == 4 || (nt == 0 && M == 1 && D == 64 && columns == 2)) ? 3 : 2;
+  if (!bf16 && D == 128) return 1;
   return pass == kEncQueries && nt == 2 && M == 2 ? 1 : 2;
 }
 

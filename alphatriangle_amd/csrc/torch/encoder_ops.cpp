@@ -116,7 +116,7 @@ void plan(int64_t samples, int64_t groups, int64_t steps, int64_t resident, int&
 int64_t resident(const EncAttnArgs& a, int pass) {
   const int nt = atrihip::enc_board_tiles(a.W, a.Lk, a.D, a.M);
   const int width = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
-  return 256 * atrihip::enc_waves(width, a.M, nt, atrihip::enc_columns(a.W, a.Lq, a.Lk, a.D, a.M, pass), a.bf16 != 0, pass);
+  return 256 * atrihip::enc_waves(width, a.M, nt, atrihip::enc_columns(a.W, a.Lq, a.Lk, a.D, a.M, a.bf16 != 0, pass), a.bf16 != 0, pass);
 }
 
 struct Sizes {
@@ -183,7 +183,7 @@ Tensor attention_forward(const Call& c, const Tensor& q, const Tensor& k, const 
     if (s.n_o32) a.o32 = at_keep + s.n_words + s.n_stat;
   }
   const bool board = atrihip::enc_board_tiles(a.W, a.Lk, a.D, a.M) > 0;  // unrolled over its tiles: never split
-  const int64_t per = 64 * atrihip::enc_columns(a.W, a.Lq, a.Lk, a.D, a.M, atrihip::kEncForward);
+  const int64_t per = 64 * atrihip::enc_columns(a.W, a.Lq, a.Lk, a.D, a.M, a.bf16 != 0, atrihip::kEncForward);
   plan(s.b, s.h * up(s.lq, per), board ? 1 : up(s.lk, atrihip::kTile), resident(a, atrihip::kEncForward), a.splits, a.chunk);
   Tensor part;
   if (a.splits > 1) {
@@ -243,9 +243,9 @@ struct Attention : torch::autograd::Function<Attention> {
     }
     // edges: q, k, v, then the table and lam where they are given
     const bool want_table = table.defined() && ctx->needs_input_grad(3), want_lam = lam.defined() && ctx->needs_input_grad(table.defined() ? 4 : 3);
-    const int64_t nqt = up(s.lq, 64 * atrihip::enc_columns(a.W, a.Lq, a.Lk, a.D, a.M, atrihip::kEncQueries));
+    const int64_t nqt = up(s.lq, 64 * atrihip::enc_columns(a.W, a.Lq, a.Lk, a.D, a.M, a.bf16 != 0, atrihip::kEncQueries));
     // shared heads take the general form of the key-owned pass
-    const int64_t nkt = up(s.lk, 64 * atrihip::enc_columns(s.h == s.kv ? a.W : 0, a.Lq, a.Lk, a.D, a.M, atrihip::kEncKeys));
+    const int64_t nkt = up(s.lk, 64 * atrihip::enc_columns(s.h == s.kv ? a.W : 0, a.Lq, a.Lk, a.D, a.M, a.bf16 != 0, atrihip::kEncKeys));
     const bool board = atrihip::enc_board_tiles(a.W, a.Lk, a.D, a.M) > 0;  // unrolled over its tiles: never split
     plan(s.b, s.h * nqt, board ? 1 : up(s.lk, atrihip::kTile), resident(a, atrihip::kEncQueries), a.q_splits, a.q_chunk);
     plan(s.b, s.kv * nkt, board && s.h == s.kv ? 1 : s.h / s.kv * up(s.lq, atrihip::kTile), resident(a, atrihip::kEncKeys), a.k_splits, a.k_chunk);
