@@ -81,6 +81,12 @@ struct Ops<unsigned short> {
     for (int e = 0; e < 8; ++e) s = fmaf(bf16_to_float((unsigned short)a[e]), o[e], s);
     return s;
   }
+  static __device__ __forceinline__ void negate(Frag& f, bool on) {
+    uint4v u = __builtin_bit_cast(uint4v, f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] ^= on ? 0x80008000u : 0u;
+    f = __builtin_bit_cast(Frag, u);
+  }
   static __device__ __forceinline__ void store4(unsigned short* p, float a, float b, float c, float d) {
     *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
   }
@@ -116,6 +122,10 @@ struct Ops<float> {
 #pragma unroll
     for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
     return c;
+  }
+  static __device__ __forceinline__ void negate(Frag& f, bool on) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = on ? -f[i] : f[i];
   }
   static __device__ __forceinline__ float dot(const Frag& a, const float* o) {
     return fmaf(a[0], o[0], fmaf(a[1], o[1], fmaf(a[2], o[2], a[3] * o[3])));
@@ -197,6 +207,10 @@ struct Ops<Split> {
       s = fmaf(x, o[e], s);
     }
     return s;
+  }
+  static __device__ __forceinline__ void negate(Frag& f, bool on) {
+#pragma unroll
+    for (int p = 0; p < 3; ++p) One::negate(f.part[p], on);
   }
   static __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) { Ops<float>::store4(p, a, b, c, d); }
 };
