@@ -235,6 +235,13 @@ __device__ __forceinline__ int clamp_slot(int d, int R2) { return max(0, min(d, 
 // million: a table used as a mask) take the difference first, which is exact where they are equal; +inf (a row
 // without keys, a query behind the last) gives zeros either way.
 struct Exponent {
+  // The rounded product itself, never fused into what follows: a row's values, the factors between its maxima (exp2 of the
+  // difference of two bases) and the backward pass agree on it.  With the unrounded one in the factors, every new maximum moved
+  // the row by 1e-7 against its sum.
+  static __device__ __forceinline__ float base_of(float top, float sl2) {
+#pragma clang fp contract(off)
+    return top * sl2;
+  }
   static __device__ __forceinline__ bool far(float base) { return fabsf(base) >= 1e6f && base != INFINITY; }
   static __device__ __forceinline__ float near_(float x, float base, float sl2) { return __builtin_amdgcn_exp2f(fmaf(x, sl2, -base)); }
   static __device__ __forceinline__ float far_(float x, float top, float sl2) { return __builtin_amdgcn_exp2f((x - top) * sl2); }

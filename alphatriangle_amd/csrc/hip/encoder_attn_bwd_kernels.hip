@@ -59,6 +59,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncQue
   using O = Ops<T>;
   using Frag = typename O::Frag;
   constexpr int DV = D * M, DC = D / O::kDims, VC = DV / O::kDims, ND = D / 16, NKB = 4 / O::kSub;
+    constexpr bool TILE_SUMS = NT == 0 && std::is_same<T, Split>::value;  // as in the forward pass
   constexpr int PK = O::row_pitch(D), PV = O::row_pitch(DV), TK = O::kParts * kTile * PK;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   typename O::Lds* k_lds = reinterpret_cast<typename O::Lds*>(smem);
@@ -202,7 +203,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncQue
     for (int m = 0; m < M; ++m)
 #pragma unroll
       for (int s = 0; s < QS; ++s) {
-        base[m][s] = top[m][s] * sl2;
+        base[m][s] = Exponent::base_of(top[m][s], sl2);
         far_any |= Exponent::far(base[m][s]);
       }
     const bool far = __any(far_any);
@@ -227,6 +228,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncQue
       }
       if (walk.sample < b_last) fetch(walk);
       float4v ds[M][QS][4];  // without the row's 1 / sum, which joins at the end of the row
+      float4v dq_tile[M][QS][ND];  // TILE_SUMS
       int side[QS];
       if (busy) {
 #pragma unroll
@@ -274,7 +276,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncQue
               const int kt = kb * O::kSub + u;
               float4v dp[QS];
 #pragma unroll
-              for (int s = 0; s < QS; ++s) dp[s] = float4v{-delta[0][s], -delta[0][s], -delta[0][s], -delta[0][s]};  // dP - delta of the first map
+              for (int s = 0; s < QS; ++s) dp[s] = float4v{0.f, 0.f, 0.f, 0.f};  // not -delta: every partial sum would be rounded at its size
 #pragma unroll
               for (int c = 0; c < VC; ++c) {
                 const Frag vf = O::row_frag(v_lds, PV, kt * 16 + l15, c, q4);
@@ -291,7 +293,6 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncQue
                 }
 #pragma unroll
                 for (int s = 0; s < QS; ++s) {
-                  const float shift = m == 0 ? 0.f : delta[0][s] - delta[m][s];
                   float4v x = ds[m][s][kt];
                   if (!PLAIN && far) {
 #pragma unroll
@@ -301,7 +302,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncQue
                     for (int j = 0; j < 4; ++j) x[j] = Exponent::near_(x[j], base[m][s], sl2);
                   }
 #pragma unroll
-                  for (int j = 0; j < 4; ++j) x[j] *= m == 0 ? dp[s][j] : dp[s][j] + shift;
+                  for (int j = 0; j < 4; ++j) x[j] *= dp[s][j] - delta[m][s];
                   if (!PLAIN && word != ~0ULL) {
                     const unsigned bits = (unsigned)(word >> (kt * 16 + q4 * 4));
 #pragma unroll
@@ -320,13 +321,24 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncQue
               for (int n = 0; n < ND; ++n) {
                 const Frag kf = O::tr_frag(k_lds + m * TK, PK, kb, n, l15, q4);
 #pragma unroll
-                for (int s = 0; s < QS; ++s) dq[m][s][n] = O::mma(kf, sf[s], dq[m][s][n]);
+                for (int s = 0; s < QS; ++s) {
+                  if constexpr (TILE_SUMS) dq_tile[m][s][n] = O::mma(kf, sf[s], kb == 0 ? float4v{0.f, 0.f, 0.f, 0.f} : dq_tile[m][s][n]);
+                  else dq[m][s][n] = O::mma(kf, sf[s], dq[m][s][n]);
+                }
               }
             }
           }
         };
         if (far || word != ~0ULL) scores(std::false_type{});
         else scores(std::true_type{});
+        if constexpr (TILE_SUMS) {
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int s = 0; s < QS; ++s)
+#pragma unroll
+              for (int n = 0; n < ND; ++n) dq[m][s][n] += dq_tile[m][s][n];
+        }
         if constexpr (NT > 0) {
 #pragma unroll
           for (int m = 0; m < M; ++m)
@@ -459,6 +471,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, Ops<T>::kBf16, kEncKey
   using O = Ops<T>;
   using Frag = typename O::Frag;
   constexpr int DV = D * M, DC = D / O::kDims, VC = DV / O::kDims, ND = D / 16, NV = DV / 16, NKB = 4 / O::kSub;
+    constexpr bool TILE_SUMS = NT == 0 && std::is_same<T, Split>::value;  // as in the forward pass
   constexpr int PQ = O::row_pitch(D), PG = O::row_pitch(DV), TQ = O::kParts * kTile * PQ;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   typename O::Lds* q_lds = reinterpret_cast<typename O::Lds*>(smem);
@@ -570,7 +583,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, Ops<T>::kBf16, kEncKey
       if (tid < M * kTile) {
         top_lds[tid] = stat.x;
         inv_lds[tid] = stat.y;
-        const bool far = __any(Exponent::far(stat.x * sl2));
+        const bool far = __any(Exponent::far(Exponent::base_of(stat.x, sl2)));
         if (lane == 0) far_lds[wave] = far;
       } else if (tid < 2 * M * kTile) {
         delta_lds[tid - M * kTile] = stat.x;
@@ -595,10 +608,9 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, Ops<T>::kBf16, kEncKey
 #pragma unroll
         for (int u = 0; u < O::kSub; ++u) {
           const int qt = kb * O::kSub + u;
-          const float4v del4 = *reinterpret_cast<const float4v*>(delta_lds + qt * 16 + q4 * 4);
           float4v dp[KS];
 #pragma unroll
-          for (int s = 0; s < KS; ++s) dp[s] = -del4;  // dP - delta of the first map
+          for (int s = 0; s < KS; ++s) dp[s] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < VC; ++c) {
             const Frag gf = O::row_frag(g_lds, PG, qt * 16 + l15, c, q4);
@@ -637,9 +649,8 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, Ops<T>::kBf16, kEncKey
             }
             const float4v top4 = *reinterpret_cast<const float4v*>(top_lds + m * kTile + qt * 16 + q4 * 4);
             const float4v inv4 = *reinterpret_cast<const float4v*>(inv_lds + m * kTile + qt * 16 + q4 * 4);
-            float4v shift = {0.f, 0.f, 0.f, 0.f};
-            if (m > 0) shift = del4 - *reinterpret_cast<const float4v*>(delta_lds + m * kTile + qt * 16 + q4 * 4);
-            const float4v base4 = top4 * sl2;
+            const float4v del4 = *reinterpret_cast<const float4v*>(delta_lds + m * kTile + qt * 16 + q4 * 4);
+            const float4v base4 = {Exponent::base_of(top4[0], sl2), Exponent::base_of(top4[1], sl2), Exponent::base_of(top4[2], sl2), Exponent::base_of(top4[3], sl2)};
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
               // a masked key's column is garbage of its own (its rows were read as zeros) and is zeroed when written
@@ -655,11 +666,11 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, Ops<T>::kBf16, kEncKey
                 const float p = x[s][j] * inv4[j];
                 if (m == 0) {
                   pmix[s][u][j] = p;
-                  ds[m][s][u][j] = p * dp[s][j];
+                  ds[m][s][u][j] = p * (dp[s][j] - del4[j]);
                 } else {
                   const float w = -lam * p;
                   pmix[s][u][j] += w;
-                  ds[m][s][u][j] = w * (dp[s][j] + shift[j]);
+                  ds[m][s][u][j] = w * (dp[s][j] - del4[j]);
                 }
               }
             }
@@ -672,7 +683,10 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, Ops<T>::kBf16, kEncKey
         for (int n = 0; n < NV; ++n) {
           const Frag gf = O::tr_frag(g_lds, PG, kb, n, l15, q4);
 #pragma unroll
-          for (int s = 0; s < KS; ++s) dv[s][n] = O::mma(gf, pf[s], dv[s][n]);
+          for (int s = 0; s < KS; ++s) {
+            if constexpr (TILE_SUMS) dv[s][n] += O::mma(gf, pf[s], float4v{0.f, 0.f, 0.f, 0.f});
+            else dv[s][n] = O::mma(gf, pf[s], dv[s][n]);
+          }
         }
 #pragma unroll
         for (int m = 0; m < M; ++m) {
@@ -683,7 +697,10 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, Ops<T>::kBf16, kEncKey
           for (int n = 0; n < ND; ++n) {
             const Frag qf = O::tr_frag(q_lds + m * TQ, PQ, kb, n, l15, q4);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) dk[m][s][n] = O::mma(qf, sf[s], dk[m][s][n]);
+            for (int s = 0; s < KS; ++s) {
+              if constexpr (TILE_SUMS) dk[m][s][n] += O::mma(qf, sf[s], float4v{0.f, 0.f, 0.f, 0.f});
+              else dk[m][s][n] = O::mma(qf, sf[s], dk[m][s][n]);
+            }
           }
         }
       };

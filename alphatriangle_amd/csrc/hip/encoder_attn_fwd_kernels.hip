@@ -20,6 +20,9 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncFor
   using Frag = typename O::Frag;
   constexpr int DV = D * M, DC = D / O::kDims, NV = DV / 16, NKB = 4 / O::kSub;
   constexpr int PK = O::row_pitch(D), PV = O::tr_pitch(DV), TK = O::kParts * kTile * PK;
+  // A sum per tile, joined to the long one together with the change of maximum: one rounding per 64 keys where the products would
+  // take twelve (2000 tokens: output 5e-7 off without, 2e-7 with; 2 to 5 % of the time).
+  constexpr bool TILE_SUMS = NT == 0 && std::is_same<T, Split>::value;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   typename O::Lds* k_lds = reinterpret_cast<typename O::Lds*>(smem);
   typename O::Lds* v_lds = k_lds + M * TK;
@@ -133,6 +136,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncFor
       // Few and wide basic blocks per map: the start of the scores, all products, one branch each for masked keys, far rows and
       // new maxima.
       float4v st[M][QS][4];
+      float fade[M][QS];
 #pragma unroll
       for (int m = 0; m < M; ++m) {
 #pragma unroll
@@ -182,7 +186,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncFor
               for (int j = 0; j < 4; ++j) st[m][s][kt][j] = (bits >> j) & 1 ? st[m][s][kt][j] : -INFINITY;
           }
         }
-        float from[QS], fade[QS];
+        float from[QS];
         bool far = false;
 #pragma unroll
         for (int s = 0; s < QS; ++s) {
@@ -193,14 +197,14 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncFor
             for (int j = 0; j < 4; ++j) top = fmaxf(top, st[m][s][kt][j]);
           top = quad_row_max(top);
           from[s] = top == -INFINITY ? 0.f : top;  // nothing seen yet: exp2(-inf - 0) = 0, never inf - inf
-          fade[s] = run_max[m][s];
+          fade[m][s] = run_max[m][s];
           run_max[m][s] = top;
-          far |= Exponent::far(from[s] * sl2);
+          far |= Exponent::far(Exponent::base_of(from[s], sl2));
         }
         if (__any(far)) {
 #pragma unroll
           for (int s = 0; s < QS; ++s) {
-            fade[s] = Exponent::far_(fade[s], from[s], sl2);
+            fade[m][s] = Exponent::far_(fade[m][s], from[s], sl2);
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
@@ -209,8 +213,8 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncFor
         } else {
 #pragma unroll
           for (int s = 0; s < QS; ++s) {
-            const float base = from[s] * sl2;
-            fade[s] = __builtin_amdgcn_exp2f(fade[s] * sl2 - base);
+            const float base = Exponent::base_of(from[s], sl2);
+            fade[m][s] = __builtin_amdgcn_exp2f(Exponent::base_of(fade[m][s], sl2) - base);
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
@@ -225,39 +229,75 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncFor
           for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
             for (int j = 0; j < 4; ++j) sum += st[m][s][kt][j];
-          run_sum[m][s] = fmaf(run_sum[m][s], fade[s], sum);
-          faded |= fade[s] != 1.0f;
+          run_sum[m][s] = fmaf(run_sum[m][s], fade[m][s], sum);
+          faded |= fade[m][s] != 1.0f;
         }
-        if (__any(faded)) {
+        if (!TILE_SUMS && __any(faded)) {
 #pragma unroll
           for (int s = 0; s < QS; ++s)
 #pragma unroll
             for (int n = 0; n < NV; ++n)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) o[m][s][n][j] *= fade[s];
+              for (int j = 0; j < 4; ++j) o[m][s][n][j] *= fade[m][s];
         }
       }
+      if constexpr (TILE_SUMS) {
+        Frag pf[NKB][M][QS][PL];
 #pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) {
-        Frag pf[M][QS][PL];
-#pragma unroll
-        for (int m = 0; m < M; ++m)
-#pragma unroll
-          for (int s = 0; s < QS; ++s)
-#pragma unroll
-            for (int p = 0; p < PL; ++p) {
-              pf[m][s][p] = O::acc_frag(&st[m][s][kb * O::kSub]);
-              if (p + 1 < PL) O::take(&st[m][s][kb * O::kSub], pf[m][s][p]);
-            }
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-          const Frag vf = O::tr_frag(v_lds, PV, kb, n, l15, q4);
+        for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
           for (int m = 0; m < M; ++m)
 #pragma unroll
             for (int s = 0; s < QS; ++s)
 #pragma unroll
-              for (int p = PL - 1; p >= 0; --p) o[m][s][n] = O::mma(vf, pf[m][s][p], o[m][s][n]);
+              for (int p = 0; p < PL; ++p) {
+                pf[kb][m][s][p] = O::acc_frag(&st[m][s][kb * O::kSub]);
+                if (p + 1 < PL) O::take(&st[m][s][kb * O::kSub], pf[kb][m][s][p]);
+              }
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          float4v sum[M][QS];
+#pragma unroll
+          for (int kb = 0; kb < NKB; ++kb) {
+            const Frag vf = O::tr_frag(v_lds, PV, kb, n, l15, q4);
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+#pragma unroll
+              for (int s = 0; s < QS; ++s)
+#pragma unroll
+                for (int p = PL - 1; p >= 0; --p)
+                  sum[m][s] = O::mma(vf, pf[kb][m][s][p], kb == 0 && p == PL - 1 ? float4v{0.f, 0.f, 0.f, 0.f} : sum[m][s]);
+          }
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int s = 0; s < QS; ++s)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) o[m][s][n][j] = fmaf(o[m][s][n][j], fade[m][s], sum[m][s][j]);
+        }
+      } else {
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) {
+          Frag pf[M][QS][PL];
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int s = 0; s < QS; ++s)
+#pragma unroll
+              for (int p = 0; p < PL; ++p) {
+                pf[m][s][p] = O::acc_frag(&st[m][s][kb * O::kSub]);
+                if (p + 1 < PL) O::take(&st[m][s][kb * O::kSub], pf[m][s][p]);
+              }
+#pragma unroll
+          for (int n = 0; n < NV; ++n) {
+            const Frag vf = O::tr_frag(v_lds, PV, kb, n, l15, q4);
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+#pragma unroll
+              for (int s = 0; s < QS; ++s)
+#pragma unroll
+                for (int p = PL - 1; p >= 0; --p) o[m][s][n] = O::mma(vf, pf[m][s][p], o[m][s][n]);
+          }
         }
       }
     };
@@ -346,13 +386,13 @@ __global__ __launch_bounds__(256) void enc_attn_join_kernel(EncAttnArgs a) {
 #pragma unroll 4
     for (int s = share; s < a.splits; s += SHARES) top = fmaxf(top, ml[2 * s * step]);
     if constexpr (SHARES == 4) top = quad_row_max(top);
-    const float from = top == -INFINITY ? 0.f : top, base = from * sl2;
+    const float from = top == -INFINITY ? 0.f : top, base = Exponent::base_of(from, sl2);
     float sum = 0.f;
     float4v acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int s = share; s < a.splits; s += SHARES) {
       const float t = ml[2 * s * step];
-      const float w = Exponent::far(base) ? Exponent::far_(t, from, sl2) : __builtin_amdgcn_exp2f(t * sl2 - base);
+      const float w = Exponent::far(base) ? Exponent::far_(t, from, sl2) : __builtin_amdgcn_exp2f(Exponent::base_of(t, sl2) - base);
       const float4v p = *reinterpret_cast<const float4v*>(po + s * step * a.DV);
       sum = fmaf(ml[2 * s * step + 1], w, sum);
 #pragma unroll
@@ -407,8 +447,7 @@ int launch_fwd(const EncAttnArgs& a, hipStream_t stream) {
   return launch_fwd_planes<T, D, M, QS, BIAS, 1, NT>(a, stream);
 }
 
-// T: bf16 rows, or Split; W: the widest fp32 heads, whose staged parts would leave one workgroup per CU (128-wide: 336 us in
-// parts, 320 us with the fp32 instruction) or fill the LDS (two 64-wide maps).
+// T: bf16 rows, or Split; W: fp32 rows with the fp32 matrix instruction for two 64-wide maps, whose parts would fill the LDS.
 template <typename T, typename W>
 int dispatch_fwd(const EncAttnArgs& a, hipStream_t stream) {
   const int w = enc_width(a.D), nt = enc_board_tiles(a.table ? a.W : 0, a.Lk, a.D, a.M);
@@ -419,7 +458,7 @@ int dispatch_fwd(const EncAttnArgs& a, hipStream_t stream) {
     if (nt == 4) return launch_fwd<T, 32, 1, 1, true, 4>(a, stream);
     if (w == 32) return two ? launch_fwd<T, 32, 1, 2, true>(a, stream) : launch_fwd<T, 32, 1, 1, true>(a, stream);
     if (w == 64) return two ? launch_fwd<T, 64, 1, 2, true>(a, stream) : launch_fwd<T, 64, 1, 1, true>(a, stream);
-    return launch_fwd<W, 128, 1, 1, true>(a, stream);
+    return launch_fwd<T, 128, 1, 1, true>(a, stream);
   }
   if (nt == 2) return launch_fwd<T, 32, 2, 1, true, 2>(a, stream);
   if (w == 32) return a.table ? launch_fwd<T, 32, 2, 1, true>(a, stream) : launch_fwd<T, 32, 2, 1, false>(a, stream);
