@@ -70,16 +70,24 @@ struct Ops<unsigned short> {
   static __device__ __forceinline__ float4v mma(const Frag& a, const Frag& b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ float4v mma_mirrored(const Frag& a, const Frag& b, float4v c) { return mma(a, b, c); }
+  // rows of 32-bit values against bf16 ones: three parts carry all of them, and a row of bf16 values gives the bits of mma
+  static __device__ __forceinline__ float4v mma_rows32(const float* row, const Frag& b, float4v c) {
+    float4v s[2] = {*reinterpret_cast<const float4v*>(row), *reinterpret_cast<const float4v*>(row + 4)};
+    Frag part[3];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      part[p] = acc_frag(s);
+      if (p < 2) take(s, part[p]);
+    }
+#pragma unroll
+    for (int p = 2; p >= 0; --p) c = mma(part[p], b, c);
+    return c;
+  }
   // s -= value(f): what the next of several fragments of the same values has to carry.
   static __device__ __forceinline__ void take(float4v* s, const Frag& f) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[e >> 2][e & 3] -= bf16_to_float((unsigned short)f[e]);
-  }
-  static __device__ __forceinline__ float dot(const Frag& a, const float* o) {
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s = fmaf(bf16_to_float((unsigned short)a[e]), o[e], s);
-    return s;
   }
   static __device__ __forceinline__ void negate(Frag& f, bool on) {
     uint4v u = __builtin_bit_cast(uint4v, f);
@@ -123,12 +131,11 @@ struct Ops<float> {
     for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
     return c;
   }
+  static __device__ __forceinline__ float4v mma_mirrored(const Frag& a, const Frag& b, float4v c) { return mma(a, b, c); }
+  static __device__ __forceinline__ float4v mma_rows32(const float* row, const Frag& b, float4v c) { return mma(from_memory(row), b, c); }
   static __device__ __forceinline__ void negate(Frag& f, bool on) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = on ? -f[i] : f[i];
-  }
-  static __device__ __forceinline__ float dot(const Frag& a, const float* o) {
-    return fmaf(a[0], o[0], fmaf(a[1], o[1], fmaf(a[2], o[2], a[3] * o[3])));
   }
   static __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
     *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
@@ -199,15 +206,15 @@ struct Ops<Split> {
     c = One::mma(a.part[0], b.part[1], c);
     return One::mma(a.part[0], b.part[0], c);
   }
-  static __device__ __forceinline__ float dot(const Frag& a, const float* o) {
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = (bf16_to_float((unsigned short)a.part[0][e]) + bf16_to_float((unsigned short)a.part[1][e])) + bf16_to_float((unsigned short)a.part[2][e]);
-      s = fmaf(x, o[e], s);
-    }
-    return s;
+  static __device__ __forceinline__ float4v mma_mirrored(const Frag& a, const Frag& b, float4v c) {  // the bits of mma(b, a)
+    c = One::mma(a.part[0], b.part[2], c);
+    c = One::mma(a.part[2], b.part[0], c);
+    c = One::mma(a.part[1], b.part[1], c);
+    c = One::mma(a.part[0], b.part[1], c);
+    c = One::mma(a.part[1], b.part[0], c);
+    return One::mma(a.part[0], b.part[0], c);
   }
+  static __device__ __forceinline__ float4v mma_rows32(const float* row, const Frag& b, float4v c) { return mma(from_memory(row), b, c); }
   static __device__ __forceinline__ void negate(Frag& f, bool on) {
 #pragma unroll
     for (int p = 0; p < 3; ++p) One::negate(f.part[p], on);

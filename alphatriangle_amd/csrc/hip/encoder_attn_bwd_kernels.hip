@@ -14,6 +14,7 @@ using namespace atrihip;
 
 namespace {
 
+__device__ const float kZeroRow[8] __attribute__((aligned(16))) = {};  // read in place of rows and columns that are not there
 constexpr int kDsPitch = kTile + 4;  // row pitch of a wave's 16 x 64 tile of dS on its way to the diagonal sums
 
 __device__ __forceinline__ void wave_lds_fence() {  // orders a wave's own LDS writes before its other lanes' reads
@@ -54,6 +55,8 @@ __device__ __forceinline__ void add_tile(const EncAttnArgs& a, float* sums, cons
 }
 
 // One 4-wave workgroup per (head, 64 QS queries, key range) and q_chunk samples, one after the other.
+// Measured (sizes as in the forward pass): boards of 120 cells, fp32 44 us; 252 cells, bf16 63 us; 4095 tokens, bf16 209 us; bound
+// like the forward pass, with five LDS reads and 36 vector instructions per pair and lane in the fp32 form.
 template <typename T, int D, int M, int QS, bool BIAS, int NT>
 __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncQueries)) void enc_attn_bwd_q_kernel(EncAttnArgs a) {
   using O = Ops<T>;
@@ -149,34 +152,6 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncQue
       const int query = q_first + s * 16 + l15;
       const bool valid = query < a.Lq;
       load_rows<T, VC>(dof[s], reinterpret_cast<const typename O::Mem*>(a.dout) + b * a.gs[0] + (long long)query * a.gs[1] + h * a.gs[2], valid, a.DV, q4);
-#pragma unroll
-      for (int m = 0; m < M; ++m) {
-        load_rows<T, DC>(qf[m][s], reinterpret_cast<const typename O::Mem*>(a.q) + b * a.qs[0] + (long long)query * a.qs[1] + (long long)(h * M + m) * a.qs[2], valid,
-                         a.D, q4);
-        float2 st = make_float2(INFINITY, 0.f);
-        if (valid) st = *reinterpret_cast<const float2*>(a.stat + 2 * (m * rows + row0 + query));
-        top[m][s] = st.x;
-        inv[m][s] = st.y;
-        const float* o = a.o32 + b * a.o32s[0] + (long long)query * a.o32s[1] + h * a.o32s[2] + m * a.o32s[3];
-        float dot = 0.f;
-#pragma unroll
-        for (int c = 0; c < VC; ++c) {
-          const int col = c * O::kDims + q4 * O::kLane;
-          if (!valid || col >= a.DV) continue;
-          float v[O::kLane];
-#pragma unroll
-          for (int e = 0; e < O::kLane; e += 4) {
-            const float4 u = *reinterpret_cast<const float4*>(o + col + e);
-            v[e] = u.x; v[e + 1] = u.y; v[e + 2] = u.z; v[e + 3] = u.w;
-          }
-          dot += O::dot(dof[s][c], v);
-        }
-        delta[m][s] = quad_row_sum(dot);
-        if (valid && q4 == 0 && split == 0) {
-          a.delta[m * rows + row0 + query] = delta[m][s];
-          if (M == 2 && m == 1) delta2_sum += delta[m][s];
-        }
-      }
       // The matrix instructions round sums down by a little (0.01 to 0.03 units in the last place on average), which adds up over
       // the pairs that share a table entry: every second row takes the other sign, from dO and delta to the 1 / sum that its
       // results meet (one sequence of 3000 tokens, error of the far buckets: 1e-5 without).
@@ -185,8 +160,28 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncQue
       for (int c = 0; c < VC; ++c) O::negate(dof[s][c], other);
 #pragma unroll
       for (int m = 0; m < M; ++m) {
-        delta[m][s] = other ? -delta[m][s] : delta[m][s];
-        inv[m][s] = other ? -inv[m][s] : inv[m][s];
+        load_rows<T, DC>(qf[m][s], reinterpret_cast<const typename O::Mem*>(a.q) + b * a.qs[0] + (long long)query * a.qs[1] + (long long)(h * M + m) * a.qs[2], valid,
+                         a.D, q4);
+        float2 st = make_float2(INFINITY, 0.f);
+        if (valid) st = *reinterpret_cast<const float2*>(a.stat + 2 * (m * rows + row0 + query));
+        top[m][s] = st.x;
+        inv[m][s] = other ? -st.y : st.y;
+        const float* o = a.o32 + b * a.o32s[0] + (long long)query * a.o32s[1] + h * a.o32s[2] + m * a.o32s[3];
+        // delta = dO . o by the instructions that make dP (o rows as the other operand, the diagonal of the product): where a row
+        // has a single key, o is v and dP - delta is what the rounding of its probability leaves.
+        float4v prod = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < VC; ++c) {
+          const int col = c * O::kDims + q4 * O::kLane;
+          prod = O::mma_rows32(valid && col < a.DV ? o + col : kZeroRow, dof[s][c], prod);
+        }
+        const float mine = l15 & 2 ? (l15 & 1 ? prod[3] : prod[2]) : (l15 & 1 ? prod[1] : prod[0]);
+        delta[m][s] = quad_row_sum(q4 == l15 >> 2 ? mine : 0.f);
+        if (valid && q4 == 0 && split == 0) {
+          const float signless = other ? -delta[m][s] : delta[m][s];
+          a.delta[m * rows + row0 + query] = signless;
+          if (M == 2 && m == 1) delta2_sum += signless;
+        }
       }
     }
     float4v dq[M][QS][ND];
@@ -466,6 +461,8 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncQue
 
 // One 4-wave workgroup per (key / value head, 64 KS keys, query range) and k_chunk samples; a wave owns 16 KS keys and walks the
 // query tiles of every query head that shares them.
+// Measured (same sizes): 53 us, 72 us and 232 us.  One pass over the pairs for all gradients would save two of seven products, but
+// needs dQ summed across workgroups (or a board's dS through LDS, as many reads as the products it saves).
 template <typename T, int D, int M, int KS, bool BIAS, int NT>
 __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, Ops<T>::kBf16, kEncKeys)) void enc_attn_bwd_k_kernel(EncAttnArgs a) {
   using O = Ops<T>;
@@ -615,7 +612,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, Ops<T>::kBf16, kEncKey
           for (int c = 0; c < VC; ++c) {
             const Frag gf = O::row_frag(g_lds, PG, qt * 16 + l15, c, q4);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) dp[s] = O::mma(gf, vf[s][c], dp[s]);
+            for (int s = 0; s < KS; ++s) dp[s] = O::mma_mirrored(gf, vf[s][c], dp[s]);
           }
           int4 p4 = make_int4(0, 0, 0, 0);
           if constexpr (BIAS && NT == 0) p4 = *reinterpret_cast<const int4*>(pos_lds + qt * 16 + q4 * 4);

@@ -64,8 +64,8 @@ constexpr int enc_columns_of(int D, int M, int nt, bool bf16, int pass) {
   // fp32 operands take three times the registers: one where two spill (two 2048-token sequences of eight 64-wide heads, backward:
   // 574 us with two, 408 us with one; 32-wide heads: 258 and 316 us)
   if (!bf16 && D > 32 && pass != kEncForward) return 1;
-  // two: every staged fragment feeds two products; one where bias and sums of dS share the registers (256 boards of 120 cells,
-  // fp32, query-owned pass: 68 us with two, 51 us with one; forward and key-owned pass: no difference within 3 %)
+  // two: every staged fragment feeds two products (256 boards of 120 cells, fp32, forward: 33 us with one, 29 us with two); one
+  // where bias and sums of dS share the registers (query-owned pass, with the fp32 instruction: 68 us with two, 51 us with one)
   return nt == 2 && pass == kEncQueries ? 1 : 2;
 }
 inline int enc_columns(int W, int L, int Lk, int D, int M, bool bf16, int pass) {
