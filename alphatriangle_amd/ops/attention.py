@@ -6,7 +6,8 @@
 (:func:`attention_reference`) for host tensors.  Both are differentiable once in every tensor argument.
 
 * Types: fp32 or bf16 ``q`` / ``k`` / ``v`` of one type; ``table`` and ``lam`` in any floating type (used in fp32, their gradients
-  are summed in at least 32 bits).  fp32 products are true fp32 products.
+  are summed in at least 32 bits).  fp32 products carry all 24 bits of their operands, most of them as three bf16 parts; in fp32 an
+  infinity (or a value above 3.38e38) in a row that takes part makes the results it reaches NaN.
 * Layouts: ``[batch, tokens, heads, dim]`` with any strides; a contiguous last dimension with 16-byte aligned rows is read in
   place, anything else is copied first.  Outputs and gradients follow the token / batch order of the tensor they belong to.
 * Shared heads: ``k`` and ``v`` may have fewer heads than ``q`` (a divisor); their gradients are summed over the group.
@@ -43,6 +44,26 @@ class RelativeBuckets:
     lut: torch.Tensor
     order: torch.Tensor
     start: torch.Tensor
+
+    def __post_init__(self) -> None:
+        """The kernels index with these tables: refuses what would lead them outside."""
+        n = 2 * self.radius + 1
+        if not 0 <= self.radius <= MAX_RADIUS or self.num_buckets < 1:
+            raise ValueError(f"RelativeBuckets: a radius of 0 to {MAX_RADIUS} and a bucket, got {self.radius} and {self.num_buckets}")
+        if (self.rows, self.cols) != (0, 0) and (self.rows < 1 or self.cols < 1 or self.radius != (self.rows - 1) * (2 * self.cols - 1) + self.cols - 1):
+            raise ValueError(f"RelativeBuckets: radius {self.radius} is not that of a {self.rows} x {self.cols} board")
+        tables = (self.lut, self.order, self.start)
+        if [tuple(t.shape) for t in tables] != [(n,), (n,), (self.num_buckets + 1,)] or any(
+            t.dtype != torch.int32 or not t.is_contiguous() or t.device != self.lut.device for t in tables
+        ):
+            raise ValueError(f"RelativeBuckets: lut and order are contiguous int32 [{n}], start [{self.num_buckets + 1}], on one device")
+        lut, order, start = (t.cpu().long() for t in tables)
+        if int(lut.min()) < 0 or int(lut.max()) >= self.num_buckets or not torch.equal(order.sort().values, torch.arange(n)):
+            raise ValueError("RelativeBuckets: lut names buckets, order every difference once")
+        if not torch.equal(start[1:], torch.bincount(lut, minlength=self.num_buckets).cumsum(0)) or int(start[0]) != 0 or not torch.equal(
+            lut[order], lut.sort().values
+        ):
+            raise ValueError("RelativeBuckets: order lists the differences bucket by bucket, start where each bucket begins")
 
     @classmethod
     def _make(cls, lut: torch.Tensor, num_buckets: int, radius: int, rows: int, cols: int, device: torch.device | str | None) -> "RelativeBuckets":

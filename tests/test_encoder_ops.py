@@ -139,3 +139,20 @@ def test_refusals():
     w = torch.randn(1, 2, 2, 72)
     with pytest.raises(ValueError):
         differential_attention(w, w, torch.randn(1, 2, 1, 144), torch.rand(1))
+
+
+def test_plans_that_would_lead_outside_are_refused():
+    good = RelativeBuckets.log(8, 6)
+    fields = dict(num_buckets=8, radius=6, rows=0, cols=0, lut=good.lut, order=good.order, start=good.start)
+    RelativeBuckets(**fields)
+    low, high = good.lut.clone(), good.lut.clone()
+    low[0], high[3] = -1, 8
+    twice = good.order.clone()
+    twice[0] = twice[1]
+    for change in (dict(radius=7), dict(radius=-1), dict(radius=1 << 20), dict(num_buckets=9), dict(num_buckets=0), dict(cols=5), dict(rows=2, cols=3),
+                   dict(lut=low), dict(lut=high), dict(order=twice), dict(order=good.order.flip(0).contiguous()), dict(lut=good.lut.long()),
+                   dict(start=good.start + 1), dict(lut=torch.stack([good.lut, good.lut], 1)[:, 0])):
+        with pytest.raises(ValueError, match="RelativeBuckets"):
+            RelativeBuckets(**{**fields, **change})
+    board = RelativeBuckets.board(3, 4)
+    assert board.radius == 2 * 7 + 3 and board.num_buckets == 5 * 7

@@ -488,3 +488,67 @@ def test_half_of_a_batch_equals_the_whole():
         whole = _call(inp, p, None, 0)
         part = {n: (x[390:] if n in ("q", "k", "v") else x) for n, x in inp.items()}
         assert torch.equal(_call(part, p, None, 0), whole[390:])
+
+
+def test_long_rows_stay_accurate():
+    """fp32 against 64 bits over 32 tiles with few workgroups to split them.  A probability is off by two roundings of the exponential
+    and that of its score (below 8 in units of its rounding in the root mean square); sums per tile add half a rounding times
+    the root of 32: 8 u in all, and nothing may grow with the number of maxima a row runs through."""
+    p = _plan(128)
+    inp = _inputs(torch.float32, 1, 4, 2000, 2000, 8, 8, 32, p)
+    names = ("q", "k", "v", "table")
+    t = {**inp, **{n: inp[n].clone().requires_grad_(True) for n in names}}
+    out = _call(t, p, None, 0)
+    got = torch.autograd.grad(out, [t[n] for n in names], inp["dout"])
+    from alphatriangle_amd.ops.attention import attention_reference
+
+    w = {n: inp[n].double().requires_grad_(True) for n in names}
+    ref = attention_reference(w["q"], w["k"], w["v"], None, w["table"], p, None, 32**-0.5, 0)
+    want = torch.autograd.grad(ref, [w[n] for n in names], inp["dout"].double())
+    assert _rel(out, ref) <= 8 * U32
+    for n, g, e in zip(names[:3], got, want):
+        assert _rel(g, e) <= 8 * U32, n
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_table_gradient_adds_up_to_zero(dtype):
+    """Over all buckets a head's table gradient is zero by definition (softmax gradients of a row add up to zero).  What is left are
+    roundings of dP - delta, |dP| about sqrt(64) = 8: one per row that does not average out in it, of random sign, over 3000 rows: 8 u sqrt(3000),
+    twice that allowed.  A rounding that always goes one way would leave 3000 of them."""
+    p = _plan(128)
+    inp = _inputs(dtype, 1, 1, 3000, 3000, 8, 2, 64, p)
+    table = inp["table"].clone().requires_grad_(True)
+    g = torch.autograd.grad(_call({**inp, "table": table}, p, None, 0), table, inp["dout"])[0]
+    assert float(g.double().sum(0).abs().max()) <= 2 * 8 * U32 * math.sqrt(3000)
+
+
+def test_rows_with_a_single_key():
+    """Their score gradients are zero by definition: dP - delta leaves roundings of products of the size of |dO| |v| only."""
+    p = _plan(16)
+    for dtype in BOTH:
+        for maps in (1, 2):
+            inp = _inputs(dtype, maps, 64, 5, 3, 2, 2, 64, p)
+            mask = torch.zeros(64, 3, dtype=torch.bool, device="cuda")
+            mask[torch.arange(64), torch.arange(64) % 3] = True
+            t = {**inp, **{n: inp[n].clone().requires_grad_(True) for n in ("q", "k", "table")}}
+            grads = torch.autograd.grad(_call(t, p, mask, 0), [t[n] for n in ("q", "k", "table")], inp["dout"])
+            # one rounding of the probability, and of o, times |dP| <= |dO| |v|, times |k| scale or |q| scale, over the five queries
+            size = float(inp["dout"].float().norm(dim=-1).max() * inp["v"].float().norm(dim=-1).max())
+            side = float(torch.maximum(inp["q"].float().norm(dim=-1).max(), inp["k"].float().norm(dim=-1).max())) * 64**-0.5
+            for g in grads[:2]:
+                assert float(g.float().abs().max()) <= 8 * U32 * size * side * 5
+            assert float(grads[2].abs().max()) <= 8 * U32 * size * 64 * 5
+
+
+def test_broadcast_keys_add_their_gradients():
+    p = _plan(24)
+    inp = _inputs(torch.float32, 1, 3, 40, 50, 2, 2, 32, p)
+    one = {n: inp[n][:1].clone().requires_grad_(True) for n in ("k", "v")}
+    out = _call({**inp, **{n: x.expand(3, -1, -1, -1) for n, x in one.items()}}, p, None, 0)
+    got = torch.autograd.grad(out, list(one.values()), inp["dout"])
+    full = {n: inp[n][:1].repeat(3, 1, 1, 1).requires_grad_(True) for n in ("k", "v")}
+    same = _call({**inp, **full}, p, None, 0)
+    want = torch.autograd.grad(same, list(full.values()), inp["dout"])
+    assert torch.equal(out, same)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y.sum(0, keepdim=True))
