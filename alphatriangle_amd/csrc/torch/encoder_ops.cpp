@@ -110,7 +110,7 @@ void plan(int64_t samples, int64_t groups, int64_t steps, int64_t resident, int6
   const double join = partial < (1 << 18) ? 0.1 : 0.5;
   const auto cost = [&](int64_t s) { return static_cast<double>(up(n * s, resident) * (up(steps, s) + 2)) + (s > 1 ? 2.0 + join * static_cast<double>(s) : 0.0); };
   double best = cost(1);
-  for (int64_t s = 2; s <= std::min<int64_t>(steps / 2, 128); ++s)
+  for (int64_t s = 2; s <= std::min<int64_t>(steps, 128); ++s)
     if (cost(s) < 0.95 * best) best = cost(s), splits = static_cast<int>(s);
 }
 
