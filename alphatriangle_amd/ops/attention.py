@@ -18,6 +18,7 @@
 
 from __future__ import annotations
 
+import copy
 import math
 from collections.abc import Callable
 from dataclasses import dataclass
@@ -68,12 +69,12 @@ class RelativeBuckets:
     @classmethod
     def _make(cls, lut: torch.Tensor, num_buckets: int, radius: int, rows: int, cols: int, device: torch.device | str | None) -> "RelativeBuckets":
         n = lut.numel()
-        tables = torch.zeros(2 * n + num_buckets + 1, dtype=torch.int32)  # one upload
+        tables = torch.zeros(2 * n + num_buckets + 1, dtype=torch.int32)
         tables[:n] = lut
         tables[n : 2 * n] = torch.argsort(lut, stable=True)
         tables[2 * n + 1 :] = torch.bincount(lut, minlength=num_buckets).cumsum(0)
-        tables = tables.to("cpu" if device is None else device)
-        return cls(num_buckets, radius, rows, cols, tables[:n], tables[n : 2 * n], tables[2 * n :])
+        plan = cls(num_buckets, radius, rows, cols, tables[:n], tables[n : 2 * n], tables[2 * n :])
+        return plan if device is None else plan.to(device)
 
     @classmethod
     def log(cls, num_buckets: int = 32, max_distance: int = 128, *, device: torch.device | str | None = None) -> "RelativeBuckets":
@@ -115,7 +116,10 @@ class RelativeBuckets:
         dev = torch.device(device)
         if dev == self.device:
             return self
-        return RelativeBuckets(self.num_buckets, self.radius, self.rows, self.cols, self.lut.to(dev), self.order.to(dev), self.start.to(dev))
+        moved = copy.copy(self)  # checked when it was made: not read back from the device again
+        for name in ("lut", "order", "start"):
+            object.__setattr__(moved, name, getattr(self, name).to(dev))
+        return moved
 
     def pairs(self, lq: int, lk: int, query_offset: int | torch.Tensor = 0) -> torch.Tensor:
         """Bucket of every pair, ``[lq, lk]`` (``[batch, lq, lk]`` for per-sample offsets): what the kernels look up."""
