@@ -15,7 +15,7 @@ namespace {
 // pass follows, for delta = dO . o has to match dP = dO V^T to 32 bits: the gradients of the table and of lam are sums
 // of p (dP - delta) in which everything but the error of delta cancels (with one fragment they were 1e-3 off).
 // Measured: 256 boards of 120 cells, four heads, fp32 29 us; 4096 of them in bf16 without gradients 151 us (3.3 TB/s); 256 boards
-// of 252 cells, bf16, training 58 us; two sequences of 4095 tokens, eight 64-wide heads, bf16, training 184 us; one token of four
+// of 252 cells, bf16, training 58 us; two sequences of 4095 tokens, eight 64-wide heads, bf16, training 197 us; one token of four
 // sequences of up to 8190, 15 us (2.2 TB/s).  At two waves per SIMD the long ones wait: half of the wave cycles for LDS
 // reads and barriers, a third issue vector instructions, a fifth matrix instructions.  A second LDS buffer (one barrier per
 // tile instead of two) changed nothing.
@@ -25,9 +25,10 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncFor
   using Frag = typename O::Frag;
   constexpr int DV = D * M, DC = D / O::kDims, NV = DV / 16, NKB = 4 / O::kSub;
   constexpr int PK = O::row_pitch(D), PV = O::tr_pitch(DV), TK = O::kParts * kTile * PK;
-  // A sum per tile, joined to the long one together with the change of maximum: one rounding per 64 keys where the products would
-  // take twelve (2000 tokens: output 5e-7 off without, 2e-7 with; 2 to 5 % of the time).
-  constexpr bool TILE_SUMS = NT == 0 && std::is_same<T, Split>::value;
+  // Where 32 bits of the output count, a sum per tile, joined to the long one together with the change of maximum: one rounding per 64
+  // keys where the products would take twelve (fp32, 2000 tokens: output 5e-7 off without, 2e-7 with; bf16 training, 4095 tokens: the
+  // table's gradient 7 to 12e-7 off without, 5 to 8e-7 with, 190 -> 200 us).
+  constexpr bool TILE_SUMS = NT == 0 && (PL == 3 || std::is_same<T, Split>::value);
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   typename O::Lds* k_lds = reinterpret_cast<typename O::Lds*>(smem);
   typename O::Lds* v_lds = k_lds + M * TK;
