@@ -878,8 +878,9 @@ int launch_bwd(EncAttnArgs a, hipStream_t stream) {
   int rc = enc_lds(enc_attn_bwd_q_kernel<TQ, D, M, QS, BIAS, NT>, lds);
   if (rc) return rc;
   const int nqt = (a.Lq + 64 * QS - 1) / (64 * QS);
-  hipLaunchKernelGGL((enc_attn_bwd_q_kernel<TQ, D, M, QS, BIAS, NT>), dim3((unsigned)((a.B + a.q_chunk - 1) / a.q_chunk * a.H * nqt * a.q_splits)), dim3(256),
-                     lds, stream, a);
+  const long long groups = (long long)((a.B + a.q_chunk - 1) / a.q_chunk) * a.H * nqt * a.q_splits;
+  if (groups != a.q_groups) return -21;  // a host side built with other rules
+  hipLaunchKernelGGL((enc_attn_bwd_q_kernel<TQ, D, M, QS, BIAS, NT>), dim3((unsigned)groups), dim3(256), lds, stream, a);
   rc = hip_err(hipGetLastError());
   if (rc) return rc;
   // the key-owned pass of a board unrolls where no heads are shared

@@ -46,6 +46,7 @@ struct EncAttnArgs {
   int splits, chunk;      // forward: key ranges per query tile, samples a workgroup walks one after the other
   int q_splits, q_chunk;  // query-owned pass: the same
   int k_splits, k_chunk;  // key-owned pass: query ranges per key tile, samples
+  long long q_groups;     // workgroups of the query-owned pass that hist and dlam_part have room for: refused unless they are the launch's
   float scale;
 };
 

@@ -253,6 +253,7 @@ struct Attention : torch::autograd::Function<Attention> {
     plan(s.b, s.kv * nkt, board && s.h == s.kv ? 1 : s.h / s.kv * up(s.lq, atrihip::kTile), resident(a, atrihip::kEncKeys),
          s.b * s.kv * s.lk * (s.maps * s.d + s.dv), a.k_splits, a.k_chunk);
     const int64_t hm = s.h * s.maps, slots = 2 * c.radius + 1, per_head = up(s.b, a.q_chunk) * a.q_splits * nqt;
+    a.q_groups = per_head * s.h;
     a.shares = static_cast<int>(std::clamp<int64_t>(per_head / 16, 1, 64));
     const int64_t n_delta = up(s.maps * s.rows, 4) * 4, n_dq = a.q_splits > 1 ? a.q_splits * s.rows * s.maps * s.d : 0;
     const int64_t n_kv = a.k_splits > 1 ? a.k_splits * s.b * s.kv * s.lk * (s.maps * s.d + s.dv) : 0;
