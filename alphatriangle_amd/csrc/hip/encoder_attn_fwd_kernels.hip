@@ -11,9 +11,10 @@ namespace {
 // One 4-wave workgroup per (head, 64 QS queries, key split) and `chunk` samples, one after the other: the bias is laid out once
 // and the next sample's first tile loads while this one's last is multiplied.  A wave owns 16 QS queries and walks the key tiles with the
 // running maximum and sum of the softmax; per lane the sum is partial (its own keys) until the end.
-// PL bf16 fragments per probability: one for inference (rounded like the values it meets); three, all 24 bits, when a backward
-// pass follows, for delta = dO . o has to match dP = dO V^T to 32 bits: the gradients of the table and of lam are sums
-// of p (dP - delta) in which everything but the error of delta cancels (with one fragment they were 1e-3 off).
+// PL bf16 fragments per probability: two, 16 bits, for inference, so that the result's own rounding is the only one that counts (one
+// fragment: 2.1e-3 off where rounding alone leaves 1.66e-3); three, all 24 bits, when a backward pass follows, for
+// delta = dO . o has to match dP = dO V^T to 32 bits: the gradients of the table and of lam are sums of p (dP - delta) in which
+// everything but the error of delta cancels (with one fragment they were 1e-3 off).
 // Measured: 256 boards of 120 cells, four heads, fp32 29 us; 4096 of them in bf16 without gradients 151 us (3.3 TB/s); 256 boards
 // of 252 cells, bf16, training 58 us; two sequences of 4095 tokens, eight 64-wide heads, bf16, training 197 us; one token of four
 // sequences of up to 8190, 15 us (2.2 TB/s).  At two waves per SIMD the long ones wait: half of the wave cycles for LDS
@@ -448,9 +449,10 @@ int launch_fwd_planes(const EncAttnArgs& a, hipStream_t stream) {
 template <typename T, int D, int M, int QS, bool BIAS, int NT = 0>
 int launch_fwd(const EncAttnArgs& a, hipStream_t stream) {
   if constexpr (Ops<T>::kBf16) {
-    if (a.o32) return launch_fwd_planes<T, D, M, QS, BIAS, 3, NT>(a, stream);
+    return a.o32 ? launch_fwd_planes<T, D, M, QS, BIAS, 3, NT>(a, stream) : launch_fwd_planes<T, D, M, QS, BIAS, 2, NT>(a, stream);
+  } else {
+    return launch_fwd_planes<T, D, M, QS, BIAS, 1, NT>(a, stream);
   }
-  return launch_fwd_planes<T, D, M, QS, BIAS, 1, NT>(a, stream);
 }
 
 // T: bf16 rows, or Split; W: fp32 rows with the fp32 matrix instruction for two 64-wide maps, whose parts would fill the LDS.

@@ -552,3 +552,25 @@ def test_broadcast_keys_add_their_gradients():
     assert torch.equal(out, same)
     for x, y in zip(got, want):
         assert torch.equal(x, y.sum(0, keepdim=True))
+
+
+@pytest.mark.parametrize("dtype,maps,kind,lq,lk,h,kv,d,b", [
+    (torch.bfloat16, 1, (8, 15), 120, 120, 4, 4, 32, 64),
+    (torch.bfloat16, 1, (12, 21), 252, 252, 4, 4, 32, 16),
+    (torch.bfloat16, 2, (8, 15), 120, 120, 2, 2, 32, 32),
+    (torch.bfloat16, 1, 128, 700, 900, 4, 2, 64, 1),
+    (torch.bfloat16, 1, 128, 1, 4001, 8, 8, 64, 4),
+    (torch.bfloat16, 2, None, 300, 600, 2, 1, 64, 1),
+])
+def test_inference_rounds_once(dtype, maps, kind, lq, lk, h, kv, d, b):
+    """Without a backward pass to come the output is off by its own rounding.  Half a step of bf16 in an output, 2^-16 of every
+    probability (two bf16 parts), and 2^-20 for the 32-bit parts (scores below 16, the exponential, sums), each times |v|."""
+    from alphatriangle_amd.ops.attention import attention_reference
+
+    p = _plan(kind)
+    inp = _inputs(dtype, maps, b, lq, lk, h, kv, d, p)
+    out = _call(inp, p, None, 0).double()
+    w = {n: (x.double() if x is not None else None) for n, x in inp.items()}
+    size = attention_reference(w["q"], w["k"], w["v"].abs(), -w["lam"] if maps == 2 else None, w["table"], p, None, d**-0.5, 0)
+    ref = attention_reference(w["q"], w["k"], w["v"], w["lam"], w["table"], p, None, d**-0.5, 0)
+    assert float(((out - ref).abs() - U16 * ref.abs() - (2.0**-16 + 2.0**-20) * size).max()) <= 0
