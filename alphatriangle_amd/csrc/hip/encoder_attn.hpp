@@ -64,7 +64,7 @@ struct Ops<unsigned short> {
     const short4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 16 * pitch));
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
-  static __device__ __forceinline__ Frag acc_frag(const float4v* s) {  // probabilities and score gradients: rounded to bf16 like the operand they meet
+  static __device__ __forceinline__ Frag acc_frag(const float4v* s) {
     return pack_bf16x8(s[0][0], s[0][1], s[0][2], s[0][3], s[1][0], s[1][1], s[1][2], s[1][3]);
   }
   static __device__ __forceinline__ float4v mma(const Frag& a, const Frag& b, float4v c) {
@@ -221,6 +221,26 @@ struct Ops<Split> {
   }
   static __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) { Ops<float>::store4(p, a, b, c, d); }
 };
+
+// An accumulator as the B fragments of the product that follows, PL of them where one holds fewer bits (bf16), and that product,
+// smallest terms first.
+template <typename T, int PL>
+__device__ __forceinline__ void acc_parts(typename Ops<T>::Frag (&f)[PL], const float4v* s) {
+  float4v rest[Ops<T>::kSub];
+#pragma unroll
+  for (int u = 0; u < Ops<T>::kSub; ++u) rest[u] = s[u];
+#pragma unroll
+  for (int p = 0; p < PL; ++p) {
+    f[p] = Ops<T>::acc_frag(rest);
+    if (p + 1 < PL) Ops<T>::take(rest, f[p]);
+  }
+}
+template <typename T, int PL>
+__device__ __forceinline__ float4v mma_parts(const typename Ops<T>::Frag& a, const typename Ops<T>::Frag (&b)[PL], float4v c) {
+#pragma unroll
+  for (int p = PL - 1; p >= 0; --p) c = Ops<T>::mma(a, b[p], c);
+  return c;
+}
 
 // Consecutive logical workgroups on the same XCD (the hardware deals blockIdx out round robin over eight), so that the query
 // tiles of one (sample, head), and the heads that share keys, meet in one L2.

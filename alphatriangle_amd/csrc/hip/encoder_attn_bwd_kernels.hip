@@ -15,6 +15,10 @@ using namespace atrihip;
 namespace {
 
 __device__ const float kZeroRow[8] __attribute__((aligned(16))) = {};  // read in place of rows and columns that are not there
+// Fragments per probability and score gradient: two in bf16, 16 bits, so that a gradient's own rounding is the only one that counts
+// (with one: 2.4e-3 off where rounding alone leaves 1.66e-3).
+template <typename T>
+constexpr int grad_parts() { return Ops<T>::kBf16 ? 2 : 1; }
 constexpr int kDsPitch = kTile + 4;  // row pitch of a wave's 16 x 64 tile of dS on its way to the diagonal sums
 
 __device__ __forceinline__ void wave_lds_fence() {  // orders a wave's own LDS writes before its other lanes' reads
@@ -61,8 +65,8 @@ template <typename T, int D, int M, int QS, bool BIAS, int NT>
 __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncQueries)) void enc_attn_bwd_q_kernel(EncAttnArgs a) {
   using O = Ops<T>;
   using Frag = typename O::Frag;
-  constexpr int DV = D * M, DC = D / O::kDims, VC = DV / O::kDims, ND = D / 16, NKB = 4 / O::kSub;
-    constexpr bool TILE_SUMS = NT == 0 && std::is_same<T, Split>::value;  // as in the forward pass
+  constexpr int DV = D * M, DC = D / O::kDims, VC = DV / O::kDims, ND = D / 16, NKB = 4 / O::kSub, PL = grad_parts<T>();
+  constexpr bool TILE_SUMS = NT == 0 && std::is_same<T, Split>::value;  // as in the forward pass
   constexpr int PK = O::row_pitch(D), PV = O::row_pitch(DV), TK = O::kParts * kTile * PK;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   typename O::Lds* k_lds = reinterpret_cast<typename O::Lds*>(smem);
@@ -309,16 +313,16 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncQue
             }
 #pragma unroll
             for (int m = 0; m < M; ++m) {
-              Frag sf[QS];
+              Frag sf[QS][PL];
 #pragma unroll
-              for (int s = 0; s < QS; ++s) sf[s] = O::acc_frag(&ds[m][s][kb * O::kSub]);
+              for (int s = 0; s < QS; ++s) acc_parts<T>(sf[s], &ds[m][s][kb * O::kSub]);
 #pragma unroll
               for (int n = 0; n < ND; ++n) {
                 const Frag kf = O::tr_frag(k_lds + m * TK, PK, kb, n, l15, q4);
 #pragma unroll
                 for (int s = 0; s < QS; ++s) {
-                  if constexpr (TILE_SUMS) dq_tile[m][s][n] = O::mma(kf, sf[s], kb == 0 ? float4v{0.f, 0.f, 0.f, 0.f} : dq_tile[m][s][n]);
-                  else dq[m][s][n] = O::mma(kf, sf[s], dq[m][s][n]);
+                  if constexpr (TILE_SUMS) dq_tile[m][s][n] = mma_parts<T>(kf, sf[s], kb == 0 ? float4v{0.f, 0.f, 0.f, 0.f} : dq_tile[m][s][n]);
+                  else dq[m][s][n] = mma_parts<T>(kf, sf[s], dq[m][s][n]);
                 }
               }
             }
@@ -467,8 +471,8 @@ template <typename T, int D, int M, int KS, bool BIAS, int NT>
 __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, Ops<T>::kBf16, kEncKeys)) void enc_attn_bwd_k_kernel(EncAttnArgs a) {
   using O = Ops<T>;
   using Frag = typename O::Frag;
-  constexpr int DV = D * M, DC = D / O::kDims, VC = DV / O::kDims, ND = D / 16, NV = DV / 16, NKB = 4 / O::kSub;
-    constexpr bool TILE_SUMS = NT == 0 && std::is_same<T, Split>::value;  // as in the forward pass
+  constexpr int DV = D * M, DC = D / O::kDims, VC = DV / O::kDims, ND = D / 16, NV = DV / 16, NKB = 4 / O::kSub, PL = grad_parts<T>();
+  constexpr bool TILE_SUMS = NT == 0 && std::is_same<T, Split>::value;  // as in the forward pass
   constexpr int PQ = O::row_pitch(D), PG = O::row_pitch(DV), TQ = O::kParts * kTile * PQ;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   typename O::Lds* q_lds = reinterpret_cast<typename O::Lds*>(smem);
@@ -673,30 +677,30 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, Ops<T>::kBf16, kEncKey
             }
           }
         }
-        Frag pf[KS];
+        Frag pf[KS][PL];
 #pragma unroll
-        for (int s = 0; s < KS; ++s) pf[s] = O::acc_frag(pmix[s]);
+        for (int s = 0; s < KS; ++s) acc_parts<T>(pf[s], pmix[s]);
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
           const Frag gf = O::tr_frag(g_lds, PG, kb, n, l15, q4);
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
-            if constexpr (TILE_SUMS) dv[s][n] += O::mma(gf, pf[s], float4v{0.f, 0.f, 0.f, 0.f});
-            else dv[s][n] = O::mma(gf, pf[s], dv[s][n]);
+            if constexpr (TILE_SUMS) dv[s][n] += mma_parts<T>(gf, pf[s], float4v{0.f, 0.f, 0.f, 0.f});
+            else dv[s][n] = mma_parts<T>(gf, pf[s], dv[s][n]);
           }
         }
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-          Frag sf[KS];
+          Frag sf[KS][PL];
 #pragma unroll
-          for (int s = 0; s < KS; ++s) sf[s] = O::acc_frag(ds[m][s]);
+          for (int s = 0; s < KS; ++s) acc_parts<T>(sf[s], ds[m][s]);
 #pragma unroll
           for (int n = 0; n < ND; ++n) {
             const Frag qf = O::tr_frag(q_lds + m * TQ, PQ, kb, n, l15, q4);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-              if constexpr (TILE_SUMS) dk[m][s][n] += O::mma(qf, sf[s], float4v{0.f, 0.f, 0.f, 0.f});
-              else dk[m][s][n] = O::mma(qf, sf[s], dk[m][s][n]);
+              if constexpr (TILE_SUMS) dk[m][s][n] += mma_parts<T>(qf, sf[s], float4v{0.f, 0.f, 0.f, 0.f});
+              else dk[m][s][n] = mma_parts<T>(qf, sf[s], dk[m][s][n]);
             }
           }
         }

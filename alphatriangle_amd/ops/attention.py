@@ -8,8 +8,8 @@
 * Types: fp32 or bf16 ``q`` / ``k`` / ``v`` of one type; ``table`` and ``lam`` in any floating type (used in fp32, their gradients
   are summed in at least 32 bits).  fp32 products carry all 24 bits of their operands, most of them as three bf16 parts; in fp32 an
   infinity (or a value above 3.38e38) in a row that takes part makes the results it reaches NaN.
-* bf16 results are rounded once, when they are written: in between, probabilities meet the bf16 operands in 16 bits at least.
-  Where a backward pass is to come the output's probabilities carry 24 bits, so the last bit of some values may
+* bf16 results are rounded once, when they are written: in between, probabilities and score gradients meet the bf16 operands in 16 bits at
+  least.  Where a backward pass is to come the output's probabilities carry 24 bits, so the last bit of some values may
   differ from a call without one; in fp32 the two are equal.
 * Layouts: ``[batch, tokens, heads, dim]`` with any strides; a contiguous last dimension with 16-byte aligned rows is read in
   place, anything else is copied first.  Outputs and gradients follow the token / batch order of the tensor they belong to.

@@ -574,3 +574,47 @@ def test_inference_rounds_once(dtype, maps, kind, lq, lk, h, kv, d, b):
     size = attention_reference(w["q"], w["k"], w["v"].abs(), -w["lam"] if maps == 2 else None, w["table"], p, None, d**-0.5, 0)
     ref = attention_reference(w["q"], w["k"], w["v"], w["lam"], w["table"], p, None, d**-0.5, 0)
     assert float(((out - ref).abs() - U16 * ref.abs() - (2.0**-16 + 2.0**-20) * size).max()) <= 0
+
+
+@pytest.mark.parametrize("maps,kind,lq,lk,h,kv,d,b", [
+    (1, (8, 15), 120, 120, 4, 4, 32, 16),
+    (1, (12, 21), 252, 252, 2, 2, 32, 8),
+    (2, (8, 15), 120, 120, 2, 2, 32, 16),
+    (1, 128, 600, 700, 4, 2, 64, 1),
+    (1, 128, 200, 300, 2, 1, 128, 1),
+    (2, None, 300, 400, 2, 2, 64, 1),
+    (2, 64, 300, 400, 2, 1, 48, 1),
+])
+def test_bf16_gradients_round_once(maps, kind, lq, lk, h, kv, d, b):
+    """Half a step of bf16 in a gradient, 2^-16 of every probability and score gradient (two bf16 parts), and for the 32-bit parts
+    2^-20 of p and of p (|dO| |v| + |delta|), each times the rows they meet."""
+    p = _plan(kind)
+    inp = _inputs(torch.bfloat16, maps, b, lq, lk, h, kv, d, p)
+    t = {**inp, **{n: inp[n].clone().requires_grad_(True) for n in ("q", "k", "v")}}
+    got = dict(zip(("q", "k", "v"), torch.autograd.grad(_call(t, p, None, 0), [t[n] for n in ("q", "k", "v")], inp["dout"])))
+    group, scale = h // kv, d**-0.5
+    q = inp["q"].double().view(b, lq, h, maps, d).permute(0, 2, 3, 1, 4)  # [b, h, maps, lq, d]
+    k = inp["k"].double().view(b, lk, kv, maps, d).permute(0, 2, 3, 1, 4).repeat_interleave(group, 1)
+    v, do = inp["v"].double().transpose(1, 2).repeat_interleave(group, 1), inp["dout"].double().transpose(1, 2)
+    s = torch.matmul(q, k.transpose(-1, -2)) * scale
+    if p is not None:
+        s = s + inp["table"].double()[p.pairs(lq, lk)].view(lq, lk, h, maps).permute(2, 3, 0, 1)
+    prob = s.softmax(-1)
+    lam = torch.stack([torch.ones(h, device="cuda"), -inp["lam"]], 1).double().view(1, h, maps, 1, 1) if maps == 2 else 1.0
+    dp, size = (torch.matmul(x, y.transpose(-1, -2)).unsqueeze(2) for x, y in ((do, v), (do.abs(), v.abs())))
+    delta = (prob * dp).sum(-1, keepdim=True)
+    ds = lam * prob * (dp - delta)
+    off_ds = 2.0**-16 * ds.abs() + 2.0**-20 * abs(lam) * prob * (size + (prob * size).sum(-1, keepdim=True))
+    mixed, off_mixed = (lam * prob).sum(2), (2.0**-16 + 2.0**-20) * (abs(lam) * prob).sum(2)
+
+    def keys(x):  # noqa: ANN001, ANN202  [b, h, (maps,) lk, width] summed over the heads that share them
+        x = x.view(b, kv, group, -1, lk, x.shape[-1]).sum(2)
+        return x.permute(0, 3, 1, 2, 4).reshape(b, lk, -1, x.shape[-1])
+
+    want = {"q": (torch.matmul(ds, k), torch.matmul(off_ds, k.abs())), "k": (torch.matmul(ds.transpose(-1, -2), q), torch.matmul(off_ds.transpose(-1, -2), q.abs())),
+            "v": (torch.matmul(mixed.transpose(-1, -2), do), torch.matmul(off_mixed.transpose(-1, -2), do.abs()))}
+    for n, (ref, off) in want.items():
+        if n != "v":
+            ref, off = ref * scale, off * scale
+        ref, off = (x.permute(0, 3, 1, 2, 4).reshape(b, lq, h * maps, d) if n == "q" else keys(x) for x in (ref, off))
+        assert float(((got[n].double() - ref).abs() - U16 * ref.abs() - off).max()) <= 0, n
