@@ -865,19 +865,26 @@ int launch_bwd_k(const EncAttnArgs& a, hipStream_t stream) {
   return hip_err(hipGetLastError());
 }
 
+// LDS of the query-owned pass with `rows` rows of sums by position.
+template <typename TQ, int D, int M, bool BIAS, int NT>
+size_t lds_bwd_q(int slots, int rows) {
+  using O = Ops<TQ>;
+  const size_t tiles = sizeof(typename O::Lds) * (size_t)(O::kParts * kTile) * (M * O::row_pitch(D) + O::row_pitch(D * M)) + (NT ? NT : 1) * kTile * sizeof(int);
+  return tiles + (BIAS ? sizeof(float) * ((size_t)(M * slots + 3) / 4 * 4 + 4 * 16 * kDsPitch + (size_t)rows * M * slots) : 0);
+}
+
 // TQ: rows of the query-owned pass
 template <typename TQ, typename T, int D, int M, bool BIAS, int NT = 0>
 int launch_bwd(EncAttnArgs a, hipStream_t stream) {
   using O = Ops<TQ>;
   constexpr int QS = enc_columns_of(D, M, NT, O::kBf16, kEncQueries);
-  const size_t slots = BIAS ? 2 * a.R + 1 : 0;
-  size_t lds = sizeof(typename O::Lds) * (size_t)(O::kParts * kTile) * (M * O::row_pitch(D) + O::row_pitch(D * M)) + (NT ? NT : 1) * kTile * sizeof(int);
-  if (BIAS) lds += sizeof(float) * ((M * slots + 3) / 4 * 4 + 4 * 16 * kDsPitch);
+  const int slots = BIAS ? 2 * a.R + 1 : 0;
   a.hist_rows = 4;
-  if (BIAS && a.hist) {
-    // a row of sums per wave; one for all where four rows would leave fewer workgroups per CU than the registers allow
-    if (lds + sizeof(float) * 4 * M * slots > kMaxLds / enc_waves(D, M, NT, QS, O::kBf16, kEncQueries)) a.hist_rows = 1;
-    lds += sizeof(float) * a.hist_rows * M * slots;
+  size_t lds = lds_bwd_q<TQ, D, M, BIAS, NT>(slots, BIAS && a.hist ? 4 : 0);
+  // a row of sums per wave; one for all where four rows would leave fewer workgroups per CU than the registers allow
+  if (BIAS && a.hist && lds > kMaxLds / enc_waves(D, M, NT, QS, O::kBf16, kEncQueries)) {
+    a.hist_rows = 1;
+    lds = lds_bwd_q<TQ, D, M, BIAS, NT>(slots, 1);
   }
   int rc = enc_lds(enc_attn_bwd_q_kernel<TQ, D, M, QS, BIAS, NT>, lds);
   if (rc) return rc;
@@ -916,9 +923,10 @@ int join_grads(const EncAttnArgs& a, hipStream_t stream) {
   return 0;
 }
 
-// T: bf16 rows, or Split; W: fp32 rows with the fp32 matrix instruction, where the parts would not fit: two 64-wide maps into LDS
-// (128-wide heads: 1081 us in parts, 1544 us without), the query-owned pass of a two-map board into registers (256 boards of
-// 120 cells: 84 us in parts, 70 us without).
+// T: bf16 rows, or Split; W: fp32 rows with the fp32 matrix instruction where three parts of the query-owned pass's tiles leave no
+// room for the table.  Parts otherwise: two 2000-token sequences of four two-map 64-wide heads, forward and backward,
+// 893 us and 3.1e-7 off, 1396 us and 7e-7 with the instruction; 16 boards of 400 cells 323 and 487 us; 256 boards of
+// 120 cells, two 32-wide maps, 178 and 182 us, dq 2.4e-7 and 3.8e-7 off.
 template <typename T, typename W>
 int dispatch_bwd(const EncAttnArgs& a, hipStream_t stream) {
   const int w = enc_width(a.D), nt = enc_board_tiles(a.table ? a.W : 0, a.Lk, a.D, a.M);
@@ -930,9 +938,11 @@ int dispatch_bwd(const EncAttnArgs& a, hipStream_t stream) {
     if (w == 64) return launch_bwd<T, T, 64, 1, true>(a, stream);
     return launch_bwd<T, T, 128, 1, true>(a, stream);
   }
-  if (nt == 2) return launch_bwd<W, T, 32, 2, true, 2>(a, stream);
+  if (nt == 2) return launch_bwd<T, T, 32, 2, true, 2>(a, stream);
   if (w == 32) return a.table ? launch_bwd<T, T, 32, 2, true>(a, stream) : launch_bwd<T, T, 32, 2, false>(a, stream);
-  return a.table ? launch_bwd<W, W, 64, 2, true>(a, stream) : launch_bwd<W, W, 64, 2, false>(a, stream);
+  if (!a.table) return launch_bwd<T, T, 64, 2, false>(a, stream);
+  const bool room = lds_bwd_q<T, 64, 2, true, 0>(2 * a.R + 1, 1) <= kMaxLds;  // up to 2416 positions; whether sums are wanted or not: same results
+  return room ? launch_bwd<T, T, 64, 2, true>(a, stream) : launch_bwd<W, T, 64, 2, true>(a, stream);
 }
 
 }  // namespace

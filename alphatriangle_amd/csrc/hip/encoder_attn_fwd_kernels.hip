@@ -29,7 +29,7 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncFor
   // Where 32 bits of the output count, a sum per tile, joined to the long one together with the change of maximum: one rounding per 64
   // keys where the products would take twelve (fp32, 2000 tokens: output 5e-7 off without, 2e-7 with; bf16 training, 4095 tokens: the
   // table's gradient 7 to 12e-7 off without, 5 to 8e-7 with, 190 -> 200 us).
-  constexpr bool TILE_SUMS = NT == 0 && (PL == 3 || std::is_same<T, Split>::value);
+  constexpr bool TILE_SUMS = NT == 0 && (PL == 3 || !O::kBf16);
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   typename O::Lds* k_lds = reinterpret_cast<typename O::Lds*>(smem);
   typename O::Lds* v_lds = k_lds + M * TK;
@@ -455,8 +455,8 @@ int launch_fwd(const EncAttnArgs& a, hipStream_t stream) {
   }
 }
 
-// T: bf16 rows, or Split; W: fp32 rows with the fp32 matrix instruction for two 64-wide maps, whose parts would fill the LDS.
-template <typename T, typename W>
+// T: bf16 rows, or Split
+template <typename T>
 int dispatch_fwd(const EncAttnArgs& a, hipStream_t stream) {
   const int w = enc_width(a.D), nt = enc_board_tiles(a.table ? a.W : 0, a.Lk, a.D, a.M);
   if (nt > 0 && a.splits > 1) return -18;
@@ -470,7 +470,7 @@ int dispatch_fwd(const EncAttnArgs& a, hipStream_t stream) {
   }
   if (nt == 2) return launch_fwd<T, 32, 2, 1, true, 2>(a, stream);
   if (w == 32) return a.table ? launch_fwd<T, 32, 2, 1, true>(a, stream) : launch_fwd<T, 32, 2, 1, false>(a, stream);
-  return a.table ? launch_fwd<W, 64, 2, 1, true>(a, stream) : launch_fwd<W, 64, 2, 1, false>(a, stream);
+  return a.table ? launch_fwd<T, 64, 2, 1, true>(a, stream) : launch_fwd<T, 64, 2, 1, false>(a, stream);
 }
 
 template <typename T, int M>
@@ -505,7 +505,7 @@ int atri_enc_attn_fwd(const EncAttnArgs* args, hipStream_t stream) {
     const int rc1 = hip_err(hipGetLastError());
     if (rc1) return rc1;
   }
-  const int rc2 = a.bf16 ? dispatch_fwd<unsigned short, unsigned short>(a, stream) : dispatch_fwd<Split, float>(a, stream);
+  const int rc2 = a.bf16 ? dispatch_fwd<unsigned short>(a, stream) : dispatch_fwd<Split>(a, stream);
   if (rc2 || a.splits == 1) return rc2;
   return a.bf16 ? join<unsigned short>(a, stream) : join<float>(a, stream);
 }

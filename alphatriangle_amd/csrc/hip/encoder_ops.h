@@ -76,9 +76,9 @@ inline int enc_columns(int W, int L, int Lk, int D, int M, bool bf16, int pass) 
 // Waves per SIMD the register allocation of a kernel leaves room for.  These kernels wait on LDS and on the matrix and
 // exponential pipes, so a second wave is worth some spilled registers (two 4095-token sequences in bf16, both backward
 // passes: 857 us with one, 466 us with two); a third is not, except where the kernel nearly fits anyway.  One where a
-// workgroup fills the LDS or keeps the sums of two maps.
+// workgroup's tiles take more than half of the LDS (three parts of 128 values, or of two maps of 64) or it keeps the sums of two maps.
 constexpr int enc_waves(int D, int M, int nt, int columns, bool bf16, int pass) {
-  if (!bf16 && D == 128) return 1;
+  if (!bf16 && D * M == 128) return 1;
   if (pass == kEncForward) return bf16 && (nt == 4 || (nt == 0 && M == 1 && D == 64 && columns == 2)) ? 3 : 2;
   return pass == kEncQueries && nt == 2 && M == 2 ? 1 : 2;
 }

@@ -618,3 +618,25 @@ def test_bf16_gradients_round_once(maps, kind, lq, lk, h, kv, d, b):
             ref, off = ref * scale, off * scale
         ref, off = (x.permute(0, 3, 1, 2, 4).reshape(b, lq, h * maps, d) if n == "q" else keys(x) for x in (ref, off))
         assert float(((got[n].double() - ref).abs() - U16 * ref.abs() - off).max()) <= 0, n
+
+
+@pytest.mark.parametrize("maps,kind,l,h,d,b", [(1, (8, 15), 120, 4, 32, 64), (2, (8, 15), 120, 2, 32, 64), (2, (20, 20), 400, 2, 64, 4), (2, 128, 300, 2, 40, 4),
+                                               (2, None, 2000, 2, 64, 1), (2, 128, 2000, 2, 64, 1)])
+def test_fp32_is_no_further_off_than_the_plain_form(maps, kind, l, h, d, b):  # noqa: E741
+    """Output and gradients against 64 bits: at most as far off as the same formulas in elementary fp32 operations."""
+    from alphatriangle_amd.ops.attention import attention_reference
+
+    p = _plan(kind)
+    inp = _inputs(torch.float32, maps, b, l, l, h, h, d, p)
+
+    def results(dtype, call):  # noqa: ANN001, ANN202
+        t = {n: (x.to(dtype).requires_grad_(n != "dout") if x is not None else None) for n, x in inp.items()}
+        out = call(t)
+        return [out, *torch.autograd.grad(out, [t[n] for n in ("q", "k", "v")], t["dout"])]
+
+    def plain(t):  # noqa: ANN001, ANN202
+        return attention_reference(t["q"], t["k"], t["v"], t["lam"], t["table"], p, None, d**-0.5, 0)
+
+    exact = results(torch.float64, plain)
+    for n, own, other, e in zip(("out", "q", "k", "v"), results(torch.float32, lambda t: _call(t, p, None, 0)), results(torch.float32, plain), exact):
+        assert _rel(own, e) <= _rel(other, e), (n, _rel(own, e), _rel(other, e))
