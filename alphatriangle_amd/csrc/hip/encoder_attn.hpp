@@ -411,13 +411,21 @@ inline int enc_check(const EncAttnArgs& a) {
 // The padded head width a kernel is built for.
 inline int enc_width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
-constexpr size_t kMaxLds = 160 * 1024;
+template <typename T>
+constexpr int enc_form() { return Ops<T>::kBf16 ? kRowsBf16 : Ops<T>::kParts == 3 ? kRowsParts : kRowsFp32; }
+// What a kernel lays out is what the shared rule counts.
+template <typename T, int D, int M, int PASS>
+constexpr bool enc_tiles_agree() {
+  using O = Ops<T>;
+  const int pitches = M * O::row_pitch(D) + (PASS == kEncForward ? O::tr_pitch(D * M) : O::row_pitch(D * M));
+  return enc_tile_bytes(enc_form<T>(), D, M, PASS) == (int)sizeof(typename O::Lds) * O::kParts * kTile * pitches;
+}
 
 // Raises a kernel's dynamic LDS limit (attribute of the function on the current device) and reports what does not fit.
 template <typename F>
-inline int enc_lds(F* fn, size_t bytes) {
+inline int enc_lds(F* fn, int bytes) {
   if (bytes > kMaxLds) return -20;
-  return hip_err(hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  return hip_err(hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
 }
 
 }  // namespace atrihip

@@ -19,7 +19,6 @@ __device__ const float kZeroRow[8] __attribute__((aligned(16))) = {};  // read i
 // (with one: 2.4e-3 off where rounding alone leaves 1.66e-3).
 template <typename T>
 constexpr int grad_parts() { return Ops<T>::kBf16 ? 2 : 1; }
-constexpr int kDsPitch = kTile + 4;  // row pitch of a wave's 16 x 64 tile of dS on its way to the diagonal sums
 
 __device__ __forceinline__ void wave_lds_fence() {  // orders a wave's own LDS writes before its other lanes' reads
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -853,10 +852,9 @@ __global__ __launch_bounds__(256) void enc_small_grads_kernel(SmallGrads a) {
 
 template <typename T, int D, int M, bool BIAS, int NT>
 int launch_bwd_k(const EncAttnArgs& a, hipStream_t stream) {
-  using O = Ops<T>;
   constexpr int KS = enc_columns_of(D, M, NT, Ops<T>::kBf16, kEncKeys);
-  const size_t lds = sizeof(typename O::Lds) * (size_t)(O::kParts * kTile) * (M * O::row_pitch(D) + O::row_pitch(D * M)) + (NT ? NT : 1) * kTile * sizeof(int) +
-                     sizeof(float) * (3 * M * kTile + 4 + (BIAS ? M * (2 * a.R + 1) : 0));
+  static_assert(enc_tiles_agree<T, D, M, kEncKeys>());
+  const int lds = enc_lds_bytes(enc_form<T>(), D, M, NT, kEncKeys, BIAS ? 2 * a.R + 1 : 0, 0);
   const int rc = enc_lds(enc_attn_bwd_k_kernel<T, D, M, KS, BIAS, NT>, lds);
   if (rc) return rc;
   const int nkt = (a.Lk + 64 * KS - 1) / (64 * KS);
@@ -865,27 +863,14 @@ int launch_bwd_k(const EncAttnArgs& a, hipStream_t stream) {
   return hip_err(hipGetLastError());
 }
 
-// LDS of the query-owned pass with `rows` rows of sums by position.
-template <typename TQ, int D, int M, bool BIAS, int NT>
-size_t lds_bwd_q(int slots, int rows) {
-  using O = Ops<TQ>;
-  const size_t tiles = sizeof(typename O::Lds) * (size_t)(O::kParts * kTile) * (M * O::row_pitch(D) + O::row_pitch(D * M)) + (NT ? NT : 1) * kTile * sizeof(int);
-  return tiles + (BIAS ? sizeof(float) * ((size_t)(M * slots + 3) / 4 * 4 + 4 * 16 * kDsPitch + (size_t)rows * M * slots) : 0);
-}
-
 // TQ: rows of the query-owned pass
 template <typename TQ, typename T, int D, int M, bool BIAS, int NT = 0>
 int launch_bwd(EncAttnArgs a, hipStream_t stream) {
-  using O = Ops<TQ>;
-  constexpr int QS = enc_columns_of(D, M, NT, O::kBf16, kEncQueries);
+  constexpr int QS = enc_columns_of(D, M, NT, Ops<TQ>::kBf16, kEncQueries);
+  static_assert(enc_tiles_agree<TQ, D, M, kEncQueries>());
   const int slots = BIAS ? 2 * a.R + 1 : 0;
-  a.hist_rows = 4;
-  size_t lds = lds_bwd_q<TQ, D, M, BIAS, NT>(slots, BIAS && a.hist ? 4 : 0);
-  // a row of sums per wave; one for all where four rows would leave fewer workgroups per CU than the registers allow
-  if (BIAS && a.hist && lds > kMaxLds / enc_waves(D, M, NT, QS, O::kBf16, kEncQueries)) {
-    a.hist_rows = 1;
-    lds = lds_bwd_q<TQ, D, M, BIAS, NT>(slots, 1);
-  }
+  a.hist_rows = enc_hist_rows(enc_form<TQ>(), D, M, NT, slots, enc_waves(D, M, NT, QS, Ops<TQ>::kBf16, kEncQueries));
+  const int lds = enc_lds_bytes(enc_form<TQ>(), D, M, NT, kEncQueries, slots, BIAS && a.hist ? a.hist_rows : 0);
   int rc = enc_lds(enc_attn_bwd_q_kernel<TQ, D, M, QS, BIAS, NT>, lds);
   if (rc) return rc;
   const int nqt = (a.Lq + 64 * QS - 1) / (64 * QS);
@@ -941,8 +926,8 @@ int dispatch_bwd(const EncAttnArgs& a, hipStream_t stream) {
   if (nt == 2) return launch_bwd<T, T, 32, 2, true, 2>(a, stream);
   if (w == 32) return a.table ? launch_bwd<T, T, 32, 2, true>(a, stream) : launch_bwd<T, T, 32, 2, false>(a, stream);
   if (!a.table) return launch_bwd<T, T, 64, 2, false>(a, stream);
-  const bool room = lds_bwd_q<T, 64, 2, true, 0>(2 * a.R + 1, 1) <= kMaxLds;  // up to 2416 positions; whether sums are wanted or not: same results
-  return room ? launch_bwd<T, T, 64, 2, true>(a, stream) : launch_bwd<W, T, 64, 2, true>(a, stream);
+  // whether sums are wanted or not: the same results
+  return enc_query_form(a.bf16 != 0, 64, 2, 2 * a.R + 1) == kRowsFp32 ? launch_bwd<W, T, 64, 2, true>(a, stream) : launch_bwd<T, T, 64, 2, true>(a, stream);
 }
 
 }  // namespace

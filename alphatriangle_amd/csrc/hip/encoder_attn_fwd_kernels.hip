@@ -435,9 +435,8 @@ __global__ __launch_bounds__(256) void key_words_kernel(const unsigned char* mas
 
 template <typename T, int D, int M, int QS, bool BIAS, int PL, int NT>
 int launch_fwd_planes(const EncAttnArgs& a, hipStream_t stream) {
-  using O = Ops<T>;
-  size_t lds = sizeof(typename O::Lds) * (size_t)(O::kParts * kTile) * (M * O::row_pitch(D) + O::tr_pitch(D * M)) + (NT ? NT : 1) * kTile * sizeof(int);
-  if (BIAS) lds += sizeof(float) * (size_t)M * (2 * a.R + 1);
+  static_assert(enc_tiles_agree<T, D, M, kEncForward>());
+  const int lds = enc_lds_bytes(enc_form<T>(), D, M, NT, kEncForward, BIAS ? 2 * a.R + 1 : 0, 0);
   const int rc = enc_lds(enc_attn_fwd_kernel<T, D, M, QS, BIAS, PL, NT>, lds);
   if (rc) return rc;
   const int nqt = (a.Lq + 64 * QS - 1) / (64 * QS);

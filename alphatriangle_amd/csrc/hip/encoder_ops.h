@@ -83,6 +83,33 @@ constexpr int enc_waves(int D, int M, int nt, int columns, bool bf16, int pass) 
   return pass == kEncQueries && nt == 2 && M == 2 ? 1 : 2;
 }
 
+// LDS of a workgroup.  Form of the staged rows: bf16, three bf16 parts of fp32, fp32.
+enum EncForm { kRowsBf16 = 0, kRowsParts = 1, kRowsFp32 = 2 };
+constexpr int kMaxLds = 160 * 1024;  // of a compute unit
+constexpr int kDsPitch = kTile + 4;  // row pitch of a wave's 16 x 64 tile of dS on its way to the sums by position
+constexpr int enc_row_bytes(int form, int width, bool transposed) {  // the paddings of Ops<T>::row_pitch and tr_pitch
+  return form == kRowsFp32 ? 4 * (width + 4) : (form == kRowsParts ? 6 : 2) * (width + (transposed ? 16 : 8));
+}
+constexpr int enc_tile_bytes(int form, int D, int M, int pass) { return kTile * (M * enc_row_bytes(form, D, false) + enc_row_bytes(form, D * M, pass == kEncForward)); }
+// slots: positions of the table (0: no bias); hist_rows: rows of sums by position (query-owned pass).
+constexpr int enc_lds_bytes(int form, int D, int M, int nt, int pass, int slots, int hist_rows) {
+  const int fixed = enc_tile_bytes(form, D, M, pass) + (nt ? nt : 1) * kTile * 4;
+  if (pass == kEncForward) return fixed + 4 * M * slots;
+  if (pass == kEncKeys) return fixed + 4 * (3 * M * kTile + 4 + M * slots);
+  return fixed + (slots ? 4 * ((M * slots + 3) / 4 * 4 + 4 * 16 * kDsPitch + hist_rows * M * slots) : 0);
+}
+// The query-owned pass of two 64-wide maps takes fp32 rows as they are where three parts leave no room for the table (more than 2416 positions).
+constexpr int enc_query_form(bool bf16, int D, int M, int slots) {
+  return bf16 ? kRowsBf16 : D == 64 && M == 2 && enc_lds_bytes(kRowsParts, D, M, 0, kEncQueries, slots, 1) > kMaxLds ? kRowsFp32 : kRowsParts;
+}
+constexpr int enc_per_cu(int waves, int lds) { return lds > kMaxLds ? 0 : kMaxLds / lds < waves ? kMaxLds / lds : waves; }
+// Rows of sums by position: one per wave; one for all, which the waves add to in turns, where four do not fit or would cost a
+// workgroup per compute unit.
+constexpr int enc_hist_rows(int form, int D, int M, int nt, int slots, int waves) {
+  const int four = enc_per_cu(waves, enc_lds_bytes(form, D, M, nt, kEncQueries, slots, 4));
+  return four > 0 && four >= enc_per_cu(waves, enc_lds_bytes(form, D, M, nt, kEncQueries, slots, 1)) ? 4 : 1;
+}
+
 // The residual joint: threads that own a row (8 values each) and threads of a workgroup.
 inline int lanes_of(int D) {
   int lanes = 16;

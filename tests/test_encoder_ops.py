@@ -3,6 +3,9 @@
 from __future__ import annotations
 
 import math
+import shutil
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -156,3 +159,37 @@ def test_plans_that_would_lead_outside_are_refused():
             RelativeBuckets(**{**fields, **change})
     board = RelativeBuckets.board(3, 4)
     assert board.radius == 2 * 7 + 3 and board.num_buckets == 5 * 7
+
+
+def _rules(tmp_path, body):  # noqa: ANN001, ANN202
+    """Lines of whitespace-separated numbers printed by a program over the rules the kernels and their host side share."""
+    if shutil.which("g++") is None:
+        pytest.skip("no host compiler")
+    header = Path(__file__).parent.parent / "alphatriangle_amd" / "csrc" / "hip" / "encoder_ops.h"
+    src = tmp_path / "rules.cpp"
+    src.write_text(f'#include "{header}"\n#include <cstdio>\n#include <initializer_list>\nusing namespace atrihip;\nint main() {{ {body} }}\n')
+    subprocess.check_call(["g++", "-std=c++17", "-O1", str(src), "-o", str(tmp_path / "rules")])
+    return [[int(x) for x in line.split()] for line in subprocess.check_output([str(tmp_path / "rules")], text=True).splitlines()]
+
+
+def test_sums_by_position_share_a_row_only_where_it_pays(tmp_path):
+    """One row of sums for all four waves (which then take turns) only where four rows do not fit or cost a workgroup per unit."""
+    rows = _rules(tmp_path, """
+      const int widths[5][2] = {{32, 1}, {64, 1}, {128, 1}, {32, 2}, {64, 2}};
+      for (auto& w : widths) for (int bf16 = 0; bf16 < 2; ++bf16) for (int slots : {1, 65, 257, 455, 1001, 2416, 2417, 4095}) {
+        const int form = enc_query_form(bf16, w[0], w[1], slots), waves = enc_waves(w[0], w[1], 0, enc_columns_of(w[0], w[1], 0, bf16, kEncQueries), bf16, kEncQueries);
+        const int rows = enc_hist_rows(form, w[0], w[1], 0, slots, waves);
+        std::printf("%d %d %d %d %d %d %d %d %d\\n", w[0], w[1], bf16, slots, form, waves, rows, enc_lds_bytes(form, w[0], w[1], 0, kEncQueries, slots, 1),
+                    enc_lds_bytes(form, w[0], w[1], 0, kEncQueries, slots, 4));
+      }""")
+    assert len(rows) == 80
+    chosen = {}
+    for width, maps, bf16, slots, form, waves, n, one, four in rows:
+        most = 160 * 1024
+        assert one <= most and (n == 1 or four <= most)
+        fits_one, fits_four = min(waves, most // one), min(waves, most // four)
+        assert n == (4 if fits_four == fits_one else 1)
+        assert form == (0 if bf16 else 2 if (width, maps) == (64, 2) and slots > 2416 else 1)
+        chosen[width, maps, bf16, slots] = n
+    assert chosen[64, 2, 0, 65] == chosen[64, 2, 0, 257] == chosen[32, 2, 0, 455] == chosen[64, 1, 0, 4095] == chosen[128, 1, 1, 4095] == 4
+    assert chosen[64, 2, 0, 4095] == chosen[64, 1, 0, 1001] == 1
