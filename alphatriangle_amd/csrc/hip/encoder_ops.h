@@ -109,6 +109,16 @@ constexpr int enc_hist_rows(int form, int D, int M, int nt, int slots, int waves
   const int four = enc_per_cu(waves, enc_lds_bytes(form, D, M, nt, kEncQueries, slots, 4));
   return four > 0 && four >= enc_per_cu(waves, enc_lds_bytes(form, D, M, nt, kEncQueries, slots, 1)) ? 4 : 1;
 }
+// Workgroups of a pass that a compute unit holds: as many as its registers and its LDS leave room for.  R: clamp of the position
+// difference (-1: no bias); own_heads: no shared key / value heads; sums: sums by position are wanted.
+inline int enc_workgroups(bool bf16, int D, int M, int R, int W, int Lq, int Lk, bool own_heads, int pass, bool sums) {
+  const int board = pass == kEncKeys && !own_heads ? 0 : W;  // shared heads take the general form of the key-owned pass
+  const int nt = enc_board_tiles(board, Lk, D, M), width = D <= 32 ? 32 : D <= 64 ? 64 : 128, slots = 2 * R + 1 > 0 ? 2 * R + 1 : 0;
+  const int waves = enc_waves(width, M, nt, enc_columns(board, Lq, Lk, D, M, bf16, pass), bf16, pass);
+  const int form = pass == kEncQueries ? enc_query_form(bf16, width, M, slots) : bf16 ? kRowsBf16 : kRowsParts;
+  const int n = enc_per_cu(waves, enc_lds_bytes(form, width, M, nt, pass, slots, sums && slots ? enc_hist_rows(form, width, M, nt, slots, waves) : 0));
+  return n > 0 ? n : 1;
+}
 
 // The residual joint: threads that own a row (8 values each) and threads of a workgroup.
 inline int lanes_of(int D) {

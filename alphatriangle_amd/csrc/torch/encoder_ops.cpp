@@ -114,11 +114,10 @@ void plan(int64_t samples, int64_t groups, int64_t steps, int64_t resident, int6
     if (cost(s) < 0.95 * best) best = cost(s), splits = static_cast<int>(s);
 }
 
-// Workgroups of one pass that the card's 256 compute units hold at a time (four waves each, one per SIMD).
-int64_t resident(const EncAttnArgs& a, int pass) {
-  const int nt = atrihip::enc_board_tiles(a.W, a.Lk, a.D, a.M);
-  const int width = a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128;
-  return 256 * atrihip::enc_waves(width, a.M, nt, atrihip::enc_columns(a.W, a.Lq, a.Lk, a.D, a.M, a.bf16 != 0, pass), a.bf16 != 0, pass);
+// Workgroups of one pass that the card's 256 compute units hold at a time (four waves each, one per SIMD); sums: with room for sums by position,
+// also where they are not wanted, so that gradients do not depend on that.
+int64_t resident(const EncAttnArgs& a, int pass, bool sums = false) {
+  return 256 * atrihip::enc_workgroups(a.bf16 != 0, a.D, a.M, a.table ? a.R : -1, a.W, a.Lq, a.Lk, a.H == a.KV, pass, sums);
 }
 
 struct Sizes {
@@ -249,7 +248,7 @@ struct Attention : torch::autograd::Function<Attention> {
     // shared heads take the general form of the key-owned pass
     const int64_t nkt = up(s.lk, 64 * atrihip::enc_columns(s.h == s.kv ? a.W : 0, a.Lq, a.Lk, a.D, a.M, a.bf16 != 0, atrihip::kEncKeys));
     const bool board = atrihip::enc_board_tiles(a.W, a.Lk, a.D, a.M) > 0;  // unrolled over its tiles: never split
-    plan(s.b, s.h * nqt, board ? 1 : up(s.lk, atrihip::kTile), resident(a, atrihip::kEncQueries), s.rows * s.maps * s.d, a.q_splits, a.q_chunk);
+    plan(s.b, s.h * nqt, board ? 1 : up(s.lk, atrihip::kTile), resident(a, atrihip::kEncQueries, table.defined()), s.rows * s.maps * s.d, a.q_splits, a.q_chunk);
     plan(s.b, s.kv * nkt, board && s.h == s.kv ? 1 : s.h / s.kv * up(s.lq, atrihip::kTile), resident(a, atrihip::kEncKeys),
          s.b * s.kv * s.lk * (s.maps * s.d + s.dv), a.k_splits, a.k_chunk);
     const int64_t hm = s.h * s.maps, slots = 2 * c.radius + 1, per_head = up(s.b, a.q_chunk) * a.q_splits * nqt;

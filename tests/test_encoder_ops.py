@@ -193,3 +193,25 @@ def test_sums_by_position_share_a_row_only_where_it_pays(tmp_path):
         chosen[width, maps, bf16, slots] = n
     assert chosen[64, 2, 0, 65] == chosen[64, 2, 0, 257] == chosen[32, 2, 0, 455] == chosen[64, 1, 0, 4095] == chosen[128, 1, 1, 4095] == 4
     assert chosen[64, 2, 0, 4095] == chosen[64, 1, 0, 1001] == 1
+
+
+def test_planned_workgroups_fit_a_compute_unit(tmp_path):
+    """What the launch planning counts as resident is what both the registers and the LDS of a unit hold."""
+    rows = _rules(tmp_path, """
+      for (int bf16 = 0; bf16 < 2; ++bf16) for (int maps = 1; maps < 3; ++maps) for (int d : {8, 32, 40, 64, 128}) {
+        if (maps == 2 && d > 64) continue;
+        for (int r : {-1, 0, 128, 500, 2047}) for (int pass = 0; pass < 3; ++pass) {
+          if (maps == 1 && r < 0) continue;
+          const int width = d <= 32 ? 32 : d <= 64 ? 64 : 128, slots = r < 0 ? 0 : 2 * r + 1;
+          const int form = pass == kEncQueries ? enc_query_form(bf16, width, maps, slots) : bf16 ? kRowsBf16 : kRowsParts;
+          const int waves = enc_waves(width, maps, 0, enc_columns(0, 4000, 4000, d, maps, bf16, pass), bf16, pass);
+          const int lds = enc_lds_bytes(form, width, maps, 0, pass, slots, slots ? enc_hist_rows(form, width, maps, 0, slots, waves) : 0);
+          std::printf("%d %d %d %d %d %d %d %d\\n", bf16, maps, d, r, pass, waves, lds, enc_workgroups(bf16, d, maps, r, 0, 4000, 4000, true, pass, true));
+        }
+      }""")
+    held = {}
+    for bf16, maps, d, r, which, waves, lds, n in rows:
+        assert n == min(waves, 160 * 1024 // lds) >= 1
+        held[bf16, maps, d, r, which] = n
+    assert held[0, 2, 40, 128, 1] == held[0, 1, 64, 2047, 1] == held[1, 1, 128, 2047, 1] == 1  # the LDS holds fewer than the registers
+    assert held[1, 1, 64, 128, 1] == held[0, 1, 32, 128, 1] == 2
