@@ -84,10 +84,10 @@ Tensor rows(const Tensor& given) {
   return aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
-// New [B, L, heads, width] in the type and the token / batch order of t.
+// New [B, L, heads, width] in the type and the token / batch order of t; no view, so that an output takes in-place operations.
 Tensor empty_rows(const Tensor& t, int64_t heads, int64_t width) {
   const int64_t b = t.size(0), n = t.size(1);
-  if (t.stride(0) < t.stride(1) && b > 1 && n > 1) return at::empty({n, b, heads, width}, t.options()).transpose(0, 1);
+  if (t.stride(0) < t.stride(1) && b > 1 && n > 1) return at::empty_strided({b, n, heads, width}, {heads * width, b * heads * width, width, 1}, t.options());
   return at::empty({b, n, heads, width}, t.options());
 }
 

@@ -640,3 +640,19 @@ def test_fp32_is_no_further_off_than_the_plain_form(maps, kind, l, h, d, b):  # 
     exact = results(torch.float64, plain)
     for n, own, other, e in zip(("out", "q", "k", "v"), results(torch.float32, lambda t: _call(t, p, None, 0)), results(torch.float32, plain), exact):
         assert _rel(own, e) <= _rel(other, e), (n, _rel(own, e), _rel(other, e))
+
+
+@pytest.mark.parametrize("maps", [1, 2])
+def test_outputs_take_in_place_operations(maps):
+    """In token order as in batch order; the gradients are those of the same operations out of place."""
+    p = _plan(16)
+    inp = _inputs(torch.bfloat16, maps, 3, 20, 20, 2, 2, 32, p)
+    for order in (lambda x: x, lambda x: x.transpose(0, 1).contiguous().transpose(0, 1)):
+        grads = []
+        for in_place in (False, True):
+            t = {**inp, **{n: order(inp[n]).detach().requires_grad_(True) for n in ("q", "k", "v")}}
+            out = _call(t, p, None, 0)
+            out = out.mul_(2).relu_() if in_place else out.mul(2).relu()
+            grads.append((out.detach(), *torch.autograd.grad(out, [t[n] for n in ("q", "k", "v")], inp["dout"])))
+        for x, y in zip(*grads):
+            assert torch.equal(x, y) and x.stride() == y.stride()
