@@ -4,6 +4,7 @@
 // before they get here; the kernel library's entry points are handed over as addresses (bind), so nothing here links HIP.
 #include <Python.h>
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -11,6 +12,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <map>
 #include <optional>
 #include <string>
@@ -42,6 +44,7 @@ void bind(const std::map<std::string, uintptr_t>& entries) {
 
 template <typename Fn, typename Args>
 void launch(Fn fn, const Args& args, const char* name, const Tensor& on) {
+  TORCH_CHECK(fn != nullptr && on.is_cuda(), name, " needs the kernel library and tensors on the GPU");
   const int rc = fn(&args, reinterpret_cast<ihipStream_t*>(c10::hip::getCurrentHIPStream(on.device().index()).stream()));
   TORCH_CHECK(rc == 0, name, " failed with code ", rc);
 }
@@ -54,6 +57,13 @@ Tensor param(const Tensor& t) {  // fp32, contiguous, on 16 bytes
   if (!t.defined()) return t;
   Tensor p = t.detach().to(at::kFloat).contiguous();
   return aligned(p) ? p : p.clone();
+}
+
+// The kernels compute values: a tangent would be lost without a word where no autograd node is made.
+void refuse_tangents(const char* name, std::initializer_list<const Tensor*> given) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : given)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), name, ": differentiable in reverse mode only, got a tensor with a forward-mode tangent");
 }
 
 // The gradients of a first-order node: usable as they are, an error when somebody differentiates them again.
@@ -292,6 +302,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::o
   c.radius = radius; c.cols = cols; c.buckets = buckets; c.q0 = q0; c.scale = scale;
   c.maps = lam.has_value() ? 2 : 1;
   const Tensor t = table.value_or(none), l = lam.value_or(none);
+  refuse_tangents("encoder attention", {&q, &k, &v, &t, &l});
   const bool grads = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (t.defined() && t.requires_grad()) ||
                                                     (l.defined() && l.requires_grad()));
   if (grads) return Attention::apply(q, k, v, table, lam, c);
@@ -393,6 +404,7 @@ struct GatedNormResidual : torch::autograd::Function<GatedNormResidual> {
 std::pair<Tensor, Tensor> gated_norm_residual(const Tensor& x, const Tensor& z, const Tensor& scale, const Tensor& post_w, const Tensor& post_b,
                                               const Tensor& pre_w, const Tensor& pre_b, const std::optional<Tensor>& gate_, double eps) {
   const Tensor gate = gate_.value_or(Tensor());
+  refuse_tangents("gated_norm_residual", {&x, &z, &scale, &post_w, &post_b, &pre_w, &pre_b, &gate});
   bool grads = false;
   for (const Tensor* t : {&x, &z, &scale, &post_w, &post_b, &pre_w, &pre_b, &gate}) grads = grads || (t->defined() && t->requires_grad());
   variable_list out;

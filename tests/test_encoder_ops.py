@@ -215,3 +215,37 @@ def test_planned_workgroups_fit_a_compute_unit(tmp_path):
         held[bf16, maps, d, r, which] = n
     assert held[0, 2, 40, 128, 1] == held[0, 1, 64, 2047, 1] == held[1, 1, 128, 2047, 1] == 1  # the LDS holds fewer than the registers
     assert held[1, 1, 64, 128, 1] == held[0, 1, 32, 128, 1] == 2
+
+
+def _kernels_host_side():  # noqa: ANN202
+    """The extension without kernels bound to it: what it refuses, it refuses before a launch."""
+    try:
+        import alphatriangle_amd._atri_torch as ops
+    except ImportError as exc:
+        pytest.skip(f"extension not built: {exc}")
+    return ops
+
+
+def _raw_calls(ops):  # noqa: ANN001, ANN202  name -> (call of one tensor list, the tensors)
+    q, table, lam = torch.randn(1, 4, 2, 8), torch.randn(8, 2), torch.rand(1)
+    p = RelativeBuckets.log(8, 5)
+    rows, row = torch.randn(3, 16), torch.randn(16)
+    return {
+        "relative": (lambda q, k, v, t: ops.attention(q, k, v, t, None, p.lut, p.order, p.start, p.radius, 0, 8, None, None, 0, 0.5), [q, q.clone(), q.clone(), table]),
+        "differential": (lambda q, k, v, m: ops.attention(q, k, v, None, m, None, None, None, 0, 0, 0, None, None, 0, 0.5), [q, q.clone(), torch.randn(1, 4, 1, 16), lam]),
+        "joint": (lambda x, z, g, *params: ops.gated_norm_residual(x, z, *params, g, 1e-5), [rows, rows.clone(), rows.clone(), *(row.clone() for _ in range(5))]),
+    }
+
+
+@pytest.mark.parametrize("name", ["relative", "differential", "joint"])
+def test_forward_mode_tangents_are_refused(name):
+    from torch.autograd import forward_ad
+
+    call, args = _raw_calls(_kernels_host_side())[name]
+    for i in range(len(args)):
+        for leaf in (False, True):
+            with forward_ad.dual_level():
+                given = list(args)
+                given[i] = forward_ad.make_dual(args[i].clone().requires_grad_(leaf), torch.ones_like(args[i]))
+                with pytest.raises(NotImplementedError, match="reverse mode"):
+                    call(*given)

@@ -656,3 +656,15 @@ def test_outputs_take_in_place_operations(maps):
             grads.append((out.detach(), *torch.autograd.grad(out, [t[n] for n in ("q", "k", "v")], inp["dout"])))
         for x, y in zip(*grads):
             assert torch.equal(x, y) and x.stride() == y.stride()
+
+
+def test_forward_mode_tangents_are_refused():
+    from torch.autograd import forward_ad
+
+    p = _plan(16)
+    inp = _inputs(torch.float32, 1, 1, 8, 8, 1, 1, 8, p)
+    with forward_ad.dual_level():
+        for n in ("q", "table"):
+            with pytest.raises(NotImplementedError, match="reverse mode"):
+                _call({**inp, n: forward_ad.make_dual(inp[n], torch.ones_like(inp[n]))}, p, None, 0)
+        _call(inp, p, None, 0)
