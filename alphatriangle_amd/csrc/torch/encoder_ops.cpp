@@ -6,9 +6,11 @@
 #include <ATen/ATen.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -59,8 +61,11 @@ Tensor param(const Tensor& t) {  // fp32, contiguous, on 16 bytes
   return aligned(p) ? p : p.clone();
 }
 
-// The kernels compute values: a tangent would be lost without a word where no autograd node is made.
-void refuse_tangents(const char* name, std::initializer_list<const Tensor*> given) {
+// The kernels compute values.  A tangent would be lost without a word where no autograd node is made, and a trace would record the
+// output's allocation and nothing else.
+void values_only(const char* name, std::initializer_list<const Tensor*> given) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(), name,
+              ": cannot be traced (torch.jit.trace, make_fx): its kernels are launched outside of PyTorch's operators");
   if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
   for (const Tensor* t : given)
     TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), name, ": differentiable in reverse mode only, got a tensor with a forward-mode tangent");
@@ -302,7 +307,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::o
   c.radius = radius; c.cols = cols; c.buckets = buckets; c.q0 = q0; c.scale = scale;
   c.maps = lam.has_value() ? 2 : 1;
   const Tensor t = table.value_or(none), l = lam.value_or(none);
-  refuse_tangents("encoder attention", {&q, &k, &v, &t, &l});
+  values_only("encoder attention", {&q, &k, &v, &t, &l});
   const bool grads = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (t.defined() && t.requires_grad()) ||
                                                     (l.defined() && l.requires_grad()));
   if (grads) return Attention::apply(q, k, v, table, lam, c);
@@ -404,7 +409,7 @@ struct GatedNormResidual : torch::autograd::Function<GatedNormResidual> {
 std::pair<Tensor, Tensor> gated_norm_residual(const Tensor& x, const Tensor& z, const Tensor& scale, const Tensor& post_w, const Tensor& post_b,
                                               const Tensor& pre_w, const Tensor& pre_b, const std::optional<Tensor>& gate_, double eps) {
   const Tensor gate = gate_.value_or(Tensor());
-  refuse_tangents("gated_norm_residual", {&x, &z, &scale, &post_w, &post_b, &pre_w, &pre_b, &gate});
+  values_only("gated_norm_residual", {&x, &z, &scale, &post_w, &post_b, &pre_w, &pre_b, &gate});
   bool grads = false;
   for (const Tensor* t : {&x, &z, &scale, &post_w, &post_b, &pre_w, &pre_b, &gate}) grads = grads || (t->defined() && t->requires_grad());
   variable_list out;

@@ -4,7 +4,7 @@
 ``relative_attention`` and ``differential_attention`` run the hand-written gfx950 kernels for CUDA tensors
 (csrc/hip/encoder_attn_*.hip; they raise when the kernel library is missing) and the elementary composition of the same formulas
 (:func:`attention_reference`) for host tensors.  Both are differentiable once, in reverse mode, in every tensor argument; on
-the GPU tensors that carry a forward-mode tangent are refused.
+the GPU they refuse tensors that carry a forward-mode tangent, and to be traced (``torch.jit.trace``, ``make_fx``).
 
 * Types: fp32 or bf16 ``q`` / ``k`` / ``v`` of one type; ``table`` and ``lam`` in any floating type (used in fp32, their gradients
   are summed in at least 32 bits).  fp32 products carry all 24 bits of their operands, most of them as three bf16 parts; in fp32 an

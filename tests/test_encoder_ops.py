@@ -249,3 +249,23 @@ def test_forward_mode_tangents_are_refused(name):
                 given[i] = forward_ad.make_dual(args[i].clone().requires_grad_(leaf), torch.ones_like(args[i]))
                 with pytest.raises(NotImplementedError, match="reverse mode"):
                     call(*given)
+
+
+@pytest.mark.parametrize("name", ["relative", "differential", "joint"])
+def test_tracing_is_refused(name):
+    """A trace would hold the output's allocation alone.  (The host path's elementary operations are traced as any.)"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    call, args = _raw_calls(_kernels_host_side())[name]
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(call, tuple(args), check_trace=False)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(call)(*args)
+
+
+def test_host_path_is_traced():
+    p = RelativeBuckets.log(8, 5)
+    q, t = torch.randn(1, 4, 2, 8), torch.randn(8, 2)
+    traced = torch.jit.trace(lambda a, b: relative_attention(a, a, a, b, p), (q, t), check_trace=False)
+    other = torch.randn(1, 4, 2, 8)
+    assert torch.allclose(traced(other, t), relative_attention(other, other, other, t, p), rtol=1e-5, atol=1e-6)

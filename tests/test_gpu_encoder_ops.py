@@ -668,3 +668,18 @@ def test_forward_mode_tangents_are_refused():
             with pytest.raises(NotImplementedError, match="reverse mode"):
                 _call({**inp, n: forward_ad.make_dual(inp[n], torch.ones_like(inp[n]))}, p, None, 0)
         _call(inp, p, None, 0)
+
+
+def test_tracing_is_refused():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    p = _plan(16)
+    inp = _inputs(torch.float32, 1, 1, 8, 8, 1, 1, 8, p)
+
+    def call(q):  # noqa: ANN001, ANN202
+        return _call({**inp, "q": q}, p, None, 0)
+
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(call, (inp["q"],), check_trace=False)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(call)(inp["q"])
