@@ -40,7 +40,8 @@ class RelativeBuckets:
     """Which bucket a (query, key) pair's relative position falls into; built once per model (:meth:`log`, :meth:`board`).
 
     ``lut[d + radius]`` is the bucket of position difference ``d = pos(key) - pos(query)``, clamped to ``+-radius``;
-    ``order`` / ``start`` list the differences of every bucket (the gradient's summation order)."""
+    ``order`` / ``start`` list the differences of every bucket (the gradient's summation order).  Without a ``device`` plans are
+    placed on the default one (on the host where that is ``meta``); :meth:`to` moves them."""
 
     num_buckets: int
     radius: int
@@ -63,7 +64,7 @@ class RelativeBuckets:
         ):
             raise ValueError(f"RelativeBuckets: lut and order are contiguous int32 [{n}], start [{self.num_buckets + 1}], on one device")
         lut, order, start = (t.cpu().long() for t in tables)
-        if int(lut.min()) < 0 or int(lut.max()) >= self.num_buckets or not torch.equal(order.sort().values, torch.arange(n)):
+        if int(lut.min()) < 0 or int(lut.max()) >= self.num_buckets or not torch.equal(order.sort().values, torch.arange(n, device="cpu")):
             raise ValueError("RelativeBuckets: lut names buckets, order every difference once")
         if not torch.equal(start[1:], torch.bincount(lut, minlength=self.num_buckets).cumsum(0)) or int(start[0]) != 0 or not torch.equal(
             lut[order], lut.sort().values
@@ -73,12 +74,13 @@ class RelativeBuckets:
     @classmethod
     def _make(cls, lut: torch.Tensor, num_buckets: int, radius: int, rows: int, cols: int, device: torch.device | str | None) -> "RelativeBuckets":
         n = lut.numel()
-        tables = torch.zeros(2 * n + num_buckets + 1, dtype=torch.int32)
+        tables = torch.zeros(2 * n + num_buckets + 1, dtype=torch.int32, device="cpu")
         tables[:n] = lut
         tables[n : 2 * n] = torch.argsort(lut, stable=True)
         tables[2 * n + 1 :] = torch.bincount(lut, minlength=num_buckets).cumsum(0)
         plan = cls(num_buckets, radius, rows, cols, tables[:n], tables[n : 2 * n], tables[2 * n :])
-        return plan if device is None else plan.to(device)
+        device = torch.get_default_device() if device is None else torch.device(device)
+        return plan if device.type == "meta" else plan.to(device)
 
     @classmethod
     def log(cls, num_buckets: int = 32, max_distance: int = 128, *, device: torch.device | str | None = None) -> "RelativeBuckets":
@@ -97,7 +99,7 @@ class RelativeBuckets:
                 n = min(half - 1, exact + math.floor(math.log(n / exact) / math.log(max_distance / exact) * (half - exact) + 1e-9))
             return n + (half if d > 0 else 0)
 
-        lut = torch.tensor([bucket(d) for d in range(-max_distance, max_distance + 1)], dtype=torch.int64)
+        lut = torch.tensor([bucket(d) for d in range(-max_distance, max_distance + 1)], dtype=torch.int64, device="cpu")
         return cls._make(lut, num_buckets, max_distance, 0, 0, device)
 
     @classmethod
@@ -110,7 +112,7 @@ class RelativeBuckets:
         if radius > MAX_RADIUS:
             raise ValueError(f"a {rows} x {cols} board has {2 * radius + 1} relative positions; at most {2 * MAX_RADIUS + 1} are supported")
         n = (2 * rows - 1) * (2 * cols - 1)
-        return cls._make(torch.arange(n, dtype=torch.int64), n, radius, rows, cols, device)
+        return cls._make(torch.arange(n, dtype=torch.int64, device="cpu"), n, radius, rows, cols, device)
 
     @property
     def device(self) -> torch.device:

@@ -269,3 +269,13 @@ def test_host_path_is_traced():
     traced = torch.jit.trace(lambda a, b: relative_attention(a, a, a, b, p), (q, t), check_trace=False)
     other = torch.randn(1, 4, 2, 8)
     assert torch.allclose(traced(other, t), relative_attention(other, other, other, t, p), rtol=1e-5, atol=1e-6)
+
+
+def test_plans_under_another_default_device():
+    """Their tables are values: made on the host, and held there where the default device holds none."""
+    want = RelativeBuckets.log(8, 5), RelativeBuckets.board(2, 3)
+    with torch.device("meta"):
+        got = RelativeBuckets.log(8, 5), RelativeBuckets.board(2, 3)
+    for a, b in zip(want, got):
+        assert a.device == b.device == torch.device("cpu")
+        assert all(torch.equal(getattr(a, n), getattr(b, n)) for n in ("lut", "order", "start"))
