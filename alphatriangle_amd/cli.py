@@ -127,6 +127,8 @@ def train(
     if attention is not None or encoder_norm is not None:
         from .config import ModelConfig
 
+        if not model_cfg.USE_TRANSFORMER or model_cfg.TRANSFORMER_LAYERS == 0:
+            raise typer.BadParameter(f"--attention / --encoder-norm: the network of preset {preset!r} has no encoder")
         chosen = {k: v for k, v in (("TRANSFORMER_ATTENTION", attention), ("TRANSFORMER_NORM", encoder_norm)) if v is not None}
         try:
             model_cfg = ModelConfig(**{**model_cfg.model_dump(), **chosen})

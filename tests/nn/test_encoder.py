@@ -196,3 +196,24 @@ def test_learner_steps_with_a_variant():
     torch.cuda.synchronize()
     moved = sum(not torch.equal(before[n], p) for n, p in net.model.named_parameters())
     assert moved >= 0.9 * len(before) and all(bool(torch.isfinite(p).all()) for p in net.model.parameters())
+
+
+def test_command_line_options_reach_the_model(monkeypatch):
+    from typer.testing import CliRunner
+
+    import alphatriangle_amd.training.runner as runner
+    from alphatriangle_amd.cli import app
+
+    given = {}
+    monkeypatch.setattr(runner, "run_training", lambda **kwargs: given.update(kwargs) or 0)
+    for options, want in ((["--attention", "relative"], ("relative", "pre")), (["--encoder-norm", "sandwich"], ("softmax", "sandwich")),
+                          (["--preset", "large", "--attention", "differential", "--encoder-norm", "sandwich"], ("differential", "sandwich"))):
+        given.clear()
+        out = CliRunner().invoke(app, ["train", *options])
+        mc = given["model_config_override"]
+        assert out.exit_code == 0 and (mc.TRANSFORMER_ATTENTION, mc.TRANSFORMER_NORM) == want
+    for options in (["--attention", "relative"], ["--encoder-norm", "sandwich"], ["--attention", "softmax"]):
+        for preset in ("tiny", "cnn"):
+            given.clear()
+            out = CliRunner().invoke(app, ["train", "--preset", preset, *options])
+            assert out.exit_code != 0 and not given and "encoder" in out.output
