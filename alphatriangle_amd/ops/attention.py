@@ -195,6 +195,8 @@ def _check(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: 
         raise ValueError(f"{name}: lam is one floating value per head, got {tuple(lam.shape)} {lam.dtype} for {hm // maps} heads")
     if (table is None) != (buckets is None):
         raise ValueError(f"{name}: table and buckets go together")
+    if table is None and lam is None:
+        raise ValueError(f"{name}: a table and its buckets are needed")
     if table is not None and buckets is not None:
         if tuple(table.shape) != (buckets.num_buckets, hm) or not table.is_floating_point():
             raise ValueError(f"{name}: table is a floating [{buckets.num_buckets}, {hm}], got {tuple(table.shape)} {table.dtype}")

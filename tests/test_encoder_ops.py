@@ -279,3 +279,9 @@ def test_plans_under_another_default_device():
     for a, b in zip(want, got):
         assert a.device == b.device == torch.device("cpu")
         assert all(torch.equal(getattr(a, n), getattr(b, n)) for n in ("lut", "order", "start"))
+
+
+def test_one_map_needs_its_bias():
+    q = torch.randn(1, 4, 2, 8)
+    with pytest.raises(ValueError, match="table"):
+        relative_attention(q, q, q, None, None)
