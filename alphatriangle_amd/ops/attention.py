@@ -209,6 +209,8 @@ def _check(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: 
             raise ValueError(f"{name}: query_offset is an int or an int32 [{b}], got {tuple(query_offset.shape)} {query_offset.dtype}")
         if buckets is not None and buckets.rows:
             raise ValueError(f"{name}: query_offset moves queries along a sequence, not on a board")
+    elif isinstance(query_offset, bool) or not hasattr(query_offset, "__index__"):
+        raise ValueError(f"{name}: query_offset is an int or an int32 [{b}], got {query_offset!r}")
     elif query_offset and buckets is not None and buckets.rows:
         raise ValueError(f"{name}: query_offset moves queries along a sequence, not on a board")
     elif abs(int(query_offset)) > MAX_OFFSET:

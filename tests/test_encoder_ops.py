@@ -285,3 +285,10 @@ def test_one_map_needs_its_bias():
     q = torch.randn(1, 4, 2, 8)
     with pytest.raises(ValueError, match="table"):
         relative_attention(q, q, q, None, None)
+
+
+@pytest.mark.parametrize("offset", [1.5, 2.0, True, None, "1", [1, 2]])
+def test_offsets_are_whole_numbers(offset):
+    q, p = torch.randn(2, 4, 2, 8), RelativeBuckets.log(8, 5)
+    with pytest.raises(ValueError, match="query_offset"):
+        relative_attention(q, q, q, torch.randn(8, 2), p, query_offset=offset)
