@@ -32,6 +32,7 @@ import torch
 from .. import native
 
 MAX_RADIUS = 2047     # largest position difference the kernels keep apart
+MIN_SCALE = 1e-30     # the kernels hold the bias in units of 1 / scale, which has to stay a finite number
 MAX_OFFSET = 1 << 29  # positions beyond this would let differences leave 32 bits
 
 
@@ -227,8 +228,8 @@ def _attend(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: t
             buckets: RelativeBuckets | None, key_mask: torch.Tensor | None, scale: float | None, query_offset: int | torch.Tensor) -> torch.Tensor:
     _check(name, q, k, v, table, lam, buckets, key_mask, query_offset)
     scale = q.shape[3] ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < 1e30:
-        raise ValueError(f"{name}: scale is a positive number, got {scale}")
+    if not MIN_SCALE <= scale < 1e30:
+        raise ValueError(f"{name}: scale is in [{MIN_SCALE}, 1e30), got {scale}")
     if not q.is_cuda or q.numel() == 0 or k.numel() == 0:
         return attention_reference(q, k, v, lam, table, buckets, key_mask, scale, query_offset)
     qoff = None
@@ -256,7 +257,8 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     """``softmax(scale q k^T + table[bucket(pos(key) - pos(query))]) v`` -> ``[B, Lq, H, D]``.
 
     ``q [B, Lq, H, D]``, ``k`` / ``v [B, Lk, KV, D]`` (``KV`` divides ``H``), ``D`` a multiple of 8 up to 128;
-    ``table [buckets.num_buckets, H]`` is learned.  ``scale`` defaults to ``D ** -0.5``.  For sequences query ``i`` stands at
+    ``table [buckets.num_buckets, H]`` is learned; values beyond ``3.4e38 scale`` count as that (-inf takes a pair out).  ``scale``
+    defaults to ``D ** -0.5``.  For sequences query ``i`` stands at
     position ``query_offset + i`` (an int, or an int32 ``[B]`` tensor: a new token behind each sample's own cache) and
     key ``j`` at ``j`` (without a bias positions have no effect); boards take all their cells as queries and keys.
     """

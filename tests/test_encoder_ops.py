@@ -292,3 +292,11 @@ def test_offsets_are_whole_numbers(offset):
     q, p = torch.randn(2, 4, 2, 8), RelativeBuckets.log(8, 5)
     with pytest.raises(ValueError, match="query_offset"):
         relative_attention(q, q, q, torch.randn(8, 2), p, query_offset=offset)
+
+
+@pytest.mark.parametrize("scale", [0.0, -1.0, 1e-38, 9e-31, 1e30, math.inf, math.nan])
+def test_scales_that_would_lose_the_bias_are_refused(scale):
+    q, t, p = torch.randn(1, 4, 2, 8), torch.randn(8, 2), RelativeBuckets.log(8, 5)
+    with pytest.raises(ValueError, match="scale"):
+        relative_attention(q, q, q, t, p, scale=scale)
+    relative_attention(q, q, q, t, p, scale=1e-30)

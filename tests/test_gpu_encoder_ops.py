@@ -694,3 +694,17 @@ def test_plans_under_a_gpu_default_device():
     for p, want in zip((*made, held), (RelativeBuckets.log(32, 16), RelativeBuckets.board(3, 5), RelativeBuckets.board(3, 5))):
         assert p.device.type == "cuda" and want.device.type == "cpu"
         assert all(torch.equal(getattr(p, n).cpu(), getattr(want, n)) for n in ("lut", "order", "start"))
+
+
+@pytest.mark.parametrize("maps", [1, 2])
+def test_smallest_scale_keeps_the_bias(maps):
+    """At a scale of 1e-30 products of queries and keys are nothing beside the bias, which the kernels hold 1e30 times as large."""
+    from alphatriangle_amd.ops.attention import attention_reference, differential_attention, relative_attention
+
+    p = _plan(16)
+    inp = _inputs(torch.float32, maps, 2, 40, 50, 2, 2, 32, p)
+    more = {"scale": 1e-30}
+    args = [inp["q"], inp["k"], inp["v"]]
+    out = relative_attention(*args, inp["table"], p, **more) if maps == 1 else differential_attention(*args, inp["lam"], inp["table"], p, **more)
+    ref = attention_reference(*(x.double() for x in args), inp["lam"].double() if maps == 2 else None, inp["table"].double(), p, None, 1e-30, 0)
+    assert _rel(out, ref) <= _tol(torch.float32, 32, 40, 50)
