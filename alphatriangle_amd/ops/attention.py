@@ -7,8 +7,9 @@
 the GPU they refuse tensors that carry a forward-mode tangent, and to be traced (``torch.jit.trace``, ``make_fx``).
 
 * Types: fp32 or bf16 ``q`` / ``k`` / ``v`` of one type; ``table`` and ``lam`` in any floating type (used in fp32, their gradients
-  are summed in at least 32 bits).  fp32 products carry all 24 bits of their operands, most of them as three bf16 parts; in fp32 an
-  infinity (or a value above 3.38e38) in a row that takes part makes the results it reaches NaN.
+  are summed in at least 32 bits).  fp32 products carry all 24 bits of their operands, most of them as three bf16 parts.
+* Infinities (in fp32 also values above 3.38e38) in rows that take part make the results they reach NaN, for an operand in several
+  parts meets them as inf - inf or 0 inf: in fp32 those of every tensor, in bf16 those of ``v`` and of the output's gradient.
 * bf16 results are rounded once, when they are written: in between, probabilities and score gradients meet the bf16 operands in 16 bits at
   least.  Where a backward pass is to come the output's probabilities carry 24 bits, so the last bit of some values may
   differ from a call without one; in fp32 the two are equal.

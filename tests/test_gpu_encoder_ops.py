@@ -708,3 +708,33 @@ def test_smallest_scale_keeps_the_bias(maps):
     out = relative_attention(*args, inp["table"], p, **more) if maps == 1 else differential_attention(*args, inp["lam"], inp["table"], p, **more)
     ref = attention_reference(*(x.double() for x in args), inp["lam"].double() if maps == 2 else None, inp["table"].double(), p, None, 1e-30, 0)
     assert _rel(out, ref) <= _tol(torch.float32, 32, 40, 50)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("maps,kind,l", [(1, (8, 15), 120), (1, 16, 90), (2, 16, 90)])
+def test_infinities_reach_their_column_only(dtype, maps, kind, l):  # noqa: E741
+    """An infinity in one value of ``v`` (or of the output's gradient) leaves every other column of the output (of ``v``'s gradient) as it is."""
+    p = _plan(kind)
+    inp = _inputs(dtype, maps, 2, l, l, 2, 2, 32, p)
+
+    def results(t, train):  # noqa: ANN001, ANN202
+        if not train:
+            return _call(t, p, None, 0), None
+        v = t["v"].clone().requires_grad_(True)
+        out = _call({**t, "v": v}, p, None, 0)
+        return out.detach(), torch.autograd.grad(out, v, t["dout"])[0]
+
+    for train in (False, True):
+        want, grad = results(inp, train)
+        v, dout = inp["v"].clone(), inp["dout"].clone()
+        v[1, 3, 1, 5] = math.inf
+        got, _ = results({**inp, "v": v}, train)
+        assert not bool(torch.isfinite(got[1, :, 1, 5]).any())
+        got[1, :, 1, 5] = want[1, :, 1, 5]
+        assert torch.equal(got, want)
+        if train:
+            dout[0, 7, 0, 9] = -math.inf
+            _, got = results({**inp, "dout": dout}, True)
+            assert not bool(torch.isfinite(got[0, :, 0, 9]).any())
+            got[0, :, 0, 9] = grad[0, :, 0, 9]
+            assert torch.equal(got, grad)
