@@ -879,6 +879,7 @@ int launch_bwd(EncAttnArgs a, hipStream_t stream) {
   hipLaunchKernelGGL((enc_attn_bwd_q_kernel<TQ, D, M, QS, BIAS, NT>), dim3((unsigned)groups), dim3(256), lds, stream, a);
   rc = hip_err(hipGetLastError());
   if (rc) return rc;
+  if (!a.dk) return 0;
   // the key-owned pass of a board unrolls where no heads are shared
   return NT > 0 && a.KV == a.H ? launch_bwd_k<T, D, M, BIAS, NT>(a, stream) : launch_bwd_k<T, D, M, BIAS, 0>(a, stream);
 }
@@ -899,7 +900,7 @@ int join_grads(const EncAttnArgs& a, hipStream_t stream) {
     const int rc = join_grad<T>(a, a.dq_part, a.q_splits, a.H, a.Lq, a.M * a.D, 0, a.M, a.D, a.dq, a.dqs, stream);
     if (rc) return rc;
   }
-  if (a.k_splits > 1) {
+  if (a.dk && a.k_splits > 1) {
     const int pitch = a.M * a.D + a.DV;
     const int rc = join_grad<T>(a, a.kv_part, a.k_splits, a.KV, a.Lk, pitch, 0, a.M, a.D, a.dk, a.dks, stream);
     if (rc) return rc;
@@ -934,13 +935,13 @@ int dispatch_bwd(const EncAttnArgs& a, hipStream_t stream) {
 
 extern "C" {
 
-// dq, dk, dv (every element written), delta and, where hist / dlam are set, the gradients of the table and of lam.
+// dq, dk and dv (every element written; both null: not wanted), delta and, where hist / dlam are set, the gradients of the table and of lam.
 int atri_enc_attn_bwd(const EncAttnArgs* args, hipStream_t stream) {
   if (!args) return -1;
   const EncAttnArgs& a = *args;
   int rc = enc_check(a);
   if (rc) return rc;
-  if (!a.q || !a.k || !a.v || !a.dout || !a.dq || !a.dk || !a.dv || !a.stat || !a.o32 || !a.delta) return -17;
+  if (!a.q || !a.k || !a.v || !a.dout || !a.dq || !a.dk != !a.dv || !a.stat || !a.o32 || !a.delta) return -17;
   const int slots = 2 * a.R + 1, hm = a.H * a.M;
   if (a.hist) {
     if (!a.table || !a.mid || !a.order || !a.start || !a.dtable) return -17;
@@ -949,7 +950,7 @@ int atri_enc_attn_bwd(const EncAttnArgs* args, hipStream_t stream) {
       return -15;
   }
   if (a.dlam && (a.M != 2 || !a.dlam_part)) return -14;
-  if ((a.q_splits > 1 && !a.dq_part) || (a.k_splits > 1 && !a.kv_part)) return -17;
+  if ((a.q_splits > 1 && !a.dq_part) || (a.dk && a.k_splits > 1 && !a.kv_part)) return -17;
   rc = a.bf16 ? dispatch_bwd<unsigned short, unsigned short>(a, stream) : dispatch_bwd<Split, float>(a, stream);
   if (rc) return rc;
   rc = a.bf16 ? join_grads<unsigned short>(a, stream) : join_grads<float>(a, stream);

@@ -244,9 +244,18 @@ struct Attention : torch::autograd::Function<Attention> {
     const Tensor dout = rows(grads[0].to(q.scalar_type()));
     const Sizes s = sizes(c, q, v, true, ints[5] != 0);
     EncAttnArgs a = base_args(c, s, q, k, v, table, lam);
-    Tensor dq = empty_rows(q, q.size(2), s.d), dk = empty_rows(k, k.size(2), s.d), dv = empty_rows(v, s.kv, s.dv);
-    a.dout = dout.data_ptr(); a.dq = dq.data_ptr(); a.dk = dk.data_ptr(); a.dv = dv.data_ptr();
-    strides(a.gs, dout); strides(a.dqs, dq); strides(a.dks, dk); strides(a.dvs, dv);
+    // edges: q, k, v, then the table and lam where they are given
+    const bool want_kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+    const bool want_table = table.defined() && ctx->needs_input_grad(3), want_lam = lam.defined() && ctx->needs_input_grad(table.defined() ? 4 : 3);
+    Tensor dq = empty_rows(q, q.size(2), s.d), dk, dv;
+    a.dout = dout.data_ptr(); a.dq = dq.data_ptr();
+    strides(a.gs, dout); strides(a.dqs, dq);
+    if (want_kv) {  // without them the key-owned pass is left out
+      dk = empty_rows(k, k.size(2), s.d);
+      dv = empty_rows(v, s.kv, s.dv);
+      a.dk = dk.data_ptr(); a.dv = dv.data_ptr();
+      strides(a.dks, dk); strides(a.dvs, dv);
+    }
     float* at_keep = f32(keep);
     if (s.n_words) a.words = reinterpret_cast<unsigned long long*>(at_keep);
     a.stat = at_keep + s.n_words;
@@ -257,8 +266,6 @@ struct Attention : torch::autograd::Function<Attention> {
     } else {
       a.o32 = a.stat + s.n_stat;
     }
-    // edges: q, k, v, then the table and lam where they are given
-    const bool want_table = table.defined() && ctx->needs_input_grad(3), want_lam = lam.defined() && ctx->needs_input_grad(table.defined() ? 4 : 3);
     const int64_t nqt = up(s.lq, 64 * atrihip::enc_columns(a.W, a.Lq, a.Lk, a.D, a.M, a.bf16 != 0, atrihip::kEncQueries));
     // shared heads take the general form of the key-owned pass
     const int64_t nkt = up(s.lk, 64 * atrihip::enc_columns(s.h == s.kv ? a.W : 0, a.Lq, a.Lk, a.D, a.M, a.bf16 != 0, atrihip::kEncKeys));
@@ -270,7 +277,7 @@ struct Attention : torch::autograd::Function<Attention> {
     a.q_groups = per_head * s.h;
     a.shares = static_cast<int>(std::clamp<int64_t>(per_head / 16, 1, 64));
     const int64_t n_delta = up(s.maps * s.rows, 4) * 4, n_dq = a.q_splits > 1 ? a.q_splits * s.rows * s.maps * s.d : 0;
-    const int64_t n_kv = a.k_splits > 1 ? a.k_splits * s.b * s.kv * s.lk * (s.maps * s.d + s.dv) : 0;
+    const int64_t n_kv = want_kv && a.k_splits > 1 ? a.k_splits * s.b * s.kv * s.lk * (s.maps * s.d + s.dv) : 0;
     const int64_t n_hist = want_table ? per_head * hm * slots : 0, n_mid = want_table ? a.shares * hm * slots : 0;
     const auto f = q.options().dtype(at::kFloat);
     const int64_t n_dlam = want_lam ? per_head * s.h * 4 : 0;

@@ -738,3 +738,25 @@ def test_infinities_reach_their_column_only(dtype, maps, kind, l):  # noqa: E741
             assert not bool(torch.isfinite(got[0, :, 0, 9]).any())
             got[0, :, 0, 9] = grad[0, :, 0, 9]
             assert torch.equal(got, grad)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("maps,kind,l,h,kv", [(1, (8, 15), 120, 2, 2), (1, 40, 700, 4, 2), (2, (8, 15), 120, 2, 2), (2, 40, 300, 2, 1), (2, None, 300, 2, 2)])
+def test_gradients_of_some_arguments(dtype, maps, kind, l, h, kv):  # noqa: E741
+    """Any subset of the arguments may be frozen: the other gradients keep their bits, and keys and values take no work where both are."""
+    p = _plan(kind)
+    inp = _inputs(dtype, maps, 2, l, l, h, kv, 32, p)
+    names = [n for n in ("q", "k", "v", "table", "lam") if inp[n] is not None]
+
+    def grads(wanted):  # noqa: ANN001, ANN202
+        t = {**inp, **{n: inp[n].clone().requires_grad_(n in wanted) for n in names}}
+        out = _call(t, p, None, 0)
+        node = out.grad_fn(inp["dout"])
+        assert (node[1] is None) == (node[2] is None) == (not {"k", "v"} & set(wanted))
+        return dict(zip(wanted, torch.autograd.grad(out, [t[n] for n in wanted], inp["dout"])))
+
+    every = grads(names)
+    for bits in range(1, 1 << len(names)):
+        wanted = [n for i, n in enumerate(names) if bits >> i & 1]
+        for n, g in grads(wanted).items():
+            assert torch.equal(g, every[n]), (wanted, n)
