@@ -217,3 +217,66 @@ def test_command_line_options_reach_the_model(monkeypatch):
             given.clear()
             out = CliRunner().invoke(app, ["train", "--preset", preset, *options])
             assert out.exit_code != 0 and not given and "encoder" in out.output
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("attention,norm", VARIANTS)
+@pytest.mark.parametrize("bf16", [False, True])
+def test_learner_step_of_a_variant_is_captured(attention: str, norm: str, bf16: bool):
+    """The trainer's forward and backward pass is replayed from a graph that holds no memset node and reproduces the eager gradients."""
+    from alphatriangle_amd.config import TrainConfig
+    from alphatriangle_amd.models.network import NeuralNetwork
+    from alphatriangle_amd.rl.core.trainer import TensorBatch, Trainer
+
+    dev = torch.device("cuda")
+    env, mc = EnvConfig(), ModelConfig(TRANSFORMER_ATTENTION=attention, TRANSFORMER_NORM=norm)
+    tc = TrainConfig(DEVICE="cuda", BATCH_SIZE=32, MAX_TRAINING_STEPS=100, COMPILE_MODEL=True)
+    torch.manual_seed(3)
+    trainer = Trainer(NeuralNetwork(mc, env, tc, dev), tc, env, autocast_bf16=bf16)
+    gen = torch.Generator().manual_seed(5)
+    for _ in range(3):
+        policy = torch.rand(32, env.ACTION_DIM, generator=gen)
+        tb = TensorBatch(torch.randint(-1, 2, (32, 1, env.ROWS, env.COLS), generator=gen).float().to(dev),
+                         torch.rand(32, mc.OTHER_NN_INPUT_FEATURES_DIM, generator=gen).to(dev), (policy / policy.sum(1, keepdim=True)).to(dev),
+                         torch.empty(32).uniform_(-5, 5, generator=gen).to(dev), torch.ones(32, device=dev))
+        info, _ = trainer.train_step_tensors(tb)
+        torch.cuda.synchronize()
+    report = trainer.graph_report
+    assert trainer.use_graph and report["replayed"] and report["memset_nodes"] == 0 and report["max_rel_err"] <= 1e-3, report
+    assert bool(torch.isfinite(info["total_loss"])) and bool(torch.isfinite(trainer.flat.flat_param).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("attention,norm", [("relative", "pre"), ("differential", "sandwich")])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_self_play_with_a_variant(attention: str, norm: str, dtype: str):
+    """Games played on the device tree with leaves through the module (its encoder through the kernels), before and after the
+    learner hands over new weights; the leaf values are the module's on the host in 64 bits."""
+    from alphatriangle_amd.rl.self_play.gpu_actor import ModuleEvaluator
+    from tests.test_gpu_engine import _actor
+
+    mc = ModelConfig(TRANSFORMER_ATTENTION=attention, TRANSFORMER_NORM=norm)
+    actor, replay, _ = _actor(games=24, sims=8, dtype=dtype, model=mc)
+    assert actor.nn.engine is None and isinstance(actor.evaluator, ModuleEvaluator)
+    for step in range(4):
+        rep = actor.play_move()
+        assert rep.moves == actor.G and rep.simulations >= actor.G * 8
+        if step == 1:
+            _randomise(actor.nn._orig_model)
+            actor.sync_weights(1)
+    n = len(replay)
+    assert n > 0 and bool(torch.isfinite(replay.ret[:n]).all())
+    assert torch.allclose(replay.policy[:n].sum(1), torch.ones(n, device=replay.policy.device), atol=1e-4)
+    ev = actor.evaluator
+    env = actor.nn.env_config
+    gen = torch.Generator().manual_seed(1)
+    grid, other = torch.randint(-1, 2, (24, env.ROWS * env.COLS), generator=gen).float(), torch.rand(24, mc.OTHER_NN_INPUT_FEATURES_DIM, generator=gen)
+    ev.forward(grid.cuda(), other.cuda())
+    host = AlphaTriangleNet(mc, env).double().eval()
+    host.load_state_dict(actor.nn._orig_model.state_dict())
+    with torch.no_grad():
+        want = host(grid.double().view(24, 1, env.ROWS, env.COLS), other.double())[0]
+    got = ev.logits[:24, : want.shape[1]].double().cpu()
+    # bf16: about forty operands and results of the chain rounded to 2^-9 rms at most, sqrt(40) 2^-9 = 1.2e-2; fp32: library convolutions
+    # and linear layers of 16 bits per operand, sqrt(40) 2^-17 = 5e-5; four times either for ReLUs and normalisations
+    assert float((got - want).norm() / want.norm()) <= (5e-2 if dtype == "bf16" else 2e-4)
