@@ -7,9 +7,11 @@
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -69,6 +71,22 @@ void values_only(const char* name, std::initializer_list<const Tensor*> given) {
   if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
   for (const Tensor* t : given)
     TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), name, ": differentiable in reverse mode only, got a tensor with a forward-mode tangent");
+}
+
+// A leaf's gradient accumulator runs on the stream it was made on, and lives as long as a graph of that leaf does.  A captured backward
+// pass would reach out to it, which on the default stream breaks the capture (and ends the process): refused while nothing is
+// recorded yet.
+void refuse_capture_beside_eager_graph(const char* name, std::initializer_list<const Tensor*> given) {
+  const c10::DeviceGuard guard((*given.begin())->device());
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const Tensor* t : given) {
+    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = accumulator ? accumulator->stream() : std::nullopt;
+    TORCH_CHECK(!stream || stream->id() != c10::hip::getDefaultHIPStream(t->device().index()).id(), name,
+                ": an eager graph of one of these leaves lives, made on the default stream; a backward pass captured now would run on that stream too: drop the eager "
+                "graph's tensors before the capture, or capture a call on detached leaves");
+  }
 }
 
 // The gradients of a first-order node: usable as they are, an error when somebody differentiates them again.
@@ -317,6 +335,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::o
   values_only("encoder attention", {&q, &k, &v, &t, &l});
   const bool grads = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || (t.defined() && t.requires_grad()) ||
                                                     (l.defined() && l.requires_grad()));
+  if (grads) refuse_capture_beside_eager_graph("encoder attention", {&q, &k, &v, &t, &l});
   if (grads) return Attention::apply(q, k, v, table, lam, c);
   const c10::DeviceGuard guard(q.device());
   Tensor keep;
@@ -421,6 +440,7 @@ std::pair<Tensor, Tensor> gated_norm_residual(const Tensor& x, const Tensor& z, 
   for (const Tensor* t : {&x, &z, &scale, &post_w, &post_b, &pre_w, &pre_b, &gate}) grads = grads || (t->defined() && t->requires_grad());
   variable_list out;
   if (grads && at::GradMode::is_enabled()) {
+    refuse_capture_beside_eager_graph("gated_norm_residual", {&x, &z, &scale, &post_w, &post_b, &pre_w, &pre_b, &gate});
     out = GatedNormResidual::apply(x, z, scale, post_w, post_b, pre_w, pre_b, gate_, eps);
   } else {
     const c10::DeviceGuard guard(x.device());

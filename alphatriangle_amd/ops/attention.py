@@ -19,6 +19,8 @@ the GPU they refuse tensors that carry a forward-mode tangent, and to be traced 
 * Masks: ``key_mask[b, j] == False`` takes key ``j`` of sample ``b`` out whatever its rows hold (NaN included); a sample without
   keys gives zero outputs and zero gradients.
 * Results do not depend on the order in which workgroups run: no floating-point atomics.
+* Graphs: forward and backward passes can be captured.  A call that takes gradients is refused inside a capture while an eager graph of
+  one of its leaves lives that was made on the default stream.
 """
 
 from __future__ import annotations

@@ -760,3 +760,50 @@ def test_gradients_of_some_arguments(dtype, maps, kind, l, h, kv):  # noqa: E741
         wanted = [n for i, n in enumerate(names) if bits >> i & 1]
         for n, g in grads(wanted).items():
             assert torch.equal(g, every[n]), (wanted, n)
+
+
+@pytest.mark.parametrize("op", ["relative", "differential", "joint"])
+def test_capture_beside_an_eager_graph_of_the_same_leaves(op):
+    """Refused at the forward call, before the backward pass would reach out of the capture; without the eager graph, captured and
+    replayed on new values beside eager calls."""
+    from alphatriangle_amd.ops.residual import gated_norm_residual
+
+    if op == "joint":
+        g = torch.Generator(device="cuda").manual_seed(0)
+        leaves = [torch.randn(*s, generator=g, device="cuda").requires_grad_(True) for s in ((64, 40), (64, 40), (40,), (40,), (40,), (40,), (40,))]
+
+        def forward(*t):  # noqa: ANN002, ANN202
+            return gated_norm_residual(*t)[1]
+    else:
+        p = _plan((3, 5))
+        inp = _inputs(torch.float32, 1 if op == "relative" else 2, 3, 15, 15, 2, 2, 32, p)
+        names = [n for n in ("q", "k", "v", "table", "lam") if inp[n] is not None]
+        leaves = [inp[n].requires_grad_(True) for n in names]
+
+        def forward(*t):  # noqa: ANN002, ANN202
+            return _call({**inp, **dict(zip(names, t))}, p, None, 0)
+
+    eager = forward(*leaves)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph"), torch.cuda.graph(graph):
+        forward(*leaves)
+    torch.cuda.synchronize()
+    detached = torch.cuda.CUDAGraph()  # other leaves of the same values: nothing to reach out to
+    with torch.cuda.graph(detached):
+        again = [t.detach().requires_grad_(True) for t in leaves]
+        held = torch.autograd.grad(forward(*again).sum(), again)
+    del eager
+    own = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(own):
+        kept = torch.autograd.grad(forward(*leaves).sum(), leaves)
+    for seed in range(3):
+        with torch.no_grad():
+            for t in leaves:
+                t.add_(0.1 * (seed + 1))
+        detached.replay()
+        own.replay()
+        torch.cuda.synchronize()
+        want = torch.autograd.grad(forward(*leaves).sum(), leaves)
+        torch.cuda.synchronize()
+        for x, y, z in zip(held, kept, want):
+            assert torch.equal(x, z) and torch.equal(y, z)
