@@ -16,7 +16,8 @@ namespace {
 
 __device__ const float kZeroRow[8] __attribute__((aligned(16))) = {};  // read in place of rows and columns that are not there
 // Fragments per probability and score gradient: two in bf16, 16 bits, so that a gradient's own rounding is the only one that counts
-// (with one: 2.4e-3 off where rounding alone leaves 1.66e-3).
+// (with one: 2.4e-3 off where rounding alone leaves 1.66e-3; two 4095-token sequences, query- and key-owned pass: 210 and 230 us with one,
+// 241 and 289 us with two).
 template <typename T>
 constexpr int grad_parts() { return Ops<T>::kBf16 ? 2 : 1; }
 
@@ -58,8 +59,10 @@ __device__ __forceinline__ void add_tile(const EncAttnArgs& a, float* sums, cons
 }
 
 // One 4-wave workgroup per (head, 64 QS queries, key range) and q_chunk samples, one after the other.
-// Measured (sizes as in the forward pass): boards of 120 cells, fp32 44 us; 252 cells, bf16 63 us; 4095 tokens, bf16 209 us; bound
-// like the forward pass, with five LDS reads and 36 vector instructions per pair and lane in the fp32 form.
+// Measured (sizes as in the forward pass): boards of 120 cells, fp32 44 us; 252 cells, bf16 67 us; 4095 tokens, bf16 241 us; 2000
+// tokens, two maps, fp32 252 us; bound like the forward pass, with five LDS reads and 36 vector instructions per pair and lane in
+// the fp32 form.  K is read transposed from a tile at row_pitch, where two of eight rows share banks: two conflict cycles per LDS
+// instruction.
 template <typename T, int D, int M, int QS, bool BIAS, int NT>
 __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncQueries)) void enc_attn_bwd_q_kernel(EncAttnArgs a) {
   using O = Ops<T>;
@@ -464,8 +467,9 @@ __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncQue
 
 // One 4-wave workgroup per (key / value head, 64 KS keys, query range) and k_chunk samples; a wave owns 16 KS keys and walks the
 // query tiles of every query head that shares them.
-// Measured (same sizes): 53 us, 72 us and 232 us.  One pass over the pairs for all gradients would save two of seven products, but
-// needs dQ summed across workgroups (or a board's dS through LDS, as many reads as the products it saves).
+// Measured (same sizes): 53 us, 82 us, 289 us and 333 us; Q and dO are read transposed at row_pitch as K above.  One pass over the
+// pairs for all gradients would save two of seven products, but needs dQ summed across workgroups (or a board's dS through LDS, as
+// many reads as the products it saves).
 template <typename T, int D, int M, int KS, bool BIAS, int NT>
 __global__ __launch_bounds__(256, enc_waves(D, M, NT, KS, Ops<T>::kBf16, kEncKeys)) void enc_attn_bwd_k_kernel(EncAttnArgs a) {
   using O = Ops<T>;
@@ -911,7 +915,7 @@ int join_grads(const EncAttnArgs& a, hipStream_t stream) {
 
 // T: bf16 rows, or Split; W: fp32 rows with the fp32 matrix instruction where three parts of the query-owned pass's tiles leave no
 // room for the table.  Parts otherwise: two 2000-token sequences of four two-map 64-wide heads, forward and backward,
-// 893 us and 3.1e-7 off, 1396 us and 7e-7 with the instruction; 16 boards of 400 cells 323 and 487 us; 256 boards of
+// 812 us and 3.1e-7 off, 1396 us and 7e-7 with the instruction; 16 boards of 400 cells 323 and 487 us; 256 boards of
 // 120 cells, two 32-wide maps, 178 and 182 us, dq 2.4e-7 and 3.8e-7 off.
 template <typename T, typename W>
 int dispatch_bwd(const EncAttnArgs& a, hipStream_t stream) {

@@ -15,11 +15,11 @@ namespace {
 // fragment: 2.1e-3 off where rounding alone leaves 1.66e-3); three, all 24 bits, when a backward pass follows, for
 // delta = dO . o has to match dP = dO V^T to 32 bits: the gradients of the table and of lam are sums of p (dP - delta) in which
 // everything but the error of delta cancels (with one fragment they were 1e-3 off).
-// Measured: 256 boards of 120 cells, four heads, fp32 29 us; 4096 of them in bf16 without gradients 151 us (3.3 TB/s); 256 boards
-// of 252 cells, bf16, training 58 us; two sequences of 4095 tokens, eight 64-wide heads, bf16, training 197 us; one token of four
-// sequences of up to 8190, 15 us (2.2 TB/s).  At two waves per SIMD the long ones wait: half of the wave cycles for LDS
-// reads and barriers, a third issue vector instructions, a fifth matrix instructions.  A second LDS buffer (one barrier per
-// tile instead of two) changed nothing.
+// Measured: 256 boards of 120 cells, four heads, fp32 29 us; 4096 of them in bf16 without gradients 149 us (3.4 TB/s; 133 us with one
+// fragment); 256 boards of 252 cells, bf16, training 57 us; two sequences of 4095 tokens, eight 64-wide heads, bf16, training
+// 192 us; two of 2000 tokens, four two-map 64-wide heads, fp32 225 us; one token of four sequences of up to 8190, 17 us
+// (2.0 TB/s).  At two waves per SIMD the long ones wait: half of the wave cycles for LDS reads and barriers, a third issue vector
+// instructions, a fifth matrix instructions.  A second LDS buffer (one barrier per tile instead of two) changed nothing.
 template <typename T, int D, int M, int QS, bool BIAS, int PL, int NT>
 __global__ __launch_bounds__(256, enc_waves(D, M, NT, QS, Ops<T>::kBf16, kEncForward)) void enc_attn_fwd_kernel(EncAttnArgs a) {
   using O = Ops<T>;
