@@ -27,6 +27,7 @@ from __future__ import annotations
 
 import copy
 import math
+import operator
 from collections.abc import Callable
 from dataclasses import dataclass
 
@@ -177,6 +178,13 @@ def attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: 
 
 
 # ---------------------------------------------------------------------------------------------------------- operators
+def _whole(x: object) -> bool:
+    try:
+        return not isinstance(x, bool) and operator.index(x) is not None  # type: ignore[arg-type]
+    except TypeError:
+        return False
+
+
 def _check(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor | None, lam: torch.Tensor | None,
            buckets: RelativeBuckets | None, key_mask: torch.Tensor | None, query_offset: int | torch.Tensor) -> None:
     maps = 1 if lam is None else 2
@@ -213,7 +221,7 @@ def _check(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: 
             raise ValueError(f"{name}: query_offset is an int or an int32 [{b}], got {tuple(query_offset.shape)} {query_offset.dtype}")
         if buckets is not None and buckets.rows:
             raise ValueError(f"{name}: query_offset moves queries along a sequence, not on a board")
-    elif isinstance(query_offset, bool) or not hasattr(query_offset, "__index__"):
+    elif not _whole(query_offset):
         raise ValueError(f"{name}: query_offset is an int or an int32 [{b}], got {query_offset!r}")
     elif query_offset and buckets is not None and buckets.rows:
         raise ValueError(f"{name}: query_offset moves queries along a sequence, not on a board")

@@ -7,6 +7,7 @@ import shutil
 import subprocess
 from pathlib import Path
 
+import numpy
 import pytest
 import torch
 
@@ -287,11 +288,12 @@ def test_one_map_needs_its_bias():
         relative_attention(q, q, q, None, None)
 
 
-@pytest.mark.parametrize("offset", [1.5, 2.0, True, None, "1", [1, 2]])
+@pytest.mark.parametrize("offset", [1.5, 2.0, True, None, "1", [1, 2], numpy.array(1.5), numpy.float32(2)])
 def test_offsets_are_whole_numbers(offset):
     q, p = torch.randn(2, 4, 2, 8), RelativeBuckets.log(8, 5)
     with pytest.raises(ValueError, match="query_offset"):
         relative_attention(q, q, q, torch.randn(8, 2), p, query_offset=offset)
+    relative_attention(q, q, q, torch.randn(8, 2), p, query_offset=numpy.int64(3))
 
 
 @pytest.mark.parametrize("scale", [0.0, -1.0, 1e-38, 9e-31, 1e30, math.inf, math.nan])
