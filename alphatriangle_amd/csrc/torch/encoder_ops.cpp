@@ -74,8 +74,7 @@ void values_only(const char* name, std::initializer_list<const Tensor*> given) {
 }
 
 // A leaf's gradient accumulator runs on the stream it was made on, and lives as long as a graph of that leaf does.  A captured backward
-// pass would reach out to it, which on the default stream breaks the capture (and ends the process): refused while nothing is
-// recorded yet.
+// pass would reach out to it, and the default stream cannot be part of a capture: refused while nothing is recorded yet.
 void refuse_capture_beside_eager_graph(const char* name, std::initializer_list<const Tensor*> given) {
   const c10::DeviceGuard guard((*given.begin())->device());
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;

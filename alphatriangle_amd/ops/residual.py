@@ -4,8 +4,8 @@ and the norm in front of the next block, as one operator.
 ``gated_norm_residual`` runs the gfx950 kernels for CUDA tensors (csrc/hip/residual_norm_kernels.hip: one launch forward, two
 backward; it raises when the kernel library is missing) and the elementary composition (:func:`gated_norm_residual_reference`)
 for host tensors.  It is differentiable once, in reverse mode, in every tensor argument (on the GPU it refuses tensors that carry a
-forward-mode tangent, and to be traced by ``torch.jit.trace`` or ``make_fx``); parameter gradients are summed in 32 bits in a
-fixed order (no atomics).
+forward-mode tangent, to be traced by ``torch.jit.trace`` or ``make_fx``, and to be captured with gradients beside an eager
+graph of the same leaves); parameter gradients are summed in 32 bits in a fixed order (no atomics).
 """
 
 from __future__ import annotations
